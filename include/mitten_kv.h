@@ -14,6 +14,14 @@
  *   wire_export / wire_import  blocks to / from a checksummed byte payload
  *                     (offload to host or disk, handoff between pools)
  *
+ * For the linear-attention layers of a hybrid model it owns a pool of states
+ * beside the K/V, and for the step between layers it has the norm:
+ *
+ *   linear_extend     linear attention of ragged prompts, reading and writing states
+ *   linear_step       one token per sequence, the same recurrence
+ *   state_copy        copies of states between slots (fork, compaction)
+ *   add_rms_norm      residual + RMSNorm, output in the model's type or e4m3
+ *
  * Pool layout in HBM (design/rust-inference-engine-design.md:1380-1387):
  *   [num_layers][2 (K then V)][num_blocks][page_size][num_kv_heads][head_dim]
  * A slot id is block * page_size + offset_in_block.
@@ -449,6 +457,120 @@ MKV_API int mkv_qk_norm_rope_append(mkv_pool *pool, int32_t layer, const void *d
                                     const float *d_inv_freq, int32_t rotary_dim, float eps,
                                     const int32_t *d_positions, const int32_t *d_slot_mapping,
                                     int32_t num_tokens, void *d_q_out, uint32_t flags, void *stream);
+
+/* ---- linear-attention states ----------------------------------------------- */
+
+/* A linear-attention layer keeps one f32 matrix per value head and sequence
+ * in place of K/V rows (the DeltaNet variant of KVCacheState,
+ * inference-model-common/src/lib.rs:5-13). For one sequence and value head,
+ * with q and k of key head h / (num_v_heads / num_k_heads):
+ *   S_t = exp(g_t) S_{t-1} + k_t v_t^T,   o_t = scale * S_t^T q_t,
+ * g_t the log decay of token t and head h. A state pool holds the matrices of
+ * num_slots sequences in every linear layer:
+ *   [num_layers][num_slots][num_v_heads][k_dim][v_dim], f32.
+ * A slot is to a sequence what its page table is to the K/V pool; slots are
+ * handed out by the caller (KvCachePool of mitten_kv_host.h does). */
+typedef struct mkv_state_pool mkv_state_pool;
+
+typedef struct {
+  int32_t num_layers;   /* linear-attention layers */
+  int32_t num_k_heads;  /* heads of q and k */
+  int32_t num_v_heads;  /* heads of v, o and the state: a multiple of num_k_heads, at most 1024 */
+  int32_t k_dim;        /* 64, 128 or 256 */
+  int32_t v_dim;        /* 64, 128 or 256 */
+  int32_t dtype;        /* mkv_dtype of q, k, v and o; states are f32 */
+  int64_t num_slots;
+} mkv_state_desc;
+
+/* A source slot that holds no state: the sequence starts from zeros. (As an
+ * int32 of the device forms: -1.) */
+#define MKV_STATE_NONE 0xFFFFFFFFu
+
+/* linear_extend / linear_step flags. */
+enum {
+  MKV_LINEAR_HEAD_DECAY = 1u << 0 /* d_log_decay is [num_v_heads]: one decay per head, the same for every token */
+};
+
+/* Bytes of the states: 4*L*slots*Hv*Dk*Dv. */
+MKV_API int mkv_state_required_bytes(const mkv_state_desc *desc, uint64_t *out_bytes);
+/* Allocate the states on `device` (hipMalloc; contents uninitialised).
+ * MKV_ERR_OUT_OF_MEMORY if HBM cannot hold them. */
+MKV_API int mkv_state_pool_create(const mkv_state_desc *desc, int device, mkv_state_pool **out_pool);
+MKV_API int mkv_state_pool_destroy(mkv_state_pool *pool);
+MKV_API int mkv_state_pool_get_desc(const mkv_state_pool *pool, mkv_state_desc *out_desc);
+MKV_API int mkv_state_pool_buffer(const mkv_state_pool *pool, void **out_dev_ptr, uint64_t *out_bytes);
+/* As mkv_pool_check, for this pool's device error word. */
+MKV_API int mkv_state_pool_check(mkv_state_pool *pool, void *stream, uint32_t *out_bits);
+
+/* Copy whole slots, all layers: states[*][dst[i]] = states[*][src[i]]. One
+ * source may go to several destinations (a fork). The result is defined when
+ * destinations are distinct and no slot is both a source and a destination;
+ * the host form checks this (at most 65535 pairs). An id outside the pool is
+ * skipped and reported (MKV_DEVERR_COPY). */
+MKV_API int mkv_state_copy(mkv_state_pool *pool, const int32_t *d_src_slots, const int32_t *d_dst_slots,
+                           int32_t num_pairs, void *stream);
+MKV_API int mkv_state_copy_host(mkv_state_pool *pool, const uint32_t *h_src_slots, const uint32_t *h_dst_slots,
+                                int32_t num_pairs, void *stream);
+
+/* One token per sequence: sequence b's state is read from slot src[b] (zeros
+ * where that is MKV_STATE_NONE), moved on by row b of q, k, v and the decays,
+ * and written to slot dst[b]; o[b] is its output. src NULL: src = dst, in
+ * place. A source other than dst[b] is a fork: it stays as it is.
+ * d_q, d_k: [num_seqs][num_k_heads][k_dim]; d_v, d_o: [num_seqs][num_v_heads][v_dim];
+ * in the pool's dtype, 16-byte aligned, d_o overlapping none of the others.
+ * d_log_decay: f32 [num_seqs][num_v_heads] (or [num_v_heads] with
+ * MKV_LINEAR_HEAD_DECAY), usually <= 0; -inf forgets all before the token.
+ * All arithmetic is f32 with one rounding per output element.
+ * Destinations must be distinct and no sequence's source another's
+ * destination (checked by the host form). A slot outside the pool is
+ * reported (MKV_DEVERR_SLOT) and its sequence skipped. num_seqs at most 65535.
+ * The host form copies its slots before it returns; slots equal to the
+ * previous call's (same stream) are not uploaded again; it cannot be captured
+ * into a graph (refused), the device form can. */
+MKV_API int mkv_linear_step(mkv_state_pool *pool, int32_t layer, const void *d_q, const void *d_k, const void *d_v,
+                            const float *d_log_decay, void *d_o, const int32_t *d_src_slots,
+                            const int32_t *d_dst_slots, int32_t num_seqs, float scale, uint32_t flags, void *stream);
+MKV_API int mkv_linear_step_host(mkv_state_pool *pool, int32_t layer, const void *d_q, const void *d_k,
+                                 const void *d_v, const float *d_log_decay, void *d_o, const uint32_t *h_src_slots,
+                                 const uint32_t *h_dst_slots, int32_t num_seqs, float scale, uint32_t flags,
+                                 void *stream);
+
+/* A chunk of tokens per sequence: sequence b has the rows d_q_indptr[b] ..
+ * d_q_indptr[b+1] of q, k, v, the decays and o ([num_tokens] rows in all),
+ * and its state moves on by all of them; what mkv_linear_step does token by
+ * token. A chunk may be empty: the state after it is the one before it. Rows
+ * that no sequence has are left as they are. max_q_len sizes the launch (a
+ * longer chunk is computed all the same); an indptr that falls back or
+ * leaves [0, num_tokens] is reported (MKV_DEVERR_CTX) and its sequence
+ * skipped. Slots, types and forms as in mkv_linear_step. */
+MKV_API int mkv_linear_extend(mkv_state_pool *pool, int32_t layer, const void *d_q, const void *d_k, const void *d_v,
+                              const float *d_log_decay, void *d_o, const int32_t *d_q_indptr,
+                              const int32_t *d_src_slots, const int32_t *d_dst_slots, int32_t num_seqs,
+                              int32_t num_tokens, int32_t max_q_len, float scale, uint32_t flags, void *d_workspace,
+                              uint64_t workspace_bytes, void *stream);
+MKV_API int mkv_linear_extend_host(mkv_state_pool *pool, int32_t layer, const void *d_q, const void *d_k,
+                                   const void *d_v, const float *d_log_decay, void *d_o, const int32_t *h_q_lens,
+                                   const uint32_t *h_src_slots, const uint32_t *h_dst_slots, int32_t num_seqs,
+                                   float scale, uint32_t flags, void *stream);
+
+/* ---- the step between layers -------------------------------------------------- */
+
+/* For each row: r = x + residual (f32), y = r * (mean(r^2) + eps)^-1/2 * (1 + w).
+ * d_x, d_residual (NULL: none), d_sum (r, NULL: not wanted), d_out (y, NULL:
+ * not wanted): [num_rows][dim] in dtype; d_weight: f32 [dim]. d_fp8 (with
+ * d_scales; both or neither): y as OCP e4m3 [num_rows][dim] with f32 scales
+ * [num_rows][dim / group]; per group of `group` consecutive columns (0: the
+ * whole row), a = max(max |y|, 2^-100), scale = a / 448, and the byte stands
+ * for e4m3(y * (448 / a)) * scale. A NaN in a row reaches its outputs and
+ * scales. The norm is of the f32 sum (r itself is rounded only where it is
+ * stored), one rounding per output element. num_rows below 2^24; dim: a multiple of 8, at most
+ * 16384; group: a multiple of 8 that divides it. Device pointers 16-byte
+ * aligned (d_scales: 4). d_sum or d_out may be d_x or d_residual, in place.
+ * Replaces the residual add and RmsNorm::forward around a layer's blocks
+ * (inference-model-qwen/src/model.rs:84-109,348-365). */
+MKV_API int mkv_add_rms_norm(int device, const void *d_x, const void *d_residual, const float *d_weight, float eps,
+                             int32_t num_rows, int32_t dim, int32_t dtype, void *d_sum, void *d_out, void *d_fp8,
+                             float *d_scales, int32_t group, void *stream);
 
 /* ---- KV block wire format --------------------------------------------------- */
 

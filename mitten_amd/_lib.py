@@ -49,7 +49,20 @@ class WireHeaderC(ctypes.Structure):
     ]
 
 
+class StateDescC(ctypes.Structure):
+    _fields_ = [
+        ("num_layers", i32),
+        ("num_k_heads", i32),
+        ("num_v_heads", i32),
+        ("k_dim", i32),
+        ("v_dim", i32),
+        ("dtype", i32),
+        ("num_slots", i64),
+    ]
+
+
 DESC_P = ctypes.POINTER(PoolDescC)
+STATE_DESC_P = ctypes.POINTER(StateDescC)
 WIRE_P = ctypes.POINTER(WireHeaderC)
 I32P = ctypes.POINTER(i32)
 U32P = ctypes.POINTER(u32)
@@ -94,6 +107,19 @@ DEVICE_SIGNATURES = {
     "mkv_wire_import_host": (c_int, [P, U32P, i32, i32, i32, P, P, P, P]),
     "mkv_decode_plan_build_tables": (c_int, [P, I32P, U32P, U32P, i32, i32, P]),
     "mkv_decode_plan_build_shared_prefix": (c_int, [P, U32P, i32, I32P, U32P, U32P, i32, i32, P]),
+    "mkv_state_required_bytes": (c_int, [STATE_DESC_P, ctypes.POINTER(u64)]),
+    "mkv_state_pool_create": (c_int, [STATE_DESC_P, c_int, ctypes.POINTER(P)]),
+    "mkv_state_pool_destroy": (c_int, [P]),
+    "mkv_state_pool_get_desc": (c_int, [P, STATE_DESC_P]),
+    "mkv_state_pool_buffer": (c_int, [P, ctypes.POINTER(P), ctypes.POINTER(u64)]),
+    "mkv_state_pool_check": (c_int, [P, P, ctypes.POINTER(u32)]),
+    "mkv_state_copy": (c_int, [P, P, P, i32, P]),
+    "mkv_state_copy_host": (c_int, [P, U32P, U32P, i32, P]),
+    "mkv_linear_step": (c_int, [P, i32, P, P, P, P, P, P, P, i32, f32, u32, P]),
+    "mkv_linear_step_host": (c_int, [P, i32, P, P, P, P, P, U32P, U32P, i32, f32, u32, P]),
+    "mkv_linear_extend": (c_int, [P, i32, P, P, P, P, P, P, P, P, i32, i32, i32, f32, u32, P, u64, P]),
+    "mkv_linear_extend_host": (c_int, [P, i32, P, P, P, P, P, I32P, U32P, U32P, i32, f32, u32, P]),
+    "mkv_add_rms_norm": (c_int, [c_int, P, P, P, f32, i32, i32, i32, P, P, P, P, i32, P]),
     "mkv_validate_slots": (c_int, [DESC_P, I32P, i32]),
     "mkv_validate_block_tables": (c_int, [DESC_P, I32P, I32P, I32P, i32, i32]),
     "mkv_validate_copy_pairs": (c_int, [DESC_P, I32P, I32P, i32]),

@@ -50,7 +50,13 @@ struct StagedCache {
   std::vector<int32_t> vals;
 };
 
-struct Pool {
+// A pool's staging slots (KV pools and state pools each own one ring).
+struct MetaRing {
+  MetaSlot meta[kMetaSlots];
+  int meta_next = 0;
+};
+
+struct Pool : MetaRing {
   mkv_pool_desc desc;
   Geom g;
   int device = 0;
@@ -72,8 +78,6 @@ struct Pool {
   // Caller events recorded around the next decode attention kernel (one
   // shot; mkv_pool_set_launch_events).
   hipEvent_t ev_start = nullptr, ev_end = nullptr;
-  MetaSlot meta[kMetaSlots];
-  int meta_next = 0;
   // The last host arrays staged by the append, gather, extend and fused prep
   // entry points (an engine step passes the same ones to every layer), and a
   // scratch array to assemble a staged array in.
@@ -84,15 +88,15 @@ struct Pool {
 // Next staging slot with room for n int32 values (waits for its previous
 // readers, grows it when needed). Fill s->h[0..n), then meta_upload, launch,
 // meta_release.
-int meta_acquire(Pool *p, size_t n, hipStream_t hs, MetaSlot **out);
+int meta_acquire(MetaRing *p, size_t n, hipStream_t hs, MetaSlot **out);
 int meta_upload(MetaSlot *s, size_t n, hipStream_t hs);
 int meta_release(MetaSlot *s, hipStream_t hs);
-void meta_free(Pool *p);
+void meta_free(MetaRing *p);
 // meta_acquire + fill + meta_upload of h[0..n), unless the cache's last
 // array equals it, was uploaded on the same stream, and its slot has not
 // been claimed since: then that device copy is handed out again. Either
 // way the caller launches from (*out)->d and calls meta_release.
-int stage_cached(Pool *p, StagedCache &c, const int32_t *h, size_t n, hipStream_t hs, MetaSlot **out);
+int stage_cached(MetaRing *p, StagedCache &c, const int32_t *h, size_t n, hipStream_t hs, MetaSlot **out);
 
 // Looks up this device's address of the static scratch of
 // mkv_decode_attention_static (once per device; called by mkv_pool_create).

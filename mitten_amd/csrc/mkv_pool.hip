@@ -223,7 +223,7 @@ copy_blocks_kernel(uint8_t *__restrict__ pool, const int32_t *__restrict__ src,
 
 // ---- host metadata staging ----------------------------------------------------------
 
-int meta_acquire(Pool *p, size_t n, hipStream_t hs, MetaSlot **out) {
+int meta_acquire(MetaRing *p, size_t n, hipStream_t hs, MetaSlot **out) {
   MetaSlot *sl = &p->meta[p->meta_next];
   p->meta_next = (p->meta_next + 1) % kMetaSlots;
   // The slot's event only tells the host that the launches reading the
@@ -270,7 +270,7 @@ int meta_release(MetaSlot *sl, hipStream_t hs) {
   return MKV_OK;
 }
 
-void meta_free(Pool *p) {
+void meta_free(MetaRing *p) {
   for (MetaSlot &sl : p->meta) {
     if (sl.h) (void)hipHostFree(sl.h);
     if (sl.d) (void)hipFree(sl.d);
@@ -544,7 +544,7 @@ extern "C" int mkv_copy_blocks(mkv_pool *pool, const int32_t *d_src_blocks,
 
 // ---- C ABI: host metadata (the engine's u32 form) --------------------------------------
 
-int mkv::stage_cached(Pool *p, StagedCache &c, const int32_t *h, size_t n, hipStream_t hs, MetaSlot **out) {
+int mkv::stage_cached(MetaRing *p, StagedCache &c, const int32_t *h, size_t n, hipStream_t hs, MetaSlot **out) {
   if (c.slot >= 0 && c.stream == hs && c.vals.size() == n) {
     MetaSlot *sl = &p->meta[c.slot];
     if (sl->gen == c.gen && std::memcmp(c.vals.data(), h, n * 4) == 0) {

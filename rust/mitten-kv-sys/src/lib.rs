@@ -29,6 +29,8 @@ pub const MKV_ATTN_PER_HEAD_LOADS: u32 = 8;
 pub const MKV_ATTN_CACHED_LOADS: u32 = 16;
 pub const MKV_PREP_PLAIN_Q: u32 = 1;
 pub const MKV_PREP_NO_NORM: u32 = 2;
+pub const MKV_STATE_NONE: u32 = 0xFFFF_FFFF;
+pub const MKV_LINEAR_HEAD_DECAY: u32 = 1;
 pub const MKV_WIRE_MAGIC: u32 = 0x57564B4D;
 pub const MKV_WIRE_VERSION: u32 = 1;
 pub const MKV_STATIC_SCRATCH_BYTES: u64 = 64 << 20;
@@ -46,6 +48,18 @@ pub struct mkv_pool_desc {
 }
 
 #[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct mkv_state_desc {
+    pub num_layers: i32,
+    pub num_k_heads: i32,
+    pub num_v_heads: i32,
+    pub k_dim: i32,
+    pub v_dim: i32,
+    pub dtype: i32,
+    pub num_slots: i64,
+}
+
+#[repr(C)]
 #[derive(Clone, Copy, Debug, Default)]
 pub struct mkv_wire_header {
     pub magic: u32, pub version: u16, pub dtype: u16,
@@ -55,6 +69,7 @@ pub struct mkv_wire_header {
 }
 #[repr(C)] pub struct mkv_pool { _p: [u8; 0] }
 #[repr(C)] pub struct mkv_decode_plan { _p: [u8; 0] }
+#[repr(C)] pub struct mkv_state_pool { _p: [u8; 0] }
 pub type hipStream_t = *mut c_void;
 
 extern "C" {
@@ -162,6 +177,40 @@ extern "C" {
     pub fn mkv_wire_header_init(desc: *const mkv_pool_desc, layer_begin: i32, num_layers: i32,
                                 num_blocks: i32, cached_len: i64, out: *mut mkv_wire_header) -> i32;
     pub fn mkv_wire_header_check(desc: *const mkv_pool_desc, header: *const mkv_wire_header) -> i32;
+    pub fn mkv_state_required_bytes(desc: *const mkv_state_desc, out_bytes: *mut u64) -> i32;
+    pub fn mkv_state_pool_create(desc: *const mkv_state_desc, device: i32,
+                                 out_pool: *mut *mut mkv_state_pool) -> i32;
+    pub fn mkv_state_pool_destroy(pool: *mut mkv_state_pool) -> i32;
+    pub fn mkv_state_pool_get_desc(pool: *const mkv_state_pool, out_desc: *mut mkv_state_desc) -> i32;
+    pub fn mkv_state_pool_buffer(pool: *const mkv_state_pool, out_dev_ptr: *mut *mut c_void,
+                                 out_bytes: *mut u64) -> i32;
+    pub fn mkv_state_pool_check(pool: *mut mkv_state_pool, stream: hipStream_t, out_bits: *mut u32) -> i32;
+    pub fn mkv_state_copy(pool: *mut mkv_state_pool, d_src_slots: *const i32, d_dst_slots: *const i32,
+                          num_pairs: i32, stream: hipStream_t) -> i32;
+    pub fn mkv_state_copy_host(pool: *mut mkv_state_pool, h_src_slots: *const u32, h_dst_slots: *const u32,
+                               num_pairs: i32, stream: hipStream_t) -> i32;
+    pub fn mkv_linear_step(pool: *mut mkv_state_pool, layer: i32, d_q: *const c_void, d_k: *const c_void,
+                           d_v: *const c_void, d_log_decay: *const f32, d_o: *mut c_void,
+                           d_src_slots: *const i32, d_dst_slots: *const i32, num_seqs: i32, scale: f32,
+                           flags: u32, stream: hipStream_t) -> i32;
+    pub fn mkv_linear_step_host(pool: *mut mkv_state_pool, layer: i32, d_q: *const c_void,
+                                d_k: *const c_void, d_v: *const c_void, d_log_decay: *const f32,
+                                d_o: *mut c_void, h_src_slots: *const u32, h_dst_slots: *const u32,
+                                num_seqs: i32, scale: f32, flags: u32, stream: hipStream_t) -> i32;
+    pub fn mkv_linear_extend(pool: *mut mkv_state_pool, layer: i32, d_q: *const c_void, d_k: *const c_void,
+                             d_v: *const c_void, d_log_decay: *const f32, d_o: *mut c_void,
+                             d_q_indptr: *const i32, d_src_slots: *const i32, d_dst_slots: *const i32,
+                             num_seqs: i32, num_tokens: i32, max_q_len: i32, scale: f32, flags: u32,
+                             d_workspace: *mut c_void, workspace_bytes: u64, stream: hipStream_t) -> i32;
+    pub fn mkv_linear_extend_host(pool: *mut mkv_state_pool, layer: i32, d_q: *const c_void,
+                                  d_k: *const c_void, d_v: *const c_void, d_log_decay: *const f32,
+                                  d_o: *mut c_void, h_q_lens: *const i32, h_src_slots: *const u32,
+                                  h_dst_slots: *const u32, num_seqs: i32, scale: f32, flags: u32,
+                                  stream: hipStream_t) -> i32;
+    pub fn mkv_add_rms_norm(device: i32, d_x: *const c_void, d_residual: *const c_void,
+                            d_weight: *const f32, eps: f32, num_rows: i32, dim: i32, dtype: i32,
+                            d_sum: *mut c_void, d_out: *mut c_void, d_fp8: *mut c_void, d_scales: *mut f32,
+                            group: i32, stream: hipStream_t) -> i32;
     pub fn mkv_validate_slots(desc: *const mkv_pool_desc, slots: *const i32, n: i32) -> i32;
     pub fn mkv_validate_block_tables(desc: *const mkv_pool_desc, indptr: *const i32, ids: *const i32,
                                      ctx_lens: *const i32, num_seqs: i32, max_ctx_len: i32) -> i32;

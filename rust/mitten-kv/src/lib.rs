@@ -20,11 +20,14 @@
 //!   queued block copies, builds the step's plan once from the batch's page
 //!   tables, and per layer appends and attends through the pool; the model
 //!   crates supply everything else through [`PagedModel`].
+//! * [`DeviceStatePool`]: the states of a hybrid model's linear-attention
+//!   layers, and [`add_rms_norm`], the residual + norm between layers.
 
 mod backend;
 mod error;
 mod host;
 mod pool;
+mod state;
 
 pub use backend::{AttentionIo, PagedBackend, PagedModel, StepLayout, SHARED_PREFIX_MIN_BYTES};
 pub use error::check;
@@ -32,3 +35,4 @@ pub use host::{
     schedule_prefill_chunks, Appended, CopyQueue, HostBlockManager, PagedLifecycle, PoolView, PrefillSchedule,
 };
 pub use pool::{DeviceKvPool, KvDtype, PoolGeometry, SharedPrefix, Stream, Tables, PAGE_SIZE};
+pub use state::{add_rms_norm, DeviceStatePool, LinearIo, StateGeometry, STATE_NONE};

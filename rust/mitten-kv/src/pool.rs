@@ -33,7 +33,7 @@ impl KvDtype {
             KvDtype::Bf16 => 2,
         }
     }
-    fn raw(self) -> i32 {
+    pub(crate) fn raw(self) -> i32 {
         match self {
             KvDtype::F32 => sys::MKV_DTYPE_F32,
             KvDtype::Bf16 => sys::MKV_DTYPE_BF16,
