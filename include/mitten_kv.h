@@ -493,8 +493,8 @@ enum {
 
 /* Bytes of the states: 4*L*slots*Hv*Dk*Dv. */
 MKV_API int mkv_state_required_bytes(const mkv_state_desc *desc, uint64_t *out_bytes);
-/* Allocate the states on `device` (hipMalloc; contents uninitialised).
- * MKV_ERR_OUT_OF_MEMORY if HBM cannot hold them. */
+/* Allocate the states and the pool's workspace on `device` (hipMalloc;
+ * contents uninitialised). MKV_ERR_OUT_OF_MEMORY if HBM cannot hold them. */
 MKV_API int mkv_state_pool_create(const mkv_state_desc *desc, int device, mkv_state_pool **out_pool);
 MKV_API int mkv_state_pool_destroy(mkv_state_pool *pool);
 MKV_API int mkv_state_pool_get_desc(const mkv_state_pool *pool, mkv_state_desc *out_desc);
@@ -542,7 +542,18 @@ MKV_API int mkv_linear_step_host(mkv_state_pool *pool, int32_t layer, const void
  * that no sequence has are left as they are. max_q_len sizes the launch (a
  * longer chunk is computed all the same); an indptr that falls back or
  * leaves [0, num_tokens] is reported (MKV_DEVERR_CTX) and its sequence
- * skipped. Slots, types and forms as in mkv_linear_step. */
+ * skipped. Slots, types and forms as in mkv_linear_step; sums, decays and
+ * states are f32 or wider, and with bf16 rows an output also carries the
+ * rounding of scores and of the state it reads to bf16.
+ * Where few long sequences would leave the device idle, their chunks are cut
+ * into segments (three launches) whose states stand in d_workspace
+ * (mkv_linear_extend_workspace_size bytes, 16-byte aligned; with less, the
+ * sequences stay whole), or in a workspace of the pool's own, allocated with
+ * it (64 MiB) when d_workspace is NULL. Calls that use the pool's own follow
+ * one another across streams; a captured one must not be replayed beside
+ * another call or graph that uses it (give each a workspace). */
+MKV_API int mkv_linear_extend_workspace_size(const mkv_state_pool *pool, int32_t num_seqs, int32_t num_tokens,
+                                             int32_t max_q_len, uint64_t *out_bytes);
 MKV_API int mkv_linear_extend(mkv_state_pool *pool, int32_t layer, const void *d_q, const void *d_k, const void *d_v,
                               const float *d_log_decay, void *d_o, const int32_t *d_q_indptr,
                               const int32_t *d_src_slots, const int32_t *d_dst_slots, int32_t num_seqs,

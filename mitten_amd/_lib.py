@@ -118,6 +118,7 @@ DEVICE_SIGNATURES = {
     "mkv_linear_step": (c_int, [P, i32, P, P, P, P, P, P, P, i32, f32, u32, P]),
     "mkv_linear_step_host": (c_int, [P, i32, P, P, P, P, P, U32P, U32P, i32, f32, u32, P]),
     "mkv_linear_extend": (c_int, [P, i32, P, P, P, P, P, P, P, P, i32, i32, i32, f32, u32, P, u64, P]),
+    "mkv_linear_extend_workspace_size": (c_int, [P, i32, i32, i32, ctypes.POINTER(u64)]),
     "mkv_linear_extend_host": (c_int, [P, i32, P, P, P, P, P, I32P, U32P, U32P, i32, f32, u32, P]),
     "mkv_add_rms_norm": (c_int, [c_int, P, P, P, f32, i32, i32, i32, P, P, P, P, i32, P]),
     "mkv_validate_slots": (c_int, [DESC_P, I32P, i32]),

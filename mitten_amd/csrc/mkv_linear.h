@@ -16,6 +16,11 @@ struct StatePool : MetaRing {
   uint64_t bytes = 0;
   int64_t state_elems = 0;    // one slot of one layer
   uint32_t *d_err = nullptr;  // device error word
+  void *ws = nullptr;         // workspace of split extend calls, allocated with the pool
+  uint64_t ws_bytes = 0;
+  hipEvent_t ws_done = nullptr;  // after the last eager call that used it, on ws_stream
+  hipStream_t ws_stream = nullptr;
+  bool ws_used = false;
   // Host arrays staged last by the step and extend entry points (every layer
   // of an engine step passes the same ones), scratch to assemble and to check
   // them in: mark[slot] = epoch of the call that last wrote the slot.
@@ -41,7 +46,7 @@ struct LinArgs {
 
 constexpr int32_t kMaxGrid = (1 << 24) - 1;  // workgroups of 256 threads in one grid dimension
 
-constexpr float kLog2eF = 1.4426950408889634f;
+constexpr uint64_t kLinWorkspace = 64ull << 20;  // bytes of a state pool's own workspace
 
 // One sequence's rows and slots; false: nothing to do (reported when `report`).
 struct LinSeq {

@@ -301,7 +301,11 @@ extern "C" int mkv_state_pool_create(const mkv_state_desc *desc, int device, mkv
   if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&p->data), bytes);
   if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&p->d_err), 256);
   if (e == hipSuccess) e = hipMemset(p->d_err, 0, 256);
+  p->ws_bytes = kLinWorkspace;
+  if (e == hipSuccess) e = hipMalloc(&p->ws, p->ws_bytes);
+  if (e == hipSuccess) e = hipEventCreateWithFlags(&p->ws_done, hipEventDisableTiming | hipEventDisableSystemFence);
   if (e != hipSuccess) {
+    if (p->ws) (void)hipFree(p->ws);
     if (p->data) (void)hipFree(p->data);
     if (p->d_err) (void)hipFree(p->d_err);
     delete p;
@@ -317,6 +321,8 @@ extern "C" int mkv_state_pool_destroy(mkv_state_pool *pool) {
   DeviceGuard guard(p->device);
   (void)hipDeviceSynchronize();
   meta_free(p);
+  (void)hipEventDestroy(p->ws_done);
+  (void)hipFree(p->ws);
   (void)hipFree(p->d_err);
   (void)hipFree(p->data);
   delete p;

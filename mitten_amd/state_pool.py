@@ -146,13 +146,14 @@ class DeviceStatePool:
         _raise(st)
 
     def tensor(self):
-        """Zero-copy torch view of the states, shape `desc.shape` (f32); valid
-        while the pool is open."""
+        """Zero-copy torch view of the states, shape `desc.shape` (f32). It
+        keeps the pool alive; after close() it must not be read."""
 
         class _View:
             pass
 
         view = _View()
+        view.pool = self  # the tensor holds the view: states are not freed under it
         view.__cuda_array_interface__ = {"shape": tuple(int(x) for x in self.desc.shape), "typestr": "<f4",
                                          "data": (self.data_ptr, False), "version": 3, "strides": None}
         return _torch().as_tensor(view, device=f"cuda:{self.device}")
@@ -251,13 +252,18 @@ class DeviceStatePool:
             raise _bad(f"q_lens add up to {int(lens.astype(np.int64).sum())} tokens, q has {n}")
         return lens, d, s
 
+    def linear_extend_workspace_size(self, num_seqs: int, num_tokens: int, max_q_len: int) -> int:
+        """Bytes of a workspace for linear_extend_device calls of that size (0: none is used)."""
+        out = ctypes.c_uint64()
+        _raise(self._lib.mkv_linear_extend_workspace_size(self._h, num_seqs, num_tokens, max_q_len, ctypes.byref(out)))
+        return out.value
+
     def linear_extend_device(self, layer: int, q, k, v, log_decay, q_indptr, slots, max_q_len: int, src_slots=None,
                              out=None, scale: float | None = None, workspace=None, stream=None):
         """linear_extend with device metadata (int32 q_indptr [B + 1], slots,
         src_slots), read when the kernels run: it can be captured into a
-        graph. workspace: a device tensor of
-        linear_extend_workspace_size(B, max_q_len) bytes, or None for the
-        pool's own."""
+        graph. workspace: a device tensor of linear_extend_workspace_size
+        bytes, or None for the pool's own."""
         torch = _torch()
         n, out, scale, flags = self._rows(q, k, v, log_decay, out, scale)
         B, dst, src, host, _ = self._slots(slots, src_slots)

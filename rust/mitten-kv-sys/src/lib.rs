@@ -197,6 +197,8 @@ extern "C" {
                                 d_k: *const c_void, d_v: *const c_void, d_log_decay: *const f32,
                                 d_o: *mut c_void, h_src_slots: *const u32, h_dst_slots: *const u32,
                                 num_seqs: i32, scale: f32, flags: u32, stream: hipStream_t) -> i32;
+    pub fn mkv_linear_extend_workspace_size(pool: *const mkv_state_pool, num_seqs: i32, num_tokens: i32,
+                                            max_q_len: i32, out_bytes: *mut u64) -> i32;
     pub fn mkv_linear_extend(pool: *mut mkv_state_pool, layer: i32, d_q: *const c_void, d_k: *const c_void,
                              d_v: *const c_void, d_log_decay: *const f32, d_o: *mut c_void,
                              d_q_indptr: *const i32, d_src_slots: *const i32, d_dst_slots: *const i32,

@@ -249,6 +249,23 @@ def test_rows_outside_the_sequences_and_bad_metadata_are_left_alone():
             assert np.all(got[~rows] == 7.0) and np.array_equal(st[0][~slots], host[0][~slots])
 
 
+def test_a_view_of_the_states_keeps_the_pool():
+    import gc
+    import weakref
+
+    pool = DeviceStatePool(StateDesc(1, 1, 1, 64, 64, 2, "f32"))
+    view = pool.tensor()[0]
+    alive = weakref.ref(pool)
+    del pool
+    gc.collect()
+    assert alive() is not None
+    view.fill_(3.0)
+    assert view.sum().item() == 3.0 * view.numel()
+    del view
+    gc.collect()
+    assert alive() is None
+
+
 def test_copies_and_forks():
     import torch
 
@@ -433,3 +450,65 @@ def test_random_batches(i):
     print(f"case {i}: heads {hk}/{hv} dims {dk}/{dv} {dtype} lens {lens} src {src} dst {dst}", flush=True)
     run_batch(lens, hk, hv, dk, dv, dtype, src, dst, n, 1000 + i, device_meta=bool(rng.integers(2)),
               rate=float(rng.choice([0.1, 1.0, 10.0])), scale=float(rng.uniform(0.1, 2.0)))
+
+
+def _long_call(pool, rng, hk, hv, dk, dv, n):
+    import torch
+
+    rows = [to_device(x) for x in inputs(rng, n, hk, hv, dk, dv, "bf16")]
+    ip = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    return rows, ip
+
+
+def test_workspaces_given_and_too_small_and_of_the_pool():
+    """A long prompt in segments from the pool's workspace and from a given one
+    is the same to the bit; with too little room it stays whole."""
+    import torch
+
+    hk, hv, dk, dv, n = 1, 2, 128, 128, 2000
+    rng = np.random.default_rng(23)
+    with DeviceStatePool(StateDesc(1, hk, hv, dk, dv, 2, "bf16")) as pool:
+        rows, ip = _long_call(pool, rng, hk, hv, dk, dv, n)
+        slots = torch.tensor([1], dtype=torch.int32, device="cuda")
+        new = torch.tensor([-1], dtype=torch.int32, device="cuda")
+        size = pool.linear_extend_workspace_size(1, n, n)
+        assert size > 0 and pool.linear_extend_workspace_size(0, 0, 0) == 0
+        got = []
+        for ws in (None, torch.empty(size, dtype=torch.uint8, device="cuda"),
+                   torch.empty(16, dtype=torch.uint8, device="cuda")):
+            o = pool.linear_extend_device(0, *rows, ip, slots, n, src_slots=new, workspace=ws)
+            pool.check()
+            got.append((o.float(), pool.tensor()[0, 1].clone()))
+        assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+        assert (got[0][0] - got[2][0]).norm() <= 2.0 ** -7 * got[2][0].norm()
+        assert (got[0][1] - got[2][1]).norm() <= 2.0 ** -20 * got[2][1].norm()
+        with pytest.raises(dp.BackendError) as ei:
+            pool.linear_extend_device(0, *rows, ip, slots, n, workspace=torch.empty(size + 8, dtype=torch.uint8,
+                                                                                   device="cuda")[8:])
+        assert "aligned" in str(ei.value)
+
+
+def test_two_streams_share_the_pools_workspace():
+    """Long prompts of two pairs of slots on two streams at once: each as alone."""
+    import torch
+
+    hk, hv, dk, dv, n = 1, 2, 128, 128, 3000
+    rng = np.random.default_rng(29)
+    with DeviceStatePool(StateDesc(1, hk, hv, dk, dv, 4, "bf16")) as pool:
+        calls = [inputs(rng, n, hk, hv, dk, dv, "bf16") for _ in range(2)]
+        calls = [[to_device(x) for x in c] for c in calls]
+        want = []
+        for b, c in enumerate(calls):
+            o = pool.linear_extend(0, *c, [n], [b], src_slots=[STATE_NONE])
+            want.append((o.clone(), pool.tensor()[0, b].clone()))
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in calls]
+        for _ in range(3):
+            outs = []
+            for b, (c, st) in enumerate(zip(calls, streams)):
+                outs.append(pool.linear_extend(0, *c, [n], [b + 2], src_slots=[STATE_NONE], out=torch.empty_like(want[b][0]),
+                                               stream=st))
+            torch.cuda.synchronize()
+            for b in range(2):
+                assert torch.equal(outs[b], want[b][0]) and torch.equal(pool.tensor()[0, b + 2], want[b][1])
+        pool.check()
