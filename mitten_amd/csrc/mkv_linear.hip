@@ -95,30 +95,31 @@ __global__ void __launch_bounds__(256) linear_recurrence_kernel(LinArgs a) {
         S[i], reinterpret_cast<f32x4 *>(a.states + s.dst * plane + off + (int64_t)(rg + R * i) * a.DV));
 }
 
-// grid.x = pair, grid.y = layer: a workgroup copies one slot's state of one
-// layer in 16-byte chunks, all loads of a pass first.
+// grid.x = (pair, part), grid.y = layer: a workgroup copies one 32 KiB part
+// of a slot's state of one layer, all its 16-byte loads first. (A state is
+// 0.5 to 8 MiB: a workgroup per state left most of the device idle in a fork
+// of a few, 78 us for 3 pairs of 6 layers against XX.)
 constexpr int kStatePer = 8;
 
 __global__ void __launch_bounds__(256)
 state_copy_kernel(float *__restrict__ states, const int32_t *__restrict__ src, const int32_t *__restrict__ dst,
-                  int64_t nslots, int64_t elems, uint32_t *__restrict__ d_err) {
-  const int32_t s = src[blockIdx.x], d = dst[blockIdx.x];
+                  int64_t nslots, int64_t elems, int parts, uint32_t *__restrict__ d_err) {
+  const int pair = blockIdx.x / parts, part = blockIdx.x % parts;
+  const int32_t s = src[pair], d = dst[pair];
   if (s < 0 || s >= nslots || d < 0 || d >= nslots) {
-    if (blockIdx.y == 0 && threadIdx.x == 0) record_error(d_err, MKV_DEVERR_COPY);
+    if (part == 0 && blockIdx.y == 0 && threadIdx.x == 0) record_error(d_err, MKV_DEVERR_COPY);
     return;
   }
   const int64_t plane = (int64_t)blockIdx.y * nslots * elems;
   const f32x4 *sp = reinterpret_cast<const f32x4 *>(states + plane + s * elems);
   f32x4 *dp = reinterpret_cast<f32x4 *>(states + plane + d * elems);
-  const int64_t total = elems / 4;
-  for (int64_t base = threadIdx.x; base < total; base += 256 * kStatePer) {
-    f32x4 r[kStatePer];
+  const int64_t total = elems / 4, base = (int64_t)part * 256 * kStatePer + threadIdx.x;
+  f32x4 r[kStatePer];
 #pragma unroll
-    for (int u = 0; u < kStatePer; u++) r[u] = __builtin_nontemporal_load(sp + min(base + u * 256, total - 1));
+  for (int u = 0; u < kStatePer; u++) r[u] = __builtin_nontemporal_load(sp + min(base + u * 256, total - 1));
 #pragma unroll
-    for (int u = 0; u < kStatePer; u++)
-      if (base + u * 256 < total) __builtin_nontemporal_store(r[u], dp + base + u * 256);
-  }
+  for (int u = 0; u < kStatePer; u++)
+    if (base + u * 256 < total) __builtin_nontemporal_store(r[u], dp + base + u * 256);
 }
 
 // ---- host side ------------------------------------------------------------------
@@ -364,12 +365,13 @@ extern "C" int mkv_state_copy(mkv_state_pool *pool, const int32_t *d_src_slots, 
   StatePool *p = reinterpret_cast<StatePool *>(pool);
   if (num_pairs < 0) return set_error(MKV_ERR_INVALID_ARGUMENT, "num_pairs < 0");
   if (num_pairs == 0) return MKV_OK;
-  if (num_pairs > kMaxGrid) return set_error(MKV_ERR_INVALID_ARGUMENT, "num_pairs > %d", kMaxGrid);
+  const int64_t parts = (p->state_elems / 4 + 256 * kStatePer - 1) / (256 * kStatePer);
+  if (num_pairs * parts > kMaxGrid) return set_error(MKV_ERR_INVALID_ARGUMENT, "too many pairs for one launch");
   if (!d_src_slots || !d_dst_slots) return set_error(MKV_ERR_INVALID_ARGUMENT, "NULL device pointer");
   DeviceGuard guard(p->device);
-  hipLaunchKernelGGL(state_copy_kernel, dim3((unsigned)num_pairs, (unsigned)p->desc.num_layers), dim3(256), 0,
+  hipLaunchKernelGGL(state_copy_kernel, dim3((unsigned)(num_pairs * parts), (unsigned)p->desc.num_layers), dim3(256), 0,
                      reinterpret_cast<hipStream_t>(stream), p->data, d_src_slots, d_dst_slots, p->desc.num_slots,
-                     p->state_elems, p->d_err);
+                     p->state_elems, (int)parts, p->d_err);
   MKV_CHECK_LAUNCH("state_copy_kernel");
   return MKV_OK;
 }

@@ -498,6 +498,257 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
   }
 }
 
+// ===========================================================================
+// f32 rows: the same products on v_mfma_f32_16x16x4 (a fifth of the bf16 rate
+// counted with its three parts, and exact), chunks of 32 tokens so that the
+// tiles of k_dim 256 leave room for two workgroups per CU. Four waves on 64
+// columns. The four products of an operand step take rows (or tokens) 4 g + i
+// for i = 0 .. 3, again what accumulators and 16-byte reads deliver. Tiles are
+// swizzled by chunk c ^ (r & 15): free of conflicts for 16-byte reads of one
+// chunk of 16 rows and for 4-byte reads of 16 columns of rows 4 g + i.
+// Decays are differences of sums kept in two floats, exact to f32's last bits.
+// ===========================================================================
+constexpr int kChunkF32 = 32;
+
+template <int DK, int MODE>
+__global__ void __launch_bounds__(256, DK == 256 ? 1 : 2) linear_chunk_f32_kernel(LinArgs a, LinSegs sg) {
+  constexpr bool OUT = MODE != kLocal;
+  constexpr int C = kChunkF32, W = 64, KC = DK / 4, VC = W / 4;  // 16-byte chunks per row
+  constexpr int KL = C * KC / 256, VL = C * VC / 256;
+  __shared__ __attribute__((aligned(16))) float kt[C * DK], qt[OUT ? C * DK : 4], vt[C * W], pt[OUT ? C * C : 4];
+  // Summed log2 decay (two floats), scale e^G, and e^{G_end - G} per token.
+  __shared__ __attribute__((aligned(16))) float gh[C], gl[C], es[C], ws[C];
+  __shared__ float gend_s;
+  __shared__ int odd_s;  // the last chunk (counted from 1) with an Inf or NaN in k or v
+
+  const int slices = a.DV / W, rep = a.Hv / a.Hk;
+  const int members = rep * slices, grp = (int)((blockIdx.x >> 3) / members) * 8 + (int)(blockIdx.x & 7);
+  const int mem = (int)((blockIdx.x >> 3) % members);
+  const int inst = grp / a.Hk, kh = grp % a.Hk;
+  const int seg = inst % sg.nseg, b = inst / sg.nseg;
+  if (b >= a.B) return;
+  const int h = kh * rep + mem / slices, sl = mem % slices;
+  int tid = threadIdx.x;
+  const int lane = tid & 63;
+  int m16 = lane & 15, g4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  LinSeq s;
+  if (!lin_seq(a, b, MODE != kLocal && tid == 0 && seg == 0 && h == 0 && sl == 0, s)) return;
+  s.row0 = __builtin_amdgcn_readfirstlane(s.row0);
+  s.n = __builtin_amdgcn_readfirstlane(s.n);
+  s.src = __builtin_amdgcn_readfirstlane((int)s.src);
+  s.dst = __builtin_amdgcn_readfirstlane((int)s.dst);
+  const int ns = lin_nseg(sg, s.n);
+  if (seg >= ns) return;
+  const int t_begin = seg * sg.len, t_end = seg == ns - 1 ? s.n : t_begin + sg.len;
+
+  const int64_t plane = (int64_t)a.Hv * DK * a.DV, hoff = (int64_t)h * DK * a.DV;
+  uint32_t lane_off = (uint32_t)(4 * g4 * a.DV + sl * W + 16 * wave + m16) * 4, srow = a.DV * 4;
+  float *const frag = sg.state + ((int64_t)b * sg.nseg + seg) * plane + hoff + (sl * 4 + wave) * (DK * 16) + lane * 4;
+  f32x4 S[DK / 16];
+  float z = 0.0f;  // a NaN where the state holds an Inf or a NaN
+  const auto from = buffer(a.states + (s.src >= 0 ? s.src : 0) * plane + hoff, s.src >= 0 ? DK * srow : 0);  // none: zeros
+#pragma unroll
+  for (int j = 0; j < DK / 16; j++) {
+    S[j] = f32x4{};
+    if constexpr (MODE == kOutputs) S[j] = *reinterpret_cast<const f32x4 *>(frag + j * 256);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if constexpr (MODE == kWhole) S[j][i] = buffer_load4(from, lane_off + (16 * j + i) * srow);
+      z = fmaf(S[j][i], 0.0f, z);
+    }
+  }
+  double total = 0.0;  // summed log2 decays of the segment so far (wave 0)
+  if (tid == 0) odd_s = 0;
+
+  const uint8_t *kp = static_cast<const uint8_t *>(a.k) + ((int64_t)s.row0 * a.Hk + kh) * (DK * 4);
+  const uint8_t *qp = static_cast<const uint8_t *>(a.q) + ((int64_t)s.row0 * a.Hk + kh) * (DK * 4);
+  const uint8_t *vp = static_cast<const uint8_t *>(a.v) + ((int64_t)s.row0 * a.Hv + h) * a.DV * 4 + sl * (W * 4);
+  const int64_t krs = (int64_t)a.Hk * DK * 4, vrs = (int64_t)a.Hv * a.DV * 4;  // row strides
+  f32x4 kr[KL], qr[OUT ? KL : 1], vr[VL];
+  float gr = 0.0f;
+  auto load = [&](int t0) {  // rows past the segment's end are zeros
+    const bool any = t0 < t_end;
+    const uint32_t last = min(C, t_end - t0) - 1;
+    const int64_t at = any ? t0 : 0;
+    const uint32_t kb = any ? last * (uint32_t)krs + DK * 4 : 0;
+    const auto rk = buffer(kp + at * krs, kb), rq = buffer(qp + at * krs, kb);
+    const auto rv = buffer(vp + at * vrs, any ? last * (uint32_t)vrs + W * 4 : 0);
+#pragma unroll
+    for (int i = 0; i < KL; i++) {
+      const uint32_t off = (tid / KC + i * (256 / KC)) * (uint32_t)krs + tid % KC * 16;
+      kr[i] = __builtin_bit_cast(f32x4, buffer_load16(rk, off));
+      if constexpr (OUT) qr[i] = __builtin_bit_cast(f32x4, buffer_load16(rq, off));
+    }
+#pragma unroll
+    for (int i = 0; i < VL; i++)
+      vr[i] = __builtin_bit_cast(
+          f32x4, buffer_load16(rv, (tid / VC + i * (256 / VC)) * (uint32_t)vrs + tid % VC * 16));
+    const uint32_t gs = a.g_stride * 4;
+    gr = buffer_load4(buffer(a.g + (any ? (int64_t)(s.row0 + t0) * a.g_stride : 0), any ? last * gs + 4 * h + 4 : 0),
+                      (lane & (C - 1)) * gs + 4 * h);
+  };
+  // Element (r, c) of a tile of cpr chunks per row.
+  auto at = [](int r, int c, int cpr) { return r * cpr * 4 + ((c >> 2) ^ (r & 15)) * 4 + (c & 3); };
+  auto read4 = [&](const float *tile, int r, int c, int cpr) {
+    return *reinterpret_cast<const f32x4 *>(tile + at(r, c, cpr));
+  };
+
+  load(t_begin);
+  int chunk = 0, t0 = t_begin;
+  for (; t0 < t_end; t0 += C) {
+    const int nt = min(C, t_end - t0);
+    chunk++;
+    // (Opaque: addresses are formed where they are used, not kept over the loop.)
+    asm volatile("" : "+v"(tid), "+v"(m16), "+v"(g4), "+v"(lane_off));
+    __syncthreads();  // the previous chunk's tiles are read
+    float odd = chunk == 1 && OUT ? z : 0.0f;
+#pragma unroll
+    for (int i = 0; i < KL; i++) {
+      const int r = tid / KC + i * (256 / KC), c = tid % KC * 4;
+      *reinterpret_cast<f32x4 *>(kt + at(r, c, KC)) = kr[i];
+      if constexpr (OUT) *reinterpret_cast<f32x4 *>(qt + at(r, c, KC)) = qr[i];
+#pragma unroll
+      for (int e = 0; e < 4; e++) odd = fmaf(kr[i][e], 0.0f, odd);
+    }
+#pragma unroll
+    for (int i = 0; i < VL; i++) {
+      const int r = tid / VC + i * (256 / VC), c = tid % VC * 4;
+      *reinterpret_cast<f32x4 *>(vt + at(r, c, VC)) = vr[i];
+#pragma unroll
+      for (int e = 0; e < 4; e++) odd = fmaf(vr[i][e], 0.0f, odd);
+    }
+    if (odd != odd) odd_s = chunk;
+    double end = 0.0;
+    if (wave == 0) {
+      const double l = lane < nt ? log2_decay(gr) : 0.0, G = wave_scan(l);
+      end = lane_d(G, 63);
+      if (lane < C) {
+        gh[lane] = (float)G;
+        gl[lane] = (float)(G - (double)(float)G);
+        es[lane] = exp2_f((float)G) * a.scale;
+        ws[lane] = exp2_f((float)(end - G));
+      }
+      if (lane == 0) gend_s = exp2_f((float)end);
+    }
+    __syncthreads();
+    if (odd_s == chunk) break;  // uniform over the workgroup
+    load(t0 + C);
+    total += end;
+
+    f32x4 acc[2];
+    if constexpr (OUT) {
+      // Scores: one tile of 16 tokens (columns) by 16 keys per wave; the one
+      // that no column sees comes out as zeros.
+      const int tq = wave & 1, st = wave >> 1, t = 16 * tq + m16;
+      f32x4 c[4] = {};  // four chains
+#pragma unroll
+      for (int j = 0; j < DK / 16; j++) {
+        const f32x4 kf = read4(kt, 16 * st + m16, 16 * j + 4 * g4, KC), qf = read4(qt, t, 16 * j + 4 * g4, KC);
+#pragma unroll
+        for (int i = 0; i < 4; i++) c[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[i], qf[i], c[i], 0, 0, 0);
+      }
+      const f32x4 r = (c[0] + c[1]) + (c[2] + c[3]);
+      f32x4 p;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {  // (selected, not multiplied: past t it may be anything)
+        const int k = 16 * st + 4 * g4 + i;
+        const float e = exp2_f((gh[t] - gh[k]) + (gl[t] - gl[k])) * a.scale;
+        p[i] = k <= t ? r[i] * e : 0.0f;
+      }
+      *reinterpret_cast<f32x4 *>(pt + t * C + ((4 * st + g4) ^ (t & 7)) * 4) = p;
+      // O^T from the state.
+#pragma unroll
+      for (int tt = 0; tt < 2; tt++) {
+        f32x4 o[2] = {};
+#pragma unroll
+        for (int j = 0; j < DK / 16; j++) {
+          const f32x4 qf = read4(qt, 16 * tt + m16, 16 * j + 4 * g4, KC);
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            o[i & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(S[j][i], qf[i], o[i & 1], 0, 0, 0);
+        }
+        acc[tt] = (o[0] + o[1]) * es[16 * tt + m16];
+      }
+      __syncthreads();  // the scores are written
+    }
+    float vf[2][4];  // [16 tokens][4 g + i] of the wave's columns
+#pragma unroll
+    for (int st = 0; st < 2; st++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) vf[st][i] = vt[at(16 * st + 4 * g4 + i, 16 * wave + m16, VC)];
+    if constexpr (OUT) {
+      const auto ob = buffer(static_cast<uint8_t *>(a.o) + ((int64_t)(s.row0 + t0) * a.Hv + h) * a.DV * 4 + sl * (W * 4),
+                             (uint32_t)(nt - 1) * (uint32_t)vrs + W * 4);
+#pragma unroll
+      for (int tt = 0; tt < 2; tt++) {
+        const int t = 16 * tt + m16;
+#pragma unroll
+        for (int st = 0; st <= tt; st++) {
+          const f32x4 p = *reinterpret_cast<const f32x4 *>(pt + t * C + ((4 * st + g4) ^ (t & 7)) * 4);
+#pragma unroll
+          for (int i = 0; i < 4; i++) acc[tt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[st][i], p[i], acc[tt], 0, 0, 0);
+        }
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[tt]), ob,
+                                               t * (uint32_t)vrs + (16 * wave + 4 * g4) * 4, 0, 0);
+      }
+    }
+    const float dend = gend_s;
+#pragma unroll
+    for (int j = 0; j < DK / 16; j++) S[j] *= dend;
+#pragma unroll
+    for (int st = 0; st < 2; st++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int r = 16 * st + 4 * g4 + i;
+        const float wv = vf[st][i] * ws[r];
+#pragma unroll
+        for (int j = 0; j < DK / 16; j++)
+          S[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(kt[at(r, 16 * j + m16, KC)], wv, S[j], 0, 0, 0);
+      }
+  }
+
+  // Token by token from the first chunk with an Inf or NaN on, as the bf16 form.
+#pragma unroll 1
+  for (; t0 < t_end; t0++) {
+    asm volatile("" : "+v"(m16), "+v"(g4));
+    const int64_t krow = ((int64_t)(s.row0 + t0) * a.Hk + kh) * DK + 4 * g4;
+    const int64_t vrow = ((int64_t)(s.row0 + t0) * a.Hv + h) * a.DV + sl * W + 16 * wave + m16;
+    const double l = log2_decay(a.g[(int64_t)(s.row0 + t0) * a.g_stride + h]);
+    const float d = exp2_f((float)l), v = static_cast<const float *>(a.v)[vrow];
+    total += l;
+    float o = 0.0f;
+#pragma unroll
+    for (int j = 0; j < DK / 16; j++) {
+      const f32x4 k = *reinterpret_cast<const f32x4 *>(static_cast<const float *>(a.k) + krow + 16 * j);
+      const f32x4 q = *reinterpret_cast<const f32x4 *>(static_cast<const float *>(a.q) + krow + 16 * j);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        S[j][i] = d * S[j][i] + k[i] * v;
+        o += q[i] * S[j][i];
+      }
+    }
+    if constexpr (OUT) {
+      o += __shfl_xor(o, 16);
+      o += __shfl_xor(o, 32);
+      if (g4 == 0) static_cast<float *>(a.o)[vrow] = o * a.scale;
+    }
+  }
+
+  if constexpr (MODE == kLocal) {
+    if (tid == 0 && sl == 0) sg.decay[((int64_t)b * sg.nseg + seg) * a.Hv + h] = exp2_f((float)total);
+#pragma unroll
+    for (int j = 0; j < DK / 16; j++) *reinterpret_cast<f32x4 *>(frag + j * 256) = S[j];
+  } else if constexpr (MODE == kWhole) {
+    const auto to = buffer(a.states + s.dst * plane + hoff, DK * srow);
+#pragma unroll
+    for (int j = 0; j < DK / 16; j++)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(S[j][i]), to, lane_off + (16 * j + i) * srow, 0, 0);
+  }
+}
+
 // The scan over segments: from the state a sequence begins with and each
 // segment's local state, the state before every segment (in place of its
 // local one) and the sequence's last, into its slot. Elementwise; a thread
@@ -548,11 +799,13 @@ static uint64_t segs_bytes(const StatePool *p, int64_t num_seqs, int64_t nseg) {
   return n * p->state_elems * 4 + ((n * p->desc.num_v_heads * 4 + 15) & ~15ull);
 }
 
+// NW 0: f32 rows.
 template <int DK, int NW, int MODE>
 static void launch_chunks(const LinArgs &a, const LinSegs &sg, hipStream_t hs) {
   const int64_t groups = ((int64_t)a.B * sg.nseg * a.Hk + 7) / 8 * 8;
-  const dim3 grid((unsigned)(groups * (a.Hv / a.Hk) * (a.DV / (16 * NW))));
-  hipLaunchKernelGGL((linear_chunk_kernel<DK, NW, MODE>), grid, dim3(64 * NW), 0, hs, a, sg);
+  const dim3 grid((unsigned)(groups * (a.Hv / a.Hk) * (a.DV / (NW ? 16 * NW : 64))));
+  if constexpr (NW) hipLaunchKernelGGL((linear_chunk_kernel<DK, NW, MODE>), grid, dim3(64 * NW), 0, hs, a, sg);
+  else hipLaunchKernelGGL((linear_chunk_f32_kernel<DK, MODE>), grid, dim3(256), 0, hs, a, sg);
 }
 
 // How a batch is computed, from the launches' measured times on the 256 CUs at
@@ -573,7 +826,8 @@ static LinPlan plan_extend(const StatePool *p, int64_t num_seqs, int64_t num_tok
   // Whole sequences: workgroups of 64 columns while two to a CU hold them all
   // (8 prompts of 300-1,500 tokens, 28 heads: 66 us against 74 with 128
   // columns), else of 128, which form the scores once for twice the columns.
-  if (d.v_dim == 64 || num_seqs * per_seq4 <= 2 * p->cus) r.waves = 4;
+  const bool f32 = d.dtype == MKV_DTYPE_F32;
+  if (f32 || d.v_dim == 64 || num_seqs * per_seq4 <= 2 * p->cus) r.waves = 4;
   const double load = (double)chunks * heads * d.v_dim / 128 / cus;  // chunks of 128 columns per CU
   const double whole = std::max(2.75 * longest, 3.3 * load);
   // Segments: 32 us for three launches and the states between them, 4.6 us
@@ -581,7 +835,7 @@ static LinPlan plan_extend(const StatePool *p, int64_t num_seqs, int64_t num_tok
   const int64_t want = std::max<int64_t>(4, (int64_t)(load / 2 + 0.5));  // chunks of one: two workgroups per CU
   const int64_t nseg = (longest + want - 1) / want;
   if (nseg > 1 && 32.0 + 4.6 * load < whole && segs_bytes(p, num_seqs, nseg) <= ws_bytes) {
-    r.waves = d.v_dim == 64 ? 4 : 8;
+    r.waves = f32 || d.v_dim == 64 ? 4 : 8;
     r.nseg = (int)nseg;
     r.len = (int)want * kChunk;
   }
@@ -604,7 +858,6 @@ static int launch_extend(StatePool *p, const LinArgs &a, int32_t max_q_len, void
                          hipStream_t hs) {
   const mkv_state_desc &d = p->desc;
   if (a.B == 0) return MKV_OK;
-  if (d.dtype != MKV_DTYPE_BF16) return launch_recurrence(p, a, hs);
   const LinPlan pl = plan_extend(p, a.B, a.num_tokens, max_q_len, ws_bytes);
   const int64_t wgs = ((int64_t)a.B * pl.nseg * a.Hk + 7) / 8 * 8 * (a.Hv / a.Hk) * (d.v_dim / (16 * pl.waves));
   if (wgs * (pl.waves / 4) > kMaxGrid || (int64_t)a.B * a.Hv * (d.k_dim * d.v_dim / 1024) > kMaxGrid)
@@ -621,7 +874,10 @@ static int launch_extend(StatePool *p, const LinArgs &a, int32_t max_q_len, void
     own_ws = ws == p->ws && st == hipStreamCaptureStatusNone;
     if (own_ws && p->ws_used && p->ws_stream != hs) MKV_CHECK_HIP(hipStreamWaitEvent(hs, p->ws_done, 0));
   }
-  switch (d.k_dim * 10 + pl.waves) {
+  switch (d.k_dim * 10 + (d.dtype == MKV_DTYPE_BF16 ? pl.waves : 0)) {
+    case 640: launch_plan<64, 0>(p, a, sg, hs); break;
+    case 1280: launch_plan<128, 0>(p, a, sg, hs); break;
+    case 2560: launch_plan<256, 0>(p, a, sg, hs); break;
     case 644: launch_plan<64, 4>(p, a, sg, hs); break;
     case 648: launch_plan<64, 8>(p, a, sg, hs); break;
     case 1284: launch_plan<128, 4>(p, a, sg, hs); break;
@@ -649,7 +905,7 @@ extern "C" int mkv_linear_extend_workspace_size(const mkv_state_pool *pool, int3
     return set_error(MKV_ERR_INVALID_ARGUMENT, "num_seqs must be in [0, 65535], num_tokens and max_q_len >= 0");
   const StatePool *p = reinterpret_cast<const StatePool *>(pool);
   *out_bytes = 0;
-  if (num_seqs == 0 || p->desc.dtype != MKV_DTYPE_BF16) return MKV_OK;
+  if (num_seqs == 0) return MKV_OK;
   const LinPlan pl = plan_extend(p, num_seqs, num_tokens, max_q_len, UINT64_MAX);
   if (pl.nseg > 1) *out_bytes = segs_bytes(p, num_seqs, pl.nseg);
   return MKV_OK;

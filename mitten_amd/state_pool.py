@@ -95,6 +95,14 @@ def _stream(stream, device: int) -> ctypes.c_void_p:
     return ctypes.c_void_p(stream.cuda_stream)
 
 
+def _raw_stream(stream, device: int) -> int:
+    """_stream as a number, without a Stream object for the current one where torch offers that."""
+    if stream is not None:
+        return stream.cuda_stream
+    raw = getattr(_torch()._C, "_cuda_getCurrentRawStream", None)
+    return raw(device) if raw is not None else _torch().cuda.current_stream(device).cuda_stream
+
+
 def _torch_type(name: str):
     torch = _torch()
     return torch.float32 if name == "f32" else torch.bfloat16
@@ -334,31 +342,40 @@ def add_rms_norm(x, weight, eps: float, residual=None, residual_out=None, out=No
     torch = _torch()
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() != 2:
         raise _bad("x must be a device tensor [rows, dim]")
-    if x.dtype not in (torch.float32, torch.bfloat16):
-        raise _bad(f"x has dtype {x.dtype}, expected float32 or bfloat16")
-    dev = x.device.index
-    rows, dim = x.shape
-    _check(x, dev, None, x.dtype, "x")
-    _check(weight, dev, (dim,), torch.float32, "weight")
-    if residual is not None:
-        _check(residual, dev, (rows, dim), x.dtype, "residual")
-        if residual_out is None:
-            residual_out = torch.empty_like(x)
-    if residual_out is not None:
-        _check(residual_out, dev, (rows, dim), x.dtype, "residual_out")
+    dt, shape, device = x.dtype, x.shape, x.device
+    if dt != torch.float32 and dt != torch.bfloat16:
+        raise _bad(f"x has dtype {dt}, expected float32 or bfloat16")
+    dev = device.index
+    rows, dim = shape
+    if not x.is_contiguous():
+        raise _bad("x must be contiguous")
+
+    def like_x(t, name):  # (_check names what is wrong)
+        if not isinstance(t, torch.Tensor) or t.dtype != dt or t.shape != shape or t.device != device or \
+                not t.is_contiguous():
+            _check(t, dev, shape, dt, name)
+        return t.data_ptr()
+
+    if not isinstance(weight, torch.Tensor) or weight.dtype != torch.float32 or weight.device != device or \
+            weight.dim() != 1 or weight.shape[0] != dim or not weight.is_contiguous():
+        _check(weight, dev, (dim,), torch.float32, "weight")
+    if residual is not None and residual_out is None:
+        residual_out = torch.empty_like(x)
     if out is None and (both or not fp8):
         out = torch.empty_like(x)
-    if out is not None:
-        _check(out, dev, (rows, dim), x.dtype, "out")
     q8 = scales = None
     if fp8:
         if group < 0 or (group and dim % group):
             raise _bad(f"group ({group}) does not divide dim ({dim})")
-        q8 = torch.empty((rows, dim), dtype=torch.float8_e4m3fn, device=x.device)
-        scales = torch.empty((rows, dim // group if group else 1), dtype=torch.float32, device=x.device)
+        q8 = torch.empty((rows, dim), dtype=torch.float8_e4m3fn, device=device)
+        scales = torch.empty((rows, dim // group if group else 1), dtype=torch.float32, device=device)
     elif group:
         raise _bad("group is for an e4m3 output")
-    _raise(_lib.device_lib().mkv_add_rms_norm(
-        dev, _dptr(x), _tptr(residual), _dptr(weight), eps, rows, dim, 0 if x.dtype == torch.float32 else 1,
-        _tptr(residual_out), _tptr(out), _tptr(q8), _tptr(scales), group, _stream(stream, dev)))
+    st = _lib.device_lib().mkv_add_rms_norm(
+        dev, x.data_ptr(), None if residual is None else like_x(residual, "residual"), weight.data_ptr(), eps, rows, dim,
+        0 if dt == torch.float32 else 1, None if residual_out is None else like_x(residual_out, "residual_out"),
+        None if out is None else like_x(out, "out"), None if q8 is None else q8.data_ptr(),
+        None if scales is None else scales.data_ptr(), group, _raw_stream(stream, dev))
+    if st:
+        _raise(st)
     return residual_out, out, q8, scales
