@@ -7,6 +7,7 @@
 // four matrix products per chunk instead of a rank-one update per token.
 #include <algorithm>
 #include <climits>
+#include <cmath>
 #include <cstring>
 #include <new>
 
@@ -808,37 +809,48 @@ static void launch_chunks(const LinArgs &a, const LinSegs &sg, hipStream_t hs) {
   else hipLaunchKernelGGL((linear_chunk_f32_kernel<DK, MODE>), grid, dim3(256), 0, hs, a, sg);
 }
 
-// How a batch is computed, from the launches' measured times on the 256 CUs at
-// head dims of 128 (the other dims scale both sides alike).
+// How a batch is computed.
 struct LinPlan {
-  int waves;       // per workgroup: 4 (64 columns) or 8 (128)
-  int nseg, len;   // segments per sequence, tokens of one
+  int waves;      // per workgroup: 4 (64 columns) or 8 (128)
+  int nseg, len;  // segments per sequence, tokens of one
 };
 
+// The costs are measured ones in microseconds at head dims of 128 on 256 CUs
+// (other dims scale both sides alike): whole sequences, `lone` per chunk of 64
+// tokens of the longest or `full` per chunk and CU (of 128 columns; f32: 64);
+// segments, `seg` per chunk of one round of workgroups or `segs` of each of
+// several, 12 for three launches, and the states between them, written,
+// scanned and read at 5 TB/s. Measured against whole: 2,000 tokens of 32 heads 51-56 us (whole 130), 600 tokens 34
+// (46), 300 tokens whole 22 (28 in segments), 8 prompts of 300-1,500 tokens of
+// 28 heads whole 76 (109), f32 2,000 tokens of 14 heads of 64 37 (202).
 static LinPlan plan_extend(const StatePool *p, int64_t num_seqs, int64_t num_tokens, int64_t max_q_len,
                            uint64_t ws_bytes) {
   const mkv_state_desc &d = p->desc;
+  const bool f32 = d.dtype == MKV_DTYPE_F32;
   const int64_t longest = std::max<int64_t>(1, (max_q_len + kChunk - 1) / kChunk);  // chunks
   const int64_t chunks = std::min(num_seqs * longest, num_tokens / kChunk + num_seqs);
-  const double cus = p->cus;
-  const int64_t heads = d.num_v_heads, per_seq4 = heads * (d.v_dim / 64);
-  LinPlan r = {8, 1, INT_MAX & ~(kChunk - 1)};
-  // Whole sequences: workgroups of 64 columns while two to a CU hold them all
-  // (8 prompts of 300-1,500 tokens, 28 heads: 66 us against 74 with 128
-  // columns), else of 128, which form the scores once for twice the columns.
-  const bool f32 = d.dtype == MKV_DTYPE_F32;
-  if (f32 || d.v_dim == 64 || num_seqs * per_seq4 <= 2 * p->cus) r.waves = 4;
-  const double load = (double)chunks * heads * d.v_dim / 128 / cus;  // chunks of 128 columns per CU
-  const double whole = std::max(2.75 * longest, 3.3 * load);
-  // Segments: 32 us for three launches and the states between them, 4.6 us
-  // per chunk and CU (8,192 tokens of 32 heads: 102 us; whole 350).
-  const int64_t want = std::max<int64_t>(4, (int64_t)(load / 2 + 0.5));  // chunks of one: two workgroups per CU
-  const int64_t nseg = (longest + want - 1) / want;
-  if (nseg > 1 && 32.0 + 4.6 * load < whole && segs_bytes(p, num_seqs, nseg) <= ws_bytes) {
-    r.waves = f32 || d.v_dim == 64 ? 4 : 8;
-    r.nseg = (int)nseg;
-    r.len = (int)want * kChunk;
+  const int cols = f32 || d.v_dim == 64 ? 64 : 128;  // of a workgroup over segments
+  const double load = (double)chunks * d.num_v_heads * d.v_dim / (f32 ? 64 : 128) / p->cus;
+  const double lone = f32 ? 6.8 : 3.6, full = f32 ? 5.6 : 3.3, seg = f32 ? 8.4 : 7.4, segs = f32 ? 6.0 : 6.2;
+  LinPlan r = {cols / 16, 1, INT_MAX & ~(kChunk - 1)};
+  double best = std::max(lone * longest, full * load);
+  for (int64_t want = 1; want < longest && want * segs < best; want++) {  // chunks of a segment
+    const int64_t nseg = (longest + want - 1) / want;
+    const uint64_t bytes = segs_bytes(p, num_seqs, nseg);
+    if (bytes > ws_bytes) continue;
+    const double wgs = (double)chunks / want * d.num_v_heads * (d.v_dim / cols);
+    const double rounds = std::max(1.0, std::ceil(wgs / p->cus - 0.05));
+    const double t = 12.0 + 3.0 * (double)bytes / 5e6 + want * (rounds > 1.0 ? segs * rounds : seg);
+    if (t < best) {
+      best = t;
+      r.nseg = (int)nseg;
+      r.len = (int)want * kChunk;
+    }
   }
+  // Whole sequences of bf16 take 64 columns a workgroup while two to a CU hold
+  // them all (8 prompts of 300-1,500 tokens, 28 heads: 76 us against 81 with
+  // 128), else 128, which form the scores once for twice the columns.
+  if (r.nseg == 1 && num_seqs * d.num_v_heads * (d.v_dim / 64) <= 2 * p->cus) r.waves = 4;
   return r;
 }
 
