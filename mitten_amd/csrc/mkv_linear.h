@@ -18,8 +18,7 @@ struct StatePool : MetaRing {
   uint32_t *d_err = nullptr;  // device error word
   void *ws = nullptr;         // workspace of split extend calls, allocated with the pool
   uint64_t ws_bytes = 0;
-  hipEvent_t ws_done = nullptr;  // after the last eager call that used it, on ws_stream
-  hipStream_t ws_stream = nullptr;
+  hipEvent_t ws_done = nullptr;  // after the last eager call that used it
   bool ws_used = false;
   // Host arrays staged last by the step and extend entry points (every layer
   // of an engine step passes the same ones), scratch to assemble and to check
@@ -86,7 +85,5 @@ int check_state_slots(StatePool *p, const uint32_t *src, const uint32_t *dst, in
 // Refuses a stream that is being captured (host metadata is staged in buffers
 // that later calls reuse).
 int refuse_capture(hipStream_t hs);
-// The recurrence, token by token: a workgroup per (sequence, value head, columns).
-int launch_recurrence(StatePool *p, const LinArgs &a, hipStream_t hs);
 
 }  // namespace mkv

@@ -1,10 +1,11 @@
-// Linear-attention states: the pool that holds them, copies between slots,
-// and the recurrence that moves them on token by token.
+// Linear-attention states: the pool that holds them, copies between slots, and
+// the step that moves each sequence's on by one token.
 //
 // A linear-attention layer keeps, instead of K/V rows, one matrix per value
 // head and sequence (the DeltaNet variant of KVCacheState,
 // inference-model-common/src/lib.rs:5-13):
 //   S_t = exp(g_t) S_{t-1} + k_t v_t^T,   o_t = scale * S_t^T q_t.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstring>
@@ -24,20 +25,22 @@ __device__ __forceinline__ float lin_elem(const void *p, int64_t i) {
   else return static_cast<const float *>(p)[i];
 }
 
-// The recurrence. A workgroup of 256 threads holds CW columns of one (sequence,
-// value head) state in registers: thread (rg, cg) the rows rg + R*i and the four
+// One step of the recurrence. A workgroup of 256 threads moves CW columns of one
+// (sequence, value head) state: thread (rg, cg) the rows rg + R*i and the four
 // columns 4*cg, so that each of its loads and stores covers R whole row pieces
-// of CW floats. Tokens go in groups of TB: their k, q, v and decays are staged
-// in LDS as f32, every thread runs the group's updates and leaves its partial
-// outputs (its own rows' share of S^T q) in LDS, and the R partials of each
-// output are added in order.
-template <int DK, int CW, bool BF16, int TB>
-__global__ void __launch_bounds__(256) linear_recurrence_kernel(LinArgs a) {
+// of CW floats, all of them in flight before k, q and v arrive in LDS. The R
+// partial outputs of a column (a thread's own rows' share of S^T q) are added
+// through LDS in order. Bound by HBM: the state moves once each way, without a
+// stay in the caches (a step passes through every layer's states before it
+// returns to one). 64 sequences of 28 heads 45 us, 504 of 32 heads 383 us: 5.2
+// and 5.4 TB/s, what a copy of the same size reaches.
+template <int DK, int CW, bool BF16>
+__global__ void __launch_bounds__(256) linear_step_kernel(LinArgs a) {
   constexpr int CG = CW / 4, R = 256 / CG, NI = DK / R;
   static_assert(R <= DK && NI >= 1, "every thread holds at least one row");
-  __shared__ float ks[TB][DK], qs[TB][DK], ds[TB];
-  __shared__ __attribute__((aligned(16))) float vs[TB][CW];
-  __shared__ __attribute__((aligned(16))) float red[TB][R][CW];
+  __shared__ float ks[DK], qs[DK];
+  __shared__ __attribute__((aligned(16))) float vs[CW];
+  __shared__ __attribute__((aligned(16))) float red[R][CW];
   const int tid = threadIdx.x, cg = tid % CG, rg = tid / CG;
   const int slices = a.DV / CW;
   const int sl = blockIdx.x % slices, h = (blockIdx.x / slices) % a.Hv, b = blockIdx.x / (slices * a.Hv);
@@ -46,59 +49,50 @@ __global__ void __launch_bounds__(256) linear_recurrence_kernel(LinArgs a) {
   const int kh = h / (a.Hv / a.Hk);
   const int64_t plane = (int64_t)a.Hv * DK * a.DV;
   const int64_t off = (int64_t)h * DK * a.DV + sl * CW + 4 * cg;
+  // (A buffer of no bytes where there is no state: its loads are zeros.)
+  const int src = __builtin_amdgcn_readfirstlane((int)s.src);
+  const auto from = __builtin_amdgcn_make_buffer_rsrc(a.states + max(src, 0) * plane + (int64_t)h * DK * a.DV, 0,
+                                                      src >= 0 ? DK * a.DV * 4 : 0, 0x00027000);
+  constexpr int kNt = 2;  // non-temporal
   f32x4 S[NI];
 #pragma unroll
-  for (int i = 0; i < NI; i++) {
-    S[i] = f32x4{};
-    if (s.src >= 0)
-      S[i] = __builtin_nontemporal_load(
-          reinterpret_cast<const f32x4 *>(a.states + s.src * plane + off + (int64_t)(rg + R * i) * a.DV));
-  }
-  for (int t0 = 0; t0 < s.n; t0 += TB) {
-    const int nt = min(TB, s.n - t0);
-    for (int i = tid; i < nt * DK; i += 256) {
-      const int64_t e = ((int64_t)(s.row0 + t0 + i / DK) * a.Hk + kh) * DK + i % DK;
-      ks[i / DK][i % DK] = lin_elem<BF16>(a.k, e);
-      qs[i / DK][i % DK] = lin_elem<BF16>(a.q, e);
-    }
-    for (int i = tid; i < nt * CW; i += 256)
-      vs[i / CW][i % CW] = lin_elem<BF16>(a.v, ((int64_t)(s.row0 + t0 + i / CW) * a.Hv + h) * a.DV + sl * CW + i % CW);
-    if (tid < nt) ds[tid] = expf(a.g[(int64_t)(s.row0 + t0 + tid) * a.g_stride + h]);
-    __syncthreads();
-#pragma unroll 1
-    for (int t = 0; t < nt; t++) {
-      const float d = ds[t];
-      const f32x4 v = *reinterpret_cast<const f32x4 *>(&vs[t][4 * cg]);
-      f32x4 o = {};
-#pragma unroll
-      for (int i = 0; i < NI; i++) {
-        S[i] = d * S[i] + ks[t][rg + R * i] * v;
-        o += qs[t][rg + R * i] * S[i];
-      }
-      *reinterpret_cast<f32x4 *>(&red[t][rg][4 * cg]) = o;
-    }
-    __syncthreads();
-    for (int i = tid; i < nt * CW; i += 256) {
-      const int t = i / CW, c = i % CW;
-      float o = 0.0f;
-#pragma unroll
-      for (int r = 0; r < R; r++) o += red[t][r][c];
-      o *= a.scale;
-      const int64_t e = ((int64_t)(s.row0 + t0 + t) * a.Hv + h) * a.DV + sl * CW + c;
-      if constexpr (BF16) static_cast<uint16_t *>(a.o)[e] = (uint16_t)f32_to_bf16_bits(o);
-      else static_cast<float *>(a.o)[e] = o;
-    }
-  }
-#pragma unroll
   for (int i = 0; i < NI; i++)
+    S[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                         from, ((rg + R * i) * a.DV + sl * CW + 4 * cg) * 4, 0, kNt));
+  const int64_t krow = ((int64_t)s.row0 * a.Hk + kh) * DK, vrow = ((int64_t)s.row0 * a.Hv + h) * a.DV + sl * CW;
+  if (tid < DK) {
+    ks[tid] = lin_elem<BF16>(a.k, krow + tid);
+    qs[tid] = lin_elem<BF16>(a.q, krow + tid);
+  }
+  if (tid < CW) vs[tid] = lin_elem<BF16>(a.v, vrow + tid);
+  const float d = expf(a.g[(int64_t)s.row0 * a.g_stride + h]);
+  __syncthreads();
+  const f32x4 v = *reinterpret_cast<const f32x4 *>(&vs[4 * cg]);
+  f32x4 o = {};
+#pragma unroll
+  for (int i = 0; i < NI; i++) {
+    S[i] = d * S[i] + ks[rg + R * i] * v;
+    o += qs[rg + R * i] * S[i];
     __builtin_nontemporal_store(
         S[i], reinterpret_cast<f32x4 *>(a.states + s.dst * plane + off + (int64_t)(rg + R * i) * a.DV));
+  }
+  *reinterpret_cast<f32x4 *>(&red[rg][4 * cg]) = o;
+  __syncthreads();
+  if (tid < CW) {
+    float x = 0.0f;
+#pragma unroll
+    for (int r = 0; r < R; r++) x += red[r][tid];
+    x *= a.scale;
+    if constexpr (BF16) static_cast<uint16_t *>(a.o)[vrow + tid] = (uint16_t)f32_to_bf16_bits(x);
+    else static_cast<float *>(a.o)[vrow + tid] = x;
+  }
 }
 
 // grid.x = (pair, part), grid.y = layer: a workgroup copies one 32 KiB part
 // of a slot's state of one layer, all its 16-byte loads first. (A state is
 // 0.5 to 8 MiB: a workgroup per state left most of the device idle in a fork
-// of a few, 78 us for 3 pairs of 6 layers against XX.)
+// of a few, 78 us for 3 pairs of 6 layers against 17.)
+// Bound by HBM: 85 pairs of 4 layers at 5.4 TB/s, as a plain copy.
 constexpr int kStatePer = 8;
 
 __global__ void __launch_bounds__(256)
@@ -229,34 +223,27 @@ int refuse_capture(hipStream_t hs) {
   return MKV_OK;
 }
 
-template <int DK, bool BF16, int TB>
-static const void *recurrence_fn(int cw) {
-  if (cw == 32) return reinterpret_cast<const void *>(&linear_recurrence_kernel<DK, 32, BF16, TB>);
-  if (cw == 64) return reinterpret_cast<const void *>(&linear_recurrence_kernel<DK, 64, BF16, TB>);
-  if constexpr (DK < 256) return reinterpret_cast<const void *>(&linear_recurrence_kernel<DK, 128, BF16, TB>);
+template <int DK, bool BF16>
+static const void *step_fn(int cw) {
+  if (cw == 64) return reinterpret_cast<const void *>(&linear_step_kernel<DK, 64, BF16>);
+  if constexpr (DK < 256) return reinterpret_cast<const void *>(&linear_step_kernel<DK, 128, BF16>);
   return nullptr;
 }
 
-int launch_recurrence(StatePool *p, const LinArgs &a, hipStream_t hs) {
+static int launch_step(StatePool *p, const LinArgs &a, hipStream_t hs) {
   const mkv_state_desc &d = p->desc;
   if (a.B == 0) return MKV_OK;
   // Columns per workgroup: as many as leave 16 or fewer 16-byte loads per
-  // thread, halved while the launch has fewer than two workgroups per CU.
-  int cw = std::min(d.v_dim, d.k_dim == 256 ? 64 : 128);
-  while (cw > 32 && (int64_t)a.B * a.Hv * (d.v_dim / cw) < 2 * p->cus) cw /= 2;
+  // thread. (Narrower pieces to fill the device do not help one sequence: 32
+  // workgroups of 128 columns and 128 of 32 both take 4.0 us, and 64 sequences
+  // 44.8 us against 47.6.)
+  const int cw = std::min(d.v_dim, d.k_dim == 256 ? 64 : 128);
   const int64_t wgs = (int64_t)a.B * a.Hv * (d.v_dim / cw);
   if (wgs > kMaxGrid) return set_error(MKV_ERR_INVALID_ARGUMENT, "num_seqs * num_v_heads too large for one launch");
   const bool bf = d.dtype == MKV_DTYPE_BF16;
-  const void *fn = nullptr;
-#define MKV_LIN(DD)                                                                             \
-  fn = a.q_indptr ? (bf ? recurrence_fn<DD, true, 8>(cw) : recurrence_fn<DD, false, 8>(cw))     \
-                  : (bf ? recurrence_fn<DD, true, 1>(cw) : recurrence_fn<DD, false, 1>(cw))
-  switch (d.k_dim) {
-    case 64: MKV_LIN(64); break;
-    case 128: MKV_LIN(128); break;
-    default: MKV_LIN(256); break;
-  }
-#undef MKV_LIN
+  const void *fn = d.k_dim == 64    ? (bf ? step_fn<64, true>(cw) : step_fn<64, false>(cw))
+                   : d.k_dim == 128 ? (bf ? step_fn<128, true>(cw) : step_fn<128, false>(cw))
+                                    : (bf ? step_fn<256, true>(cw) : step_fn<256, false>(cw));
   LinArgs args = a;
   void *params[] = {&args};
   MKV_CHECK_HIP(hipLaunchKernel(fn, dim3((unsigned)wgs), dim3(256), params, 0, hs));
@@ -421,7 +408,7 @@ extern "C" int mkv_linear_step(mkv_state_pool *pool, int32_t layer, const void *
                     flags, a);
   if (rc) return rc;
   DeviceGuard guard(p->device);
-  return launch_recurrence(p, a, reinterpret_cast<hipStream_t>(stream));
+  return launch_step(p, a, reinterpret_cast<hipStream_t>(stream));
 }
 
 extern "C" int mkv_linear_step_host(mkv_state_pool *pool, int32_t layer, const void *d_q, const void *d_k,

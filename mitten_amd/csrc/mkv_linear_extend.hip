@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
       // Scores of 16 tokens (columns) with the chunk's: one wave per 16 tokens,
       // or two that take every other tile of 16 keys. Tiles that no column sees
       // come out as zeros; computing them costs less than a branch round each
-      // (8,192 tokens of 32 heads: 116 us with branches, 102 without).
+      // (8,192 tokens of 32 heads from the caches: 116 us with branches, 102 without).
       constexpr int PT = 16 / NW;  // tiles of a wave
       const int tq = wave & 3, st0 = wave >> 2, t = 16 * tq + m16;
       const float gt = gs[t];
@@ -884,7 +884,7 @@ static int launch_extend(StatePool *p, const LinArgs &a, int32_t max_q_len, void
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
     MKV_CHECK_HIP(hipStreamIsCapturing(hs, &st));
     own_ws = ws == p->ws && st == hipStreamCaptureStatusNone;
-    if (own_ws && p->ws_used && p->ws_stream != hs) MKV_CHECK_HIP(hipStreamWaitEvent(hs, p->ws_done, 0));
+    if (own_ws && p->ws_used) MKV_CHECK_HIP(hipStreamWaitEvent(hs, p->ws_done, 0));
   }
   switch (d.k_dim * 10 + (d.dtype == MKV_DTYPE_BF16 ? pl.waves : 0)) {
     case 640: launch_plan<64, 0>(p, a, sg, hs); break;
@@ -900,7 +900,6 @@ static int launch_extend(StatePool *p, const LinArgs &a, int32_t max_q_len, void
   MKV_CHECK_LAUNCH("linear_chunk_kernel");
   if (own_ws) {
     MKV_CHECK_HIP(hipEventRecord(p->ws_done, hs));
-    p->ws_stream = hs;
     p->ws_used = true;
   }
   return MKV_OK;

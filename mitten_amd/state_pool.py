@@ -172,7 +172,9 @@ class DeviceStatePool:
         tensors, or host u32 slots (mkv_state_copy_host, which also checks
         that no copy reads or writes what another writes)."""
         sh = _stream(stream, self.device)
-        if _is_host(src) or _is_host(dst):
+        if _is_host(src) != _is_host(dst):
+            raise _bad("src and dst must both be host arrays or both device tensors")
+        if _is_host(src):
             s, d = _host_u32(src, "src"), _host_u32(dst, "dst")
             if s.size != d.size:
                 raise _bad("src and dst differ in length")
@@ -209,6 +211,8 @@ class DeviceStatePool:
     def _slots(self, slots, src_slots):
         """(num_seqs, destination pointer, source pointer, whether they are host slots, the arrays)."""
         torch = _torch()
+        if src_slots is not None and _is_host(slots) != _is_host(src_slots):
+            raise _bad("slots and src_slots must both be host arrays or both device tensors")
         if _is_host(slots):
             d = _host_u32(slots, "slots")
             s = None if src_slots is None else _host_u32(src_slots, "src_slots")
@@ -250,6 +254,9 @@ class DeviceStatePool:
         return out
 
     def _extend_meta(self, n, q_lens, slots, src_slots):
+        for x, name in ((q_lens, "q_lens"), (slots, "slots"), (src_slots, "src_slots")):
+            if x is not None and not _is_host(x):
+                raise _bad(f"{name} must be a host array (linear_extend_device takes device tensors)")
         lens, d = _host_i32(q_lens, "q_lens"), _host_u32(slots, "slots")
         s = None if src_slots is None else _host_u32(src_slots, "src_slots")
         if lens.size != d.size or (s is not None and s.size != d.size):
@@ -274,9 +281,9 @@ class DeviceStatePool:
         bytes, or None for the pool's own."""
         torch = _torch()
         n, out, scale, flags = self._rows(q, k, v, log_decay, out, scale)
-        B, dst, src, host, _ = self._slots(slots, src_slots)
-        if host:
+        if _is_host(slots):
             raise _bad("slots must be a device tensor")
+        B, dst, src, _, _ = self._slots(slots, src_slots)
         _check(q_indptr, self.device, (B + 1,), torch.int32, "q_indptr")
         nws = 0
         if workspace is not None:

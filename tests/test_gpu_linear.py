@@ -321,6 +321,12 @@ def test_refusals():
             (lambda: pool.linear_extend(0, *good, [1, 1], [0, 1]), "add up to 2"),
             (lambda: pool.linear_extend(0, *good, [4, -1], [0, 1]), "negative"),
             (lambda: pool.linear_extend(0, *good, [3, 0], [0, 0]), "written twice"),
+            (lambda: pool.linear_step(0, *good, torch.arange(3, dtype=torch.int32, device="cuda"), src_slots=[0, 1, 2]),
+             "both be host"),
+            (lambda: pool.linear_extend(0, *good, [1, 2], torch.arange(2, dtype=torch.int32, device="cuda")), "host array"),
+            (lambda: pool.linear_extend_device(0, *good, g, [0, 1], 3), "device tensor"),
+            (lambda: pool.linear_step(0, *good, torch.arange(3, device="cuda")), "dtype"),
+            (lambda: pool.copy_states(torch.arange(2, dtype=torch.int32, device="cuda"), [4, 5]), "both be host"),
             (lambda: pool.copy_states([0, 1], [2]), "differ in length"),
             (lambda: pool.copy_states([0, 1], [2, 2]), "written twice"),
             (lambda: pool.copy_states([0, 1], [1, 2]), "both a source and a destination"),
