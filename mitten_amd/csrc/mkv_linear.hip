@@ -91,15 +91,25 @@ __global__ void __launch_bounds__(256) linear_step_kernel(LinArgs a) {
 // grid.x = (pair, part), grid.y = layer: a workgroup copies one 32 KiB part
 // of a slot's state of one layer, all its 16-byte loads first. (A state is
 // 0.5 to 8 MiB: a workgroup per state left most of the device idle in a fork
-// of a few, 78 us for 3 pairs of 6 layers against 17.)
+// of a few, 78 us for 3 pairs of 6 layers against 12.)
 // Bound by HBM: 85 pairs of 4 layers at 5.4 TB/s, as a plain copy.
 constexpr int kStatePer = 8;
 
-__global__ void __launch_bounds__(256)
-state_copy_kernel(float *__restrict__ states, const int32_t *__restrict__ src, const int32_t *__restrict__ dst,
-                  int64_t nslots, int64_t elems, int parts, uint32_t *__restrict__ d_err) {
+// A few pairs travel as kernel arguments (3 pairs of 6 layers 17 us with an
+// upload ahead of the launch, 12 without).
+constexpr int kArgPairs = 64;
+struct ArgPairs {
+  int32_t src[kArgPairs], dst[kArgPairs];
+};
+struct MemPairs {
+  const int32_t *src, *dst;
+};
+
+template <class Pairs>
+__global__ void __launch_bounds__(256) state_copy_kernel(float *__restrict__ states, Pairs pairs, int64_t nslots,
+                                                         int64_t elems, int parts, uint32_t *__restrict__ d_err) {
   const int pair = blockIdx.x / parts, part = blockIdx.x % parts;
-  const int32_t s = src[pair], d = dst[pair];
+  const int32_t s = pairs.src[pair], d = pairs.dst[pair];
   if (s < 0 || s >= nslots || d < 0 || d >= nslots) {
     if (part == 0 && blockIdx.y == 0 && threadIdx.x == 0) record_error(d_err, MKV_DEVERR_COPY);
     return;
@@ -346,21 +356,26 @@ extern "C" int mkv_state_pool_check(mkv_state_pool *pool, void *stream, uint32_t
 
 // ---- C ABI: copies -------------------------------------------------------------------
 
+template <class Pairs>
+static int launch_copy(StatePool *p, const Pairs &pairs, int32_t n, void *stream) {
+  const int64_t parts = (p->state_elems / 4 + 256 * kStatePer - 1) / (256 * kStatePer);
+  if (n * parts > kMaxGrid) return set_error(MKV_ERR_INVALID_ARGUMENT, "too many pairs for one launch");
+  hipLaunchKernelGGL(state_copy_kernel<Pairs>, dim3((unsigned)(n * parts), (unsigned)p->desc.num_layers), dim3(256), 0,
+                     reinterpret_cast<hipStream_t>(stream), p->data, pairs, p->desc.num_slots, p->state_elems, (int)parts,
+                     p->d_err);
+  MKV_CHECK_LAUNCH("state_copy_kernel");
+  return MKV_OK;
+}
+
 extern "C" int mkv_state_copy(mkv_state_pool *pool, const int32_t *d_src_slots, const int32_t *d_dst_slots,
                               int32_t num_pairs, void *stream) {
   if (!pool) return set_error(MKV_ERR_INVALID_ARGUMENT, "pool is NULL");
   StatePool *p = reinterpret_cast<StatePool *>(pool);
   if (num_pairs < 0) return set_error(MKV_ERR_INVALID_ARGUMENT, "num_pairs < 0");
   if (num_pairs == 0) return MKV_OK;
-  const int64_t parts = (p->state_elems / 4 + 256 * kStatePer - 1) / (256 * kStatePer);
-  if (num_pairs * parts > kMaxGrid) return set_error(MKV_ERR_INVALID_ARGUMENT, "too many pairs for one launch");
   if (!d_src_slots || !d_dst_slots) return set_error(MKV_ERR_INVALID_ARGUMENT, "NULL device pointer");
   DeviceGuard guard(p->device);
-  hipLaunchKernelGGL(state_copy_kernel, dim3((unsigned)(num_pairs * parts), (unsigned)p->desc.num_layers), dim3(256), 0,
-                     reinterpret_cast<hipStream_t>(stream), p->data, d_src_slots, d_dst_slots, p->desc.num_slots,
-                     p->state_elems, (int)parts, p->d_err);
-  MKV_CHECK_LAUNCH("state_copy_kernel");
-  return MKV_OK;
+  return launch_copy(p, MemPairs{d_src_slots, d_dst_slots}, num_pairs, stream);
 }
 
 extern "C" int mkv_state_copy_host(mkv_state_pool *pool, const uint32_t *h_src_slots, const uint32_t *h_dst_slots,
@@ -385,6 +400,12 @@ extern "C" int mkv_state_copy_host(mkv_state_pool *pool, const uint32_t *h_src_s
   DeviceGuard guard(p->device);
   hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
   if ((rc = refuse_capture(hs))) return rc;
+  if (num_pairs <= kArgPairs) {
+    ArgPairs pairs = {};
+    std::memcpy(pairs.src, h_src_slots, (size_t)num_pairs * 4);
+    std::memcpy(pairs.dst, h_dst_slots, (size_t)num_pairs * 4);
+    return launch_copy(p, pairs, num_pairs, stream);
+  }
   MetaSlot *sl = nullptr;
   if ((rc = meta_acquire(p, 2 * (size_t)num_pairs, hs, &sl))) return rc;
   std::memcpy(sl->h, h_src_slots, (size_t)num_pairs * 4);

@@ -282,6 +282,14 @@ def test_copies_and_forks():
             want = host.copy()
             want[:, dst] = host[:, src]
             assert np.array_equal(pool.tensor().cpu().numpy(), want)
+        many = DeviceStatePool(StateDesc(2, 1, 1, 64, 64, 150, "f32"))  # more pairs than travel as arguments
+        for n in (64, 65, 70):
+            was = torch.randn(many.desc.shape, device="cuda")
+            many.tensor().copy_(was)
+            many.copy_states(np.arange(n), np.arange(149, 149 - n, -1))
+            many.check()
+            was[:, 150 - n:] = was[:, :n].flip(1)
+            assert torch.equal(many.tensor(), was)
         pool.copy_states(*(torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 9, -1, 1], [5, 4, 3, -1])))
         with pytest.raises(dp.DeviceIndexError) as ei:
             pool.check()
