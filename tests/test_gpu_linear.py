@@ -142,6 +142,26 @@ def test_extend_of_long_chunks(lens, fork, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (64, 128), (128, 64), (128, 256), (256, 64), (256, 128)])
+def test_extend_in_segments(dk, dv, dtype):
+    """Prompts long enough for segments, beside short and empty ones, at every
+    head dim; the source of a sequence among them is its own or another slot."""
+    lens = [900, 0, 70, 1025]
+    with DeviceStatePool(StateDesc(1, 1, 2, dk, dv, 1, dtype)) as pool:
+        assert pool.linear_extend_workspace_size(len(lens), sum(lens), max(lens)) > 0
+    run_batch(lens, 1, 2, dk, dv, dtype, [0, 4, STATE_NONE, 4], [0, 1, 2, 3], 6, 35)
+
+
+@pytest.mark.parametrize("dk,dv", [(64, 128), (128, 128), (128, 256), (256, 128)])
+def test_extend_of_many_sequences(dk, dv):
+    """More sequences and heads than workgroups of 64 columns would fit at once."""
+    rng = np.random.default_rng(37)
+    lens = [int(x) for x in rng.integers(0, 90, 40)]
+    dst = [int(x) for x in rng.permutation(42)[:40]]
+    run_batch(lens, 2, 8, dk, dv, "bf16", [d if d % 3 else STATE_NONE for d in dst], dst, 42, 38)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("max_q_len", [0, 1, 70, 5000])
 def test_device_metadata_with_any_bound(dtype, max_q_len):
     """max_q_len sizes the launch only."""
@@ -176,17 +196,19 @@ def test_a_decay_of_minus_infinity_forgets():
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
 @pytest.mark.parametrize("where", ["v", "k", "state", "g"])
-def test_an_inf_or_nan_reaches_only_what_follows_it(dtype, bad, where):
-    """Token 70 of 150 holds it: the tokens before, and the other sequences
-    and heads, do not see it; the classes of what follows are the recurrence's."""
+@pytest.mark.parametrize("n", [150, 700])
+def test_an_inf_or_nan_reaches_only_what_follows_it(dtype, bad, where, n):
+    """Token 70 of n (whole, or in segments) holds it: the tokens before, and
+    the other sequences and heads, do not see it; the classes of what follows
+    are the recurrence's."""
     import torch
 
     hk, hv, dk, dv, at = 1, 2, 128, 64, 70
     if where == "g" and bad == np.inf:
         pytest.skip("an infinite growth has no defined state")
     rng = np.random.default_rng(81)
-    lens = [150, 20]
-    q, k, v, g = inputs(rng, 170, hk, hv, dk, dv, "f32")
+    lens = [n, 20]
+    q, k, v, g = inputs(rng, n + 20, hk, hv, dk, dv, "f32")
     if dtype == "bf16":
         q, k, v = (widen(orc.f32_to_bf16(x)) for x in (q, k, v))
     host = rng.standard_normal((1, 2, hv, dk, dv)).astype(np.float32)
