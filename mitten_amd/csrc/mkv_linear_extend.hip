@@ -10,6 +10,7 @@
 #include <cmath>
 #include <cstring>
 #include <new>
+#include <type_traits>
 
 #include "mkv_linear.h"
 
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
       z = fmaf(S[j][i], 0.0f, z);
     }
   }
-  double total = 0.0, g_end = 0.0;  // summed log2 decays of the segment so far, and of this chunk (wave NW - 4)
+  double total = 0.0, g_end = 0.0;  // summed log2 decays of the segment so far, and of this chunk (wave NW - 1)
   if (tid == 0) odd_s = 0;
 
   const uint8_t *kp = static_cast<const uint8_t *>(a.k) + ((int64_t)s.row0 * a.Hk + kh) * KRB;
@@ -241,7 +242,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
 #pragma unroll
     for (int i = 0; i < VL; i++) vr[i] = buffer_load16(r, v_off + i * (T / VC) * (uint32_t)vrs);
   };
-  // Token t0 + lane's decay, and (wave NW - 4, which has the fewest scores) a chunk's
+  // Token t0 + lane's decay, and (wave NW - 1, which has one tile of scores) a chunk's
   // vectors from it.
   auto load_g = [&](int t0) {
     const bool any = t0 < t_end;
@@ -287,7 +288,11 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
   load_k(t_begin);
   load_q(t_begin);
   load_v(t_begin);
-  if (wave == NW - 4) g_end = vectors(t_begin, 0);
+  if constexpr (OUT) {
+#pragma unroll
+    for (int i = 0; i < kChunk * 128 / (16 * T); i++) *reinterpret_cast<u32x4 *>(pt + (tid + T * i) * 16) = u32x4{};
+  }
+  if (wave == NW - 1) g_end = vectors(t_begin, 0);
   gr = load_g(t_begin + kChunk);
   __syncthreads();  // (odd_s is set)
   stage(1);
@@ -311,51 +316,61 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
     // The next chunk's rows are asked for in three parts between the products.
     load_k(t0 + kChunk);
     double next_end = 0.0;
-    if (wave == NW - 4) next_end = vectors(t0 + kChunk, chunk & 1);
+    if (wave == NW - 1) next_end = vectors(t0 + kChunk, chunk & 1);
     gr = load_g(t0 + 2 * kChunk);
 
     f32x4 acc[4];
     if constexpr (OUT) {
-      // Scores of 16 tokens (columns) with the chunk's: one wave per 16 tokens,
-      // or two that take every other tile of 16 keys. Tiles that no column sees
-      // come out as zeros; computing them costs less than a branch round each
-      // (8,192 tokens of 32 heads from the caches: 116 us with branches, 102 without).
-      constexpr int PT = 16 / NW;  // tiles of a wave
-      const int tq = wave & 3, st0 = wave >> 2, t = 16 * tq + m16;
-      const float gt = gs[t];
+      // Scores: the ten tiles of 16 tokens (columns) by 16 keys on and below the
+      // diagonal, up to three per wave; the two above it that a product of 32
+      // keys reaches over are zeros from the start. A wave's tiles are straight
+      // code: with a branch round each they wait for one another.
       auto read16 = [&](const uint8_t *tile, int at, int p) {  // 16 rows by 32 columns from column 32 p on
         return join_b64(*reinterpret_cast<const uint64_t *>(tile + (at ^ (p * 64))),
                         *reinterpret_cast<const uint64_t *>(tile + (at ^ (p * 64 + 32))));
       };
-      f32x4 c[PT];
+      auto scores = [&](auto count, int n0, int step) {
+        constexpr int N = decltype(count)::value;
+        int tq[N], st[N];
+        f32x4 c[N], gk[N], r[N];
+        float gt[N], e[N];
 #pragma unroll
-      for (int p = 0; p < NP; p++) {
-        const bf16x8 qf = read16(qt + tq * 16 * KRB, q_row, p);
-#pragma unroll
-        for (int u = 0; u < PT; u++) {
-          const bf16x8 kf = read16(kt + (st0 + u * (NW / 4)) * 16 * KRB, k_at[u], p);
-          c[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf, p ? c[u] : f32x4{}, 0, 0, 0);
+        for (int u = 0; u < N; u++) {  // tiles by rows from the last one: (3, 0) .. (3, 3), (2, 0) .. (0, 0)
+          const int n = n0 + step * u;
+          tq[u] = n < 4 ? 3 : n < 7 ? 2 : n < 9 ? 1 : 0;
+          st[u] = n - (n < 4 ? 0 : n < 7 ? 4 : n < 9 ? 7 : 9);
+          gt[u] = gs[16 * tq[u] + m16];
+          e[u] = gs[16 * st[u] + 15];
+          gk[u] = *reinterpret_cast<const f32x4 *>(&gs[16 * st[u] + 4 * g4]);
+          r[u] = *reinterpret_cast<const f32x4 *>(&rs[16 * st[u] + 4 * g4]);
         }
-      }
 #pragma unroll
-      for (int u = 0; u < PT; u++) {
-        const int st = st0 + u * (NW / 4);
-        if (st < tq) {  // e^{G_t - G_end of tile} e^{G_end of tile - G_k}: one exponential per lane
-          const float e = exp2_f(gt - gs[16 * st + 15]) * a.scale;
-          const f32x4 r = *reinterpret_cast<const f32x4 *>(&rs[16 * st + 4 * g4]);
+        for (int p = 0; p < NP; p++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) c[u][i] *= e * r[i];
-        } else {
-          const f32x4 gk = *reinterpret_cast<const f32x4 *>(&gs[16 * st + 4 * g4]);
-#pragma unroll
-          for (int i = 0; i < 4; i++) {  // (selected, not multiplied: past t it may be anything)
-            const float e = exp2_f(gt - gk[i]) * a.scale;
-            c[u][i] = 16 * st + 4 * g4 + i <= t ? c[u][i] * e : 0.0f;
+          for (int u = 0; u < N; u++) {
+            const bf16x8 qf = read16(qt + tq[u] * 16 * KRB, q_at[u], p), kf = read16(kt + st[u] * 16 * KRB, k_at[u], p);
+            c[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf, p ? c[u] : f32x4{}, 0, 0, 0);
           }
+#pragma unroll
+        for (int u = 0; u < N; u++) {
+          if (st[u] < tq[u]) {  // e^{G_t - G_end of tile} e^{G_end of tile - G_k}: one exponential per lane
+            const float f = exp2_f(gt[u] - e[u]) * a.scale;
+#pragma unroll
+            for (int i = 0; i < 4; i++) c[u][i] *= f * r[u][i];
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {  // (selected, not multiplied: past t it may be anything)
+              const float f = exp2_f(gt[u] - gk[u][i]) * a.scale;
+              c[u][i] = 4 * g4 + i <= m16 ? c[u][i] * f : 0.0f;
+            }
+          }
+          *reinterpret_cast<uint64_t *>(pt + (p_row ^ (st[u] * 32)) + tq[u] * 16 * 128) =
+              (uint64_t)pack_bf16x2(c[u][2], c[u][3]) << 32 | pack_bf16x2(c[u][0], c[u][1]);
         }
-        *reinterpret_cast<uint64_t *>(pt + (p_row ^ (st * 32)) + tq * 16 * 128) =
-            (uint64_t)pack_bf16x2(c[u][2], c[u][3]) << 32 | pack_bf16x2(c[u][0], c[u][1]);
-      }
+      };
+      constexpr int kFull = NW == 8 ? 2 : 3;  // waves with NW == 8 ? 2 : 3 tiles; the others have one
+      if (wave < kFull) scores(std::integral_constant<int, kFull>(), NW == 8 ? wave : 3 * wave, NW == 8 ? 8 : 1);
+      else scores(std::integral_constant<int, 1>(), NW == 8 ? wave : 9, 0);
       load_q(t0 + kChunk);
       // O^T from the state.
 #pragma unroll
@@ -485,7 +500,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
   }
 
   if constexpr (MODE == kLocal) {
-    if (tid == 64 * (NW - 4) && sl == 0)
+    if (tid == 64 * (NW - 1) && sl == 0)
       sg.decay[((int64_t)b * sg.nseg + seg) * a.Hv + h] = exp2_f((float)total);
 #pragma unroll
     for (int j = 0; j < DK / 16; j++) *reinterpret_cast<f32x4 *>(frag + j * 256) = S[j];
