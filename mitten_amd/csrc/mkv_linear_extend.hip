@@ -375,21 +375,17 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
       // O^T from the state.
 #pragma unroll
       for (int p = 0; p < NP; p++) {
-        bf16x8 sf;
         const f32x4 x = S[2 * p], y = S[2 * p + 1];
-        sf = __builtin_bit_cast(bf16x8, u32x4{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
-                                                 pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])});
+        const bf16x8 sf = __builtin_bit_cast(bf16x8, u32x4{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
+                                                           pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])});
 #pragma unroll
         for (int tt = 0; tt < 4; tt++) {
           const bf16x8 q = read16(qt + tt * 16 * KRB, q_at[tt], p);
-            acc[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sf, q, p ? acc[tt] : f32x4{}, 0, 0, 0);
+          acc[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sf, q, p ? acc[tt] : f32x4{}, 0, 0, 0);
         }
       }
-  #pragma unroll
-      for (int tt = 0; tt < 4; tt++) {
-        const float e = es[16 * tt + m16];
-        acc[tt] *= e;
-      }
+#pragma unroll
+      for (int tt = 0; tt < 4; tt++) acc[tt] *= es[16 * tt + m16];
       __syncthreads();  // the scores are written
     }
 
@@ -423,8 +419,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
     g_end = next_end;
     const float dend = gend2[(chunk - 1) & 1];
 #pragma unroll
-    for (int j = 0; j < DK / 16; j++)
-      S[j] *= dend;
+    for (int j = 0; j < DK / 16; j++) S[j] *= dend;
 #pragma unroll
     for (int x = 0; x < 2; x++) {  // 32 tokens
       uint32_t wv[TERMS][4];       // w V: high, middle and low bits
@@ -451,10 +446,9 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
         const i16x4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(at + 16 * KRB));
         const bf16x8 kf = join_b64(__builtin_bit_cast(uint64_t, lo), __builtin_bit_cast(uint64_t, hi));
 #pragma unroll
-          for (int u = 0; u < TERMS; u++)
-            S[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                kf, __builtin_bit_cast(bf16x8, u32x4{wv[u][0], wv[u][1], wv[u][2], wv[u][3]}), S[j], 0,
-                0, 0);
+        for (int u = 0; u < TERMS; u++)
+          S[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              kf, __builtin_bit_cast(bf16x8, u32x4{wv[u][0], wv[u][1], wv[u][2], wv[u][3]}), S[j], 0, 0, 0);
       }
     }
     t0 += kChunk;
@@ -474,9 +468,8 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
     const double l = log2_decay(a.g[(int64_t)(s.row0 + t0) * a.g_stride + h]);
     const float d = exp2_f((float)l);
     total += l;
-    float v, o;
-    v = __uint_as_float((uint32_t)static_cast<const uint16_t *>(a.v)[vrow] << 16);
-    o = 0.0f;
+    const float v = __uint_as_float((uint32_t)static_cast<const uint16_t *>(a.v)[vrow] << 16);
+    float o = 0.0f;
 #pragma unroll
     for (int j = 0; j < DK / 16; j++) {
       const uint2 kw = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.k) + krow + 16 * j);
@@ -487,10 +480,10 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
         q[0] = bf16_lo(qw.x), q[1] = bf16_hi(qw.x), q[2] = bf16_lo(qw.y), q[3] = bf16_hi(qw.y);
       }
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          S[j][i] = d * S[j][i] + k[i] * v;
-          if constexpr (OUT) o += q[i] * S[j][i];
-        }
+      for (int i = 0; i < 4; i++) {
+        S[j][i] = d * S[j][i] + k[i] * v;
+        if constexpr (OUT) o += q[i] * S[j][i];
+      }
     }
     if constexpr (OUT) {
       o += __shfl_xor(o, 16);
@@ -800,8 +793,10 @@ __global__ void __launch_bounds__(256) linear_scan_kernel(LinArgs a, LinSegs sg,
     for (int u = 0; u < U; u++) {
       if (j0 + u >= ns) break;
       *reinterpret_cast<f32x4 *>(at + (j0 + u) * plane) = S;
-      // (An infinity in S stays one under a decay that is 0 only by underflow.)
-      S = (d[u] < 1.17549435e-38f ? 1.17549435e-38f : d[u]) * S + l[u];
+      // (An infinity stays one under a product of decays that is 0 only by underflow.)
+      const bool gone = d[u] < 1.17549435e-38f;
+#pragma unroll
+      for (int i = 0; i < 4; i++) S[i] = (gone && isinf(S[i]) ? S[i] : d[u] * S[i]) + l[u][i];
     }
   }
 #pragma unroll

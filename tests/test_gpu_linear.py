@@ -194,6 +194,26 @@ def test_a_decay_of_minus_infinity_forgets():
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n", [1, 60, 700])
+def test_a_large_state_is_forgotten_wholly(dtype, n):
+    """A finite state of 1e36 behind a decay of minus infinity leaves nothing,
+    in one step, one chunk and in segments."""
+    import torch
+
+    rng = np.random.default_rng(72)
+    q, k, v, g = inputs(rng, n, 1, 2, 64, 64, dtype)
+    g[0] = -np.inf
+    v[:] = 0
+    with DeviceStatePool(StateDesc(1, 1, 2, 64, 64, 1, dtype)) as pool:
+        pool.tensor().fill_(1e36)
+        if n == 1:
+            o = pool.linear_step(0, *(to_device(x) for x in (q, k, v, g)), [0])
+        else:
+            o = pool.linear_extend(0, *(to_device(x) for x in (q, k, v, g)), np.array([n], np.int32), [0])
+        assert not torch.any(o.cpu() != 0) and not torch.any(pool.tensor().cpu() != 0)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
 @pytest.mark.parametrize("where", ["v", "k", "state", "g"])
 @pytest.mark.parametrize("n", [150, 700])
