@@ -329,8 +329,21 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
         return join_b64(*reinterpret_cast<const uint64_t *>(tile + (at ^ (p * 64))),
                         *reinterpret_cast<const uint64_t *>(tile + (at ^ (p * 64 + 32))));
       };
-      auto scores = [&](auto count, int n0, int step) {
+      // O^T from the state, 32 of its rows.
+      auto from_state = [&](int p, bf16x8 q[4]) {
+        const f32x4 x = S[2 * p], y = S[2 * p + 1];
+        const bf16x8 sf = __builtin_bit_cast(bf16x8, u32x4{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
+                                                           pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])});
+#pragma unroll
+        for (int tt = 0; tt < 4; tt++) {
+          q[tt] = read16(qt + tt * 16 * KRB, q_at[tt], p);
+          acc[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sf, q[tt], p ? acc[tt] : f32x4{}, 0, 0, 0);
+        }
+      };
+      // N tiles from n0 on; JOINT (constant n0): with the outputs from the state, off one read of q.
+      auto scores = [&](auto count, auto joint, int n0, int step) {
         constexpr int N = decltype(count)::value;
+        constexpr bool JOINT = decltype(joint)::value;
         int tq[N], st[N];
         f32x4 c[N], gk[N], r[N];
         float gt[N], e[N];
@@ -345,12 +358,16 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
           r[u] = *reinterpret_cast<const f32x4 *>(&rs[16 * st[u] + 4 * g4]);
         }
 #pragma unroll
-        for (int p = 0; p < NP; p++)
+        for (int p = 0; p < NP; p++) {
+          bf16x8 q[4];
+          if constexpr (JOINT) from_state(p, q);
 #pragma unroll
           for (int u = 0; u < N; u++) {
-            const bf16x8 qf = read16(qt + tq[u] * 16 * KRB, q_at[u], p), kf = read16(kt + st[u] * 16 * KRB, k_at[u], p);
+            const bf16x8 qf = JOINT ? q[tq[u]] : read16(qt + tq[u] * 16 * KRB, q_at[u], p);
+            const bf16x8 kf = read16(kt + st[u] * 16 * KRB, k_at[u], p);
             c[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf, p ? c[u] : f32x4{}, 0, 0, 0);
           }
+        }
 #pragma unroll
         for (int u = 0; u < N; u++) {
           if (st[u] < tq[u]) {  // e^{G_t - G_end of tile} e^{G_end of tile - G_k}: one exponential per lane
@@ -368,20 +385,23 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
               (uint64_t)pack_bf16x2(c[u][2], c[u][3]) << 32 | pack_bf16x2(c[u][0], c[u][1]);
         }
       };
-      constexpr int kFull = NW == 8 ? 2 : 3;  // waves with NW == 8 ? 2 : 3 tiles; the others have one
-      if (wave < kFull) scores(std::integral_constant<int, kFull>(), NW == 8 ? wave : 3 * wave, NW == 8 ? 8 : 1);
-      else scores(std::integral_constant<int, 1>(), NW == 8 ? wave : 9, 0);
-      load_q(t0 + kChunk);
-      // O^T from the state.
+      const std::true_type with_state;
+      const std::false_type alone;
+      if constexpr (NW == 4) {
+        const std::integral_constant<int, 3> three;
+        if (wave == 0) scores(three, with_state, 0, 1);
+        else if (wave == 1) scores(three, with_state, 3, 1);
+        else if (wave == 2) scores(three, with_state, 6, 1);
+        else scores(std::integral_constant<int, 1>(), with_state, 9, 0);
+        load_q(t0 + kChunk);
+      } else {
+        if (wave < 2) scores(std::integral_constant<int, 2>(), alone, wave, 8);
+        else scores(std::integral_constant<int, 1>(), alone, wave, 0);
+        load_q(t0 + kChunk);
 #pragma unroll
-      for (int p = 0; p < NP; p++) {
-        const f32x4 x = S[2 * p], y = S[2 * p + 1];
-        const bf16x8 sf = __builtin_bit_cast(bf16x8, u32x4{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
-                                                           pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])});
-#pragma unroll
-        for (int tt = 0; tt < 4; tt++) {
-          const bf16x8 q = read16(qt + tt * 16 * KRB, q_at[tt], p);
-          acc[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sf, q, p ? acc[tt] : f32x4{}, 0, 0, 0);
+        for (int p = 0; p < NP; p++) {
+          bf16x8 q[4];
+          from_state(p, q);
         }
       }
 #pragma unroll
