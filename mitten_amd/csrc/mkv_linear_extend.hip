@@ -115,6 +115,12 @@ __device__ __forceinline__ bf16x8 join_b64(uint64_t a, uint64_t b) {
   return __builtin_bit_cast(bf16x8, u32x4{(uint32_t)a, (uint32_t)(a >> 32), (uint32_t)b, (uint32_t)(b >> 32)});
 }
 
+// Two tiles' accumulators, rounded, as an operand of 32 rows.
+__device__ __forceinline__ bf16x8 round_rows(f32x4 x, f32x4 y) {
+  return __builtin_bit_cast(bf16x8, u32x4{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
+                                          pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])});
+}
+
 // ===========================================================================
 // bf16 rows. One workgroup of NW waves per (sequence, segment, value head,
 // slice of 16 NW columns); wave w holds columns 16 w .. of the state, all DK
@@ -329,21 +335,10 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
         return join_b64(*reinterpret_cast<const uint64_t *>(tile + (at ^ (p * 64))),
                         *reinterpret_cast<const uint64_t *>(tile + (at ^ (p * 64 + 32))));
       };
-      // O^T from the state, 32 of its rows.
-      auto from_state = [&](int p, bf16x8 q[4]) {
-        const f32x4 x = S[2 * p], y = S[2 * p + 1];
-        const bf16x8 sf = __builtin_bit_cast(bf16x8, u32x4{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
-                                                           pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])});
-#pragma unroll
-        for (int tt = 0; tt < 4; tt++) {
-          q[tt] = read16(qt + tt * 16 * KRB, q_at[tt], p);
-          acc[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sf, q[tt], p ? acc[tt] : f32x4{}, 0, 0, 0);
-        }
-      };
-      // N tiles from n0 on; JOINT (constant n0): with the outputs from the state, off one read of q.
-      auto scores = [&](auto count, auto joint, int n0, int step) {
+      // N tiles from n0 on. Four waves form O^T from the state with them, off one
+      // read of q (their n0 is a constant, and so is the tile of q each takes).
+      auto scores = [&](auto count, int n0, int step) {
         constexpr int N = decltype(count)::value;
-        constexpr bool JOINT = decltype(joint)::value;
         int tq[N], st[N];
         f32x4 c[N], gk[N], r[N];
         float gt[N], e[N];
@@ -360,10 +355,17 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
 #pragma unroll
         for (int p = 0; p < NP; p++) {
           bf16x8 q[4];
-          if constexpr (JOINT) from_state(p, q);
+          if constexpr (NW == 4) {
+            const bf16x8 sf = round_rows(S[2 * p], S[2 * p + 1]);
+#pragma unroll
+            for (int tt = 0; tt < 4; tt++) {
+              q[tt] = read16(qt + tt * 16 * KRB, q_at[tt], p);
+              acc[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sf, q[tt], p ? acc[tt] : f32x4{}, 0, 0, 0);
+            }
+          }
 #pragma unroll
           for (int u = 0; u < N; u++) {
-            const bf16x8 qf = JOINT ? q[tq[u]] : read16(qt + tq[u] * 16 * KRB, q_at[u], p);
+            const bf16x8 qf = NW == 4 ? q[tq[u]] : read16(qt + tq[u] * 16 * KRB, q_at[u], p);
             const bf16x8 kf = read16(kt + st[u] * 16 * KRB, k_at[u], p);
             c[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf, p ? c[u] : f32x4{}, 0, 0, 0);
           }
@@ -385,23 +387,27 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
               (uint64_t)pack_bf16x2(c[u][2], c[u][3]) << 32 | pack_bf16x2(c[u][0], c[u][1]);
         }
       };
-      const std::true_type with_state;
-      const std::false_type alone;
-      if constexpr (NW == 4) {
-        const std::integral_constant<int, 3> three;
-        if (wave == 0) scores(three, with_state, 0, 1);
-        else if (wave == 1) scores(three, with_state, 3, 1);
-        else if (wave == 2) scores(three, with_state, 6, 1);
-        else scores(std::integral_constant<int, 1>(), with_state, 9, 0);
-        load_q(t0 + kChunk);
+      constexpr int kFull = NW == 8 ? 2 : 3;  // that many waves have that many tiles, the others one
+      const std::integral_constant<int, kFull> full;
+      const std::integral_constant<int, 1> one;
+      if constexpr (NW == 8) {
+        if (wave < kFull) scores(full, wave, 8);
+        else scores(one, wave, 0);
       } else {
-        if (wave < 2) scores(std::integral_constant<int, 2>(), alone, wave, 8);
-        else scores(std::integral_constant<int, 1>(), alone, wave, 0);
-        load_q(t0 + kChunk);
+        if (wave == 0) scores(full, 0, 1);
+        else if (wave == 1) scores(full, 3, 1);
+        else if (wave == 2) scores(full, 6, 1);
+        else scores(one, 9, 0);
+      }
+      load_q(t0 + kChunk);
+      // O^T from the state: eight waves, which have no registers for more at once.
 #pragma unroll
-        for (int p = 0; p < NP; p++) {
-          bf16x8 q[4];
-          from_state(p, q);
+      for (int p = 0; p < (NW == 8 ? NP : 0); p++) {
+        const bf16x8 sf = round_rows(S[2 * p], S[2 * p + 1]);
+#pragma unroll
+        for (int tt = 0; tt < 4; tt++) {
+          const bf16x8 q = read16(qt + tt * 16 * KRB, q_at[tt], p);
+          acc[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sf, q, p ? acc[tt] : f32x4{}, 0, 0, 0);
         }
       }
 #pragma unroll
