@@ -128,8 +128,8 @@ __device__ __forceinline__ bf16x8 round_rows(f32x4 x, f32x4 y) {
 // 4 g .. 4 g + 3), which are the operand layout of the product with q:
 //   O^T = S^T Q^T      S tiles 2p and 2p + 1 as one operand of 32 rows, rounded
 //                      to bf16 (2^-8 of a term: as much as the output's own rounding)
-//   P   = K Q^T        each wave 16 tokens' scores, decayed and masked, through
-//                      LDS as bf16 (as attention rounds its weights)
+//   P   = K Q^T        tiles of 16 keys by 16 tokens dealt over the waves, decayed
+//                      and masked, through LDS as bf16 (as attention rounds its weights)
 //   O^T += V^T P^T     V^T by the transposing LDS read
 //   S   = e^G S + K^T (w V)   w V in f32 split into three bf16 (8 + 8 + 8 bits
 //                      by truncation), so that the state keeps f32's accuracy
@@ -851,14 +851,17 @@ struct LinPlan {
   int nseg, len;  // segments per sequence, tokens of one
 };
 
-// The costs are measured ones in microseconds at head dims of 128 on 256 CUs
-// (other dims scale both sides alike): whole sequences, `lone` per chunk of 64
-// tokens of the longest or `full` per chunk and CU (of 128 columns; f32: 64);
-// segments, `seg` per chunk of one round of workgroups or `segs` of each of
-// several, 12 for three launches, and the states between them, written,
-// scanned and read at 5 TB/s. Measured against whole: 2,000 tokens of 32 heads 51-56 us (whole 130), 600 tokens 34
-// (46), 300 tokens whole 22 (28 in segments), 8 prompts of 300-1,500 tokens of
-// 28 heads whole 76 (109), f32 2,000 tokens of 14 heads of 64 37 (202).
+// The costs are measured ones in microseconds at a k_dim of 128 (f32: 64) on 256
+// CUs: whole sequences, `lone` per chunk of 64 tokens of the longest or `full`
+// per chunk and CU (of 128 columns; f32: 64); segments, `seg` per chunk of one
+// round of workgroups or `segs` of each of several, 12 for three launches, and
+// the states between them, written, scanned and read at 5 TB/s. A chunk's
+// products grow with k_dim, its latency (most of `lone`) less. Measured against
+// the other way: 2,000 tokens of 32 heads of 128 in segments 52 us (whole 134),
+// 600 tokens 34 (47), 300 tokens whole 21 (28), 8 prompts of 300-1,500 tokens of
+// 28 heads whole 69 (108), 2 of 1,000-2,000 of 8 heads of 256 in segments 64
+// (155); f32 2,000 tokens of 14 heads of 64 37 (201), 2 of 500-1,000 of 16 heads
+// of 128 65 (133; 89 in the segments that costs without k_dim choose).
 static LinPlan plan_extend(const StatePool *p, int64_t num_seqs, int64_t num_tokens, int64_t max_q_len,
                            uint64_t ws_bytes) {
   const mkv_state_desc &d = p->desc;
@@ -867,7 +870,9 @@ static LinPlan plan_extend(const StatePool *p, int64_t num_seqs, int64_t num_tok
   const int64_t chunks = std::min(num_seqs * longest, num_tokens / kChunk + num_seqs);
   const int cols = f32 || d.v_dim == 64 ? 64 : 128;  // of a workgroup over segments
   const double load = (double)chunks * d.num_v_heads * d.v_dim / (f32 ? 64 : 128) / p->cus;
-  const double lone = f32 ? 6.8 : 3.6, full = f32 ? 5.6 : 3.3, seg = f32 ? 8.4 : 7.4, segs = f32 ? 6.0 : 6.2;
+  const double dim = d.k_dim / (f32 ? 64.0 : 128.0);
+  const double lone = (f32 ? 6.8 : 3.6) * std::min(dim, (1.0 + dim) / 2), full = (f32 ? 5.6 : 3.3) * dim;
+  const double seg = (f32 ? 8.4 : 7.4) * dim, segs = (f32 ? 6.0 : 6.2) * dim;
   LinPlan r = {cols / 16, 1, INT_MAX & ~(kChunk - 1)};
   double best = std::max(lone * longest, full * load);
   for (int64_t want = 1; want < longest && want * segs < best; want++) {  // chunks of a segment
@@ -884,7 +889,7 @@ static LinPlan plan_extend(const StatePool *p, int64_t num_seqs, int64_t num_tok
     }
   }
   // Whole sequences of bf16 take 64 columns a workgroup while two to a CU hold
-  // them all (8 prompts of 300-1,500 tokens, 28 heads: 76 us against 81 with
+  // them all (8 prompts of 300-1,500 tokens, 28 heads: 69 us against 85 with
   // 128), else 128, which form the scores once for twice the columns.
   if (r.nseg == 1 && num_seqs * d.num_v_heads * (d.v_dim / 64) <= 2 * p->cus) r.waves = 4;
   return r;
