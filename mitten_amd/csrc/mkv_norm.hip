@@ -183,6 +183,7 @@ extern "C" int mkv_add_rms_norm(int device, const void *d_x, const void *d_resid
   if (num_rows == 0) return MKV_OK;
   if (!d_fp8 != !d_scales) return set_error(MKV_ERR_INVALID_ARGUMENT, "give both the e4m3 output and its scales, or neither");
   if (!d_out && !d_fp8) return set_error(MKV_ERR_INVALID_ARGUMENT, "no output asked for");
+  if (d_sum && d_sum == d_out) return set_error(MKV_ERR_INVALID_ARGUMENT, "d_sum and d_out are the same");
   if (group && (!d_fp8 || group < 8 || group % 8 || group > dim || dim % group))
     return set_error(MKV_ERR_INVALID_ARGUMENT,
                      "group (%d) must be 0 (one scale per row) or a multiple of 8 that divides dim (%d), with an e4m3 output",

@@ -63,3 +63,10 @@ def test_norm_refusals(change, msg):
     st = lib.mkv_add_rms_norm(0, p(64), None, p(80), a["eps"], a["rows"], a["dim"], a["dtype"], None, p(a["out"]),
                               p(a["fp8"]), p(a["scales"]), a["group"], None)
     assert st == 1 and msg in lib.mkv_last_error().decode()
+
+
+def test_norm_refuses_one_buffer_for_two_outputs():
+    lib = _lib.device_lib()
+    p = ctypes.c_void_p
+    st = lib.mkv_add_rms_norm(0, p(64), p(96), p(80), 1e-6, 4, 64, 1, p(16), p(16), None, None, 0, None)
+    assert st == 1 and "same" in lib.mkv_last_error().decode()
