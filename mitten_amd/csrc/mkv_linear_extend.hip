@@ -875,7 +875,9 @@ static LinPlan plan_extend(const StatePool *p, int64_t num_seqs, int64_t num_tok
   const double seg = (f32 ? 8.4 : 7.4) * dim, segs = (f32 ? 6.0 : 6.2) * dim;
   LinPlan r = {cols / 16, 1, INT_MAX & ~(kChunk - 1)};
   double best = std::max(lone * longest, full * load);
-  for (int64_t want = 1; want < longest && want * segs < best; want++) {  // chunks of a segment
+  for (int64_t want = 1; want < longest && want * segs < best; want += 1 + want / 64) {
+    // Chunks of a segment, to 2%: max_q_len may be a loose bound, and the steps are
+    // the same whatever the workspace holds.
     const int64_t nseg = (longest + want - 1) / want;
     const uint64_t bytes = segs_bytes(p, num_seqs, nseg);
     if (bytes > ws_bytes) continue;
@@ -913,7 +915,8 @@ static int launch_extend(StatePool *p, const LinArgs &a, int32_t max_q_len, void
   if (a.B == 0) return MKV_OK;
   const LinPlan pl = plan_extend(p, a.B, a.num_tokens, max_q_len, ws_bytes);
   const int64_t wgs = ((int64_t)a.B * pl.nseg * a.Hk + 7) / 8 * 8 * (a.Hv / a.Hk) * (d.v_dim / (16 * pl.waves));
-  if (wgs * (pl.waves / 4) > kMaxGrid || (int64_t)a.B * a.Hv * (d.k_dim * d.v_dim / 1024) > kMaxGrid)
+  if (wgs * (pl.waves / 4) > kMaxGrid ||
+      (pl.nseg > 1 && (int64_t)a.B * a.Hv * (d.k_dim * d.v_dim / 1024) > kMaxGrid))
     return set_error(MKV_ERR_INVALID_ARGUMENT, "num_seqs * num_v_heads too large for one launch");
   LinSegs sg = {pl.nseg, pl.len, nullptr, nullptr};
   // Calls on different streams that share the pool's workspace follow one

@@ -490,6 +490,57 @@ def test_a_prompt_then_steps_as_an_engine_runs_them():
             check_close(st[layer, slot], rs, f32_bound(n[b], dk, as_), f"state {b}")
 
 
+def test_thousands_of_sequences_of_large_states():
+    """4,100 sequences of 64 heads of 256 x 256 (the scan over segments could
+    not be launched for them, and need not be). One has a slot; the others'
+    are outside the pool, and are reported."""
+    import torch
+
+    rng = np.random.default_rng(93)
+    q, k, v, g = inputs(rng, 1, 1, 64, 256, 256, "bf16")
+    B = 4100
+    with DeviceStatePool(StateDesc(1, 1, 64, 256, 256, 1, "bf16")) as pool:
+        pool.tensor().zero_()
+        ip = torch.ones(B + 1, dtype=torch.int32, device="cuda")
+        ip[0] = 0
+        slots = torch.ones(B, dtype=torch.int32, device="cuda")
+        slots[0] = 0
+        assert pool.linear_extend_workspace_size(B, 1, 1) == 0
+        o = pool.linear_extend_device(0, *(to_device(x) for x in (q, k, v, g)), ip, slots, 1)
+        with pytest.raises(dp.DeviceIndexError) as ei:
+            pool.check()
+        assert ei.value.bits == dp.DEVERR_SLOT
+        ro, rs, ao, as_ = reference(*(widen(x) for x in (q, k, v)), g, np.zeros((64, 256, 256)), 1 / 16)
+        check_close(widen(to_host(o)), ro, out_bound(1, 256, "bf16", ro, ao), "outputs")
+        check_close(pool.tensor().cpu().numpy()[0, 0], rs, f32_bound(1, 256, as_), "state")
+
+
+def test_a_loose_bound_on_the_lengths_costs_no_time():
+    """max_q_len is only a bound: the largest one is planned as fast as any."""
+    import time
+
+    import torch
+
+    rng = np.random.default_rng(94)
+    q, k, v, g = (to_device(x) for x in inputs(rng, 5, 1, 64, 256, 256, "bf16"))
+    with DeviceStatePool(StateDesc(1, 1, 64, 256, 256, 1, "bf16")) as pool:
+        ip, slots = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 5], [0]))
+        outs, times = [], []
+        for bound in (5, 2 ** 31 - 1):
+            pool.tensor().zero_()
+            pool.linear_extend_device(0, q, k, v, g, ip, slots, bound)
+            pool.tensor().zero_()
+            torch.cuda.synchronize()
+            t = time.perf_counter()
+            outs.append(pool.linear_extend_device(0, q, k, v, g, ip, slots, bound).float())
+            times.append(time.perf_counter() - t)
+            torch.cuda.synchronize()
+        ro, _, ao, _ = reference(*(widen(to_host(x)) for x in (q, k, v)), to_host(g), np.zeros((64, 256, 256)), 1 / 16)
+        for o in outs:
+            check_close(o.cpu().numpy(), ro, out_bound(5, 256, "bf16", ro, ao), "outputs")
+        assert times[1] < 0.02 + times[0]
+
+
 @pytest.mark.parametrize("i", range(16))
 def test_random_batches(i):
     rng = np.random.default_rng(900 + i)
