@@ -543,8 +543,9 @@ MKV_API int mkv_linear_step_host(mkv_state_pool *pool, int32_t layer, const void
  * longer chunk is computed all the same); an indptr that falls back or
  * leaves [0, num_tokens] is reported (MKV_DEVERR_CTX) and its sequence
  * skipped. Slots, types and forms as in mkv_linear_step; sums, decays and
- * states are f32 or wider, and with bf16 rows an output also carries the
- * rounding of scores and of the state it reads to bf16.
+ * states are f32 or wider; with bf16 rows the scores, and the state where an
+ * output reads it, enter products in 16 bits (2^-15 of a term; a term of the
+ * states between segments 2^-14), and the output is rounded once.
  * Where few long sequences would leave the device idle, their chunks are cut
  * into segments (three launches) whose states stand in d_workspace
  * (mkv_linear_extend_workspace_size bytes, 16-byte aligned; with less, the

@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <cstddef>
 #include <cstring>
 #include <new>
 #include <type_traits>
@@ -115,10 +116,32 @@ __device__ __forceinline__ bf16x8 join_b64(uint64_t a, uint64_t b) {
   return __builtin_bit_cast(bf16x8, u32x4{(uint32_t)a, (uint32_t)(a >> 32), (uint32_t)b, (uint32_t)(b >> 32)});
 }
 
-// Two tiles' accumulators, rounded, as an operand of 32 rows.
-__device__ __forceinline__ bf16x8 round_rows(f32x4 x, f32x4 y) {
-  return __builtin_bit_cast(bf16x8, u32x4{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
-                                          pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])});
+// The upper halves of two f32: bf16 by truncation (a finite value stays finite).
+__device__ __forceinline__ uint32_t upper_bf16x2(float a, float b) {
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
+}
+// What they leave of the two, exact in f32, rounded to bf16.
+__device__ __forceinline__ uint32_t rest_bf16x2(float a, float b, uint32_t upper) {
+  // -1 in the lower and in the upper half. (Opaque: as a constant the first is
+  // encoded as the f32 -1.0, which is the second.)
+  uint32_t lower = 0x0000bf80u, higher = 0xbf800000u;
+  asm("" : "+s"(lower), "+s"(higher));
+  const bf16x2 u = __builtin_bit_cast(bf16x2, upper);
+  return pack_bf16x2(__builtin_amdgcn_fdot2_f32_bf16(u, __builtin_bit_cast(bf16x2, lower), a, false),
+                     __builtin_amdgcn_fdot2_f32_bf16(u, __builtin_bit_cast(bf16x2, higher), b, false));
+}
+
+// Two tiles' accumulators as an operand of 32 rows in two parts, together 16
+// bits or more of each. An Inf leaves a NaN in the second.
+struct RowParts {
+  bf16x8 hi, lo;
+};
+__device__ __forceinline__ RowParts split_rows(f32x4 x, f32x4 y) {
+  const u32x4 hi = {upper_bf16x2(x[0], x[1]), upper_bf16x2(x[2], x[3]), upper_bf16x2(y[0], y[1]),
+                    upper_bf16x2(y[2], y[3])};
+  const u32x4 lo = {rest_bf16x2(x[0], x[1], hi[0]), rest_bf16x2(x[2], x[3], hi[1]), rest_bf16x2(y[0], y[1], hi[2]),
+                    rest_bf16x2(y[2], y[3], hi[3])};
+  return {__builtin_bit_cast(bf16x8, hi), __builtin_bit_cast(bf16x8, lo)};
 }
 
 // ===========================================================================
@@ -126,11 +149,15 @@ __device__ __forceinline__ bf16x8 round_rows(f32x4 x, f32x4 y) {
 // slice of 16 NW columns); wave w holds columns 16 w .. of the state, all DK
 // rows, in the accumulators of 16x16 tiles (lane m16 + 16 g: column m16, rows
 // 4 g .. 4 g + 3), which are the operand layout of the product with q:
-//   O^T = S^T Q^T      S tiles 2p and 2p + 1 as one operand of 32 rows, rounded
-//                      to bf16 (2^-8 of a term: as much as the output's own rounding)
+//   O^T = S^T Q^T      S tiles 2p and 2p + 1 as one operand of 32 rows, in two
+//                      parts of bf16 (8 + 8 bits: 2^-15 of a term)
 //   P   = K Q^T        tiles of 16 keys by 16 tokens dealt over the waves, decayed
-//                      and masked, through LDS as bf16 (as attention rounds its weights)
+//                      and masked, through LDS in two parts as well
 //   O^T += V^T P^T     V^T by the transposing LDS read
+//                      (With one part of S and of P each an output's error was 1.41
+//                      times that of its own rounding, now it is that rounding's:
+//                      one prompt of 8,192 tokens 115 -> 122 us, 8 of 300-1,500
+//                      67.5 -> 77.5.)
 //   S   = e^G S + K^T (w V)   w V in f32 split into three bf16 (8 + 8 + 8 bits
 //                      by truncation), so that the state keeps f32's accuracy
 // The order of the 32 tokens (or rows) of an operand is (4 g + e, 16 + 4 g + e)
@@ -153,16 +180,25 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
   constexpr int KC = DK / 8, VC = W / 8;   // 16-byte chunks per row
   constexpr int KL = kChunk * KC / T, VL = kChunk * VC / T;  // chunks per thread
   constexpr int NP = DK / 32;              // operands of 32 state rows
-  __shared__ __attribute__((aligned(16))) uint8_t kt[kChunk * KRB];
-  __shared__ __attribute__((aligned(16))) uint8_t qt[OUT ? kChunk * KRB : 16];
-  __shared__ __attribute__((aligned(16))) uint8_t vt[kChunk * VRB];
-  __shared__ __attribute__((aligned(16))) uint8_t pt[OUT ? kChunk * 128 : 16];
-  // Per token: summed log2 decay G, scale e^G, the weight e^{G_end - G}, and
-  // e^{G' - G}, G' that of the last of its 16 tokens; then the chunk's whole decay.
-  // Two of each: the next chunk's are made beside this chunk's products.
-  __shared__ __attribute__((aligned(16))) float gs2[2][kChunk], es2[2][kChunk], ws2[2][kChunk], rs2[2][kChunk];
-  __shared__ float gend2[2];
-  __shared__ int odd_s;  // the last chunk (counted from 1) with an Inf or NaN in k or v
+  constexpr int kPlane = kChunk * 128;     // bytes of one part of the scores
+  // In this order every read's offset from its lane's part fits an instruction
+  // (16 bits) at k_dim 128 (apart, the vectors came last and cost 5 registers).
+  struct Tiles {
+    // Per token: summed log2 decay G, scale e^G, the weight e^{G_end - G}, and
+    // e^{G' - G}, G' that of the last of its 16 tokens; then the chunk's whole decay.
+    // Two of each: the next chunk's are made beside this chunk's products.
+    float gs2[2][kChunk], es2[2][kChunk], ws2[2][kChunk], rs2[2][kChunk], gend2[2];
+    int odd, pad;  // the last chunk (counted from 1) with an Inf or NaN in k or v
+    uint8_t vt[kChunk * VRB];
+    uint8_t pt[OUT ? 2 * kPlane : 16];  // the scores' two parts
+    uint8_t kt[kChunk * KRB], qt[OUT ? kChunk * KRB : 16];
+  };
+  static_assert(offsetof(Tiles, vt) % 16 == 0, "tiles are read 16 bytes at a time");
+  __shared__ __attribute__((aligned(16))) Tiles lds;
+  auto &gs2 = lds.gs2, &es2 = lds.es2, &ws2 = lds.ws2, &rs2 = lds.rs2;
+  auto &gend2 = lds.gend2;
+  uint8_t *const kt = lds.kt, *const qt = lds.qt, *const pt = lds.pt, *const vt = lds.vt;
+  int &odd_s = lds.odd;
 
   const int slices = a.DV / W, rep = a.Hv / a.Hk;
   // Workgroups that share a key head's q and k (its value heads and their
@@ -296,7 +332,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
   load_v(t_begin);
   if constexpr (OUT) {
 #pragma unroll
-    for (int i = 0; i < kChunk * 128 / (16 * T); i++) *reinterpret_cast<u32x4 *>(pt + (tid + T * i) * 16) = u32x4{};
+    for (int i = 0; i < 2 * kPlane / (16 * T); i++) *reinterpret_cast<u32x4 *>(pt + (tid + T * i) * 16) = u32x4{};
   }
   if (wave == NW - 1) g_end = vectors(t_begin, 0);
   gr = load_g(t_begin + kChunk);
@@ -356,12 +392,15 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
         for (int p = 0; p < NP; p++) {
           bf16x8 q[4];
           if constexpr (NW == 4) {
-            const bf16x8 sf = round_rows(S[2 * p], S[2 * p + 1]);
+            const RowParts sf = split_rows(S[2 * p], S[2 * p + 1]);
 #pragma unroll
             for (int tt = 0; tt < 4; tt++) {
               q[tt] = read16(qt + tt * 16 * KRB, q_at[tt], p);
-              acc[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sf, q[tt], p ? acc[tt] : f32x4{}, 0, 0, 0);
+              acc[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sf.hi, q[tt], p ? acc[tt] : f32x4{}, 0, 0, 0);
             }
+#pragma unroll
+            for (int tt = 0; tt < 4; tt++)
+              acc[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sf.lo, q[tt], acc[tt], 0, 0, 0);
           }
 #pragma unroll
           for (int u = 0; u < N; u++) {
@@ -383,8 +422,11 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
               c[u][i] = 4 * g4 + i <= m16 ? c[u][i] * f : 0.0f;
             }
           }
-          *reinterpret_cast<uint64_t *>(pt + (p_row ^ (st[u] * 32)) + tq[u] * 16 * 128) =
-              (uint64_t)pack_bf16x2(c[u][2], c[u][3]) << 32 | pack_bf16x2(c[u][0], c[u][1]);
+          uint8_t *at = pt + (p_row ^ (st[u] * 32)) + tq[u] * 16 * 128;
+          const uint32_t h0 = upper_bf16x2(c[u][0], c[u][1]), h1 = upper_bf16x2(c[u][2], c[u][3]);
+          *reinterpret_cast<uint64_t *>(at) = (uint64_t)h1 << 32 | h0;
+          *reinterpret_cast<uint64_t *>(at + kPlane) =
+              (uint64_t)rest_bf16x2(c[u][2], c[u][3], h1) << 32 | rest_bf16x2(c[u][0], c[u][1], h0);
         }
       };
       constexpr int kFull = NW == 8 ? 2 : 3;  // that many waves have that many tiles, the others one
@@ -403,11 +445,12 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
       // O^T from the state: eight waves, which have no registers for more at once.
 #pragma unroll
       for (int p = 0; p < (NW == 8 ? NP : 0); p++) {
-        const bf16x8 sf = round_rows(S[2 * p], S[2 * p + 1]);
+        const RowParts sf = split_rows(S[2 * p], S[2 * p + 1]);
 #pragma unroll
         for (int tt = 0; tt < 4; tt++) {
           const bf16x8 q = read16(qt + tt * 16 * KRB, q_at[tt], p);
-          acc[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sf, q, p ? acc[tt] : f32x4{}, 0, 0, 0);
+          acc[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sf.hi, q, p ? acc[tt] : f32x4{}, 0, 0, 0);
+          acc[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sf.lo, q, acc[tt], 0, 0, 0);
         }
       }
 #pragma unroll
@@ -431,10 +474,13 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
       for (int tt = 0; tt < 4; tt++) {
 #pragma unroll
         for (int x = 0; x <= tt / 2; x++) {
-          const bf16x8 pf =
-              join_b64(*reinterpret_cast<const uint64_t *>(pt + (p_at[tt] ^ (x * 64)) + tt * 16 * 128),
-                       *reinterpret_cast<const uint64_t *>(pt + (p_at[tt] ^ (x * 64 + 32)) + tt * 16 * 128));
-          acc[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[x], pf, acc[tt], 0, 0, 0);
+#pragma unroll
+          for (int u = 0; u < 2; u++) {
+            const uint8_t *at = pt + u * kPlane + tt * 16 * 128;
+            const bf16x8 pf = join_b64(*reinterpret_cast<const uint64_t *>(at + (p_at[tt] ^ (x * 64))),
+                                       *reinterpret_cast<const uint64_t *>(at + (p_at[tt] ^ (x * 64 + 32))));
+            acc[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[x], pf, acc[tt], 0, 0, 0);
+          }
         }
         typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
         __builtin_amdgcn_raw_buffer_store_b64(u32x2{pack_bf16x2(acc[tt][0], acc[tt][1]), pack_bf16x2(acc[tt][2], acc[tt][3])},
