@@ -103,6 +103,11 @@ def _raw_stream(stream, device: int) -> int:
     return raw(device) if raw is not None else _torch().cuda.current_stream(device).cuda_stream
 
 
+def _host_copy(x):
+    """Host metadata as an array of its own; anything else as it is."""
+    return np.array(x.numpy() if hasattr(x, "numpy") else x) if x is not None and _is_host(x) else x
+
+
 def _torch_type(name: str):
     torch = _torch()
     return torch.float32 if name == "f32" else torch.bfloat16
@@ -299,7 +304,9 @@ class DeviceStatePool:
         """Checks, once, the buffers of one engine step (with a leading layer
         dimension, [L, B, ...], or without one, then shared by every layer)
         and returns `run(layer)`, which enqueues linear_step for that layer
-        with no per-call Python checks."""
+        with no per-call Python checks. Host slots are copied here: a later
+        change of the caller's arrays does not reach the bound call. Device
+        slots are read by every call's kernel."""
         return self._bind(q, k, v, log_decay, None, slots, out, src_slots, scale, stream)
 
     def bind_linear_extend(self, q, k, v, log_decay, q_lens, slots, out, src_slots=None, scale: float | None = None,
@@ -312,6 +319,8 @@ class DeviceStatePool:
         lead = (L,) if q.dim() == 4 else ()
         n, out, scale, flags = self._rows(q, k, v, log_decay, out, scale, lead)
         sh = _stream(stream, self.device)
+        # (The lengths are checked against q's rows here, and here only.)
+        q_lens, slots, src_slots = (_host_copy(x) for x in (q_lens, slots, src_slots))
         if q_lens is None:
             B, dst, src, host, keep = self._slots(slots, src_slots)
             if B != n:
