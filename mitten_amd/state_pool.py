@@ -306,7 +306,8 @@ class DeviceStatePool:
         and returns `run(layer)`, which enqueues linear_step for that layer
         with no per-call Python checks. Host slots are copied here: a later
         change of the caller's arrays does not reach the bound call. Device
-        slots are read by every call's kernel."""
+        slots are read by every call's kernel. A run goes to the given stream,
+        or to the one that is current then."""
         return self._bind(q, k, v, log_decay, None, slots, out, src_slots, scale, stream)
 
     def bind_linear_extend(self, q, k, v, log_decay, q_lens, slots, out, src_slots=None, scale: float | None = None,
@@ -318,7 +319,6 @@ class DeviceStatePool:
         L = self.desc.num_layers
         lead = (L,) if q.dim() == 4 else ()
         n, out, scale, flags = self._rows(q, k, v, log_decay, out, scale, lead)
-        sh = _stream(stream, self.device)
         # (The lengths are checked against q's rows here, and here only.)
         q_lens, slots, src_slots = (_host_copy(x) for x in (q_lens, slots, src_slots))
         if q_lens is None:
@@ -335,11 +335,12 @@ class DeviceStatePool:
         def at(t, layer):
             return ctypes.c_void_p(t.data_ptr() + (layer * (t.numel() // L) * t.element_size() if lead else 0))
 
-        args = [(self._h, layer) + tuple(at(t, layer) for t in (q, k, v, log_decay, out)) + meta + (scale, flags, sh)
+        args = [(self._h, layer) + tuple(at(t, layer) for t in (q, k, v, log_decay, out)) + meta + (scale, flags)
                 for layer in range(L)]
+        device = self.device
 
         def run(layer: int) -> None:
-            st = fn(*args[layer])
+            st = fn(*args[layer], _raw_stream(stream, device))
             if st:
                 _raise(st)
 

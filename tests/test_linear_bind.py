@@ -13,13 +13,15 @@ class Recorder:
     """Stands in for libmitten_kv: notes the host metadata a call arrives with."""
 
     def __init__(self):
-        self.calls = []
+        self.calls, self.at = [], []
 
     def mkv_linear_extend_host(self, h, layer, q, k, v, g, o, lens, src, dst, n, scale, flags, stream):
+        self.at.append((h, stream))
         self.calls.append((layer, lens[:n], None if not src else src[:n], dst[:n]))
         return 0
 
     def mkv_linear_step_host(self, h, layer, q, k, v, g, o, src, dst, n, scale, flags, stream):
+        self.at.append((h, stream))
         self.calls.append((layer, None, None if not src else src[:n], dst[:n]))
         return 0
 
@@ -63,3 +65,20 @@ def test_lists_are_bound_too(pool):
     pool.bind_linear_step(*io, [1, 2, 3], out, stream=pool.stream)(0)
     pool.bind_linear_extend(*io, (2, 0, 1), (1, 2, 3), out, stream=pool.stream)(1)
     assert pool._lib.calls == [(0, None, None, [1, 2, 3]), (1, [2, 0, 1], None, [1, 2, 3])]
+
+
+@pytest.mark.parametrize("step", [False, True])
+def test_a_run_takes_the_stream_that_is_current_then(pool, step, monkeypatch):
+    """Not the one at the bind: a call bound before a graph's capture must be
+    captured with the rest. A given stream stays."""
+    now = [11]
+    monkeypatch.setattr(state_pool, "_raw_stream", lambda s, device: now[0] if s is None else s.cuda_stream)
+    io, out = rows(3)
+    bind, more = (pool.bind_linear_step, ()) if step else (pool.bind_linear_extend, ([1, 1, 1],))
+    current = bind(*io, *more, [1, 2, 3], out)
+    given = bind(*io, *more, [1, 2, 3], out, stream=type("Stream", (), {"cuda_stream": 5})())
+    current(0)
+    now[0] = 12
+    current(1)
+    given(1)
+    assert [stream for _, stream in pool._lib.at] == [11, 12, 5]
