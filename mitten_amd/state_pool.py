@@ -307,7 +307,7 @@ class DeviceStatePool:
         with no per-call Python checks. Host slots are copied here: a later
         change of the caller's arrays does not reach the bound call. Device
         slots are read by every call's kernel. A run goes to the given stream,
-        or to the one that is current then."""
+        or to the one that is current then; after close() it raises."""
         return self._bind(q, k, v, log_decay, None, slots, out, src_slots, scale, stream)
 
     def bind_linear_extend(self, q, k, v, log_decay, q_lens, slots, out, src_slots=None, scale: float | None = None,
@@ -335,12 +335,13 @@ class DeviceStatePool:
         def at(t, layer):
             return ctypes.c_void_p(t.data_ptr() + (layer * (t.numel() // L) * t.element_size() if lead else 0))
 
-        args = [(self._h, layer) + tuple(at(t, layer) for t in (q, k, v, log_decay, out)) + meta + (scale, flags)
+        args = [(layer,) + tuple(at(t, layer) for t in (q, k, v, log_decay, out)) + meta + (scale, flags)
                 for layer in range(L)]
         device = self.device
 
         def run(layer: int) -> None:
-            st = fn(*args[layer], _raw_stream(stream, device))
+            # (self._h is None after close(), which the library refuses.)
+            st = fn(self._h, *args[layer], _raw_stream(stream, device))
             if st:
                 _raise(st)
 

@@ -62,7 +62,7 @@ def test_bound_calls_equal_the_unbound(layered, head_decay, kind):
         pool.check()
 
 
-def test_bind_refusals():
+def test_bind_refusals_and_a_closed_pool():
     import torch
 
     rng = np.random.default_rng(4)
@@ -79,7 +79,13 @@ def test_bind_refusals():
         with pytest.raises(dp.BackendError) as ei:
             call()
         assert msg in str(ei.value), (msg, str(ei.value))
+    runs = [pool.bind_linear_step(*io, [0, 1, 2], out), pool.bind_linear_extend(*io, [1, 1, 1], [0, 1, 2], out)]
+    torch.cuda.synchronize()
     pool.close()
+    for run in runs:
+        with pytest.raises(dp.BackendError) as ei:
+            run(0)
+        assert "pool is NULL" in str(ei.value)
 
 
 def test_a_call_bound_before_a_capture_is_captured():

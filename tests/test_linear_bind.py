@@ -82,3 +82,16 @@ def test_a_run_takes_the_stream_that_is_current_then(pool, step, monkeypatch):
     current(1)
     given(1)
     assert [stream for _, stream in pool._lib.at] == [11, 12, 5]
+
+
+@pytest.mark.parametrize("step", [False, True])
+def test_a_run_after_close_has_no_pool(pool, step):
+    """The library refuses it (no pool), where it would use freed memory."""
+    pool._h = 77
+    io, out = rows(3)
+    bind, more = (pool.bind_linear_step, ()) if step else (pool.bind_linear_extend, ([1, 1, 1],))
+    run = bind(*io, *more, [1, 2, 3], out, stream=pool.stream)
+    run(0)
+    pool._h = None
+    run(0)
+    assert [h for h, _ in pool._lib.at] == [77, None]
