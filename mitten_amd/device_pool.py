@@ -206,6 +206,22 @@ def _stream_handle(stream) -> ctypes.c_void_p:
     return ctypes.c_void_p(stream.cuda_stream)
 
 
+def _empty_on(stream, shape, dtype, device):
+    """A tensor for a call on `stream` (None: the current one) to write. With a
+    stream it is allocated there: memory that the current stream's work has just
+    let go of may still be written by it. It is noted as used on the current
+    stream too, where the caller goes on with it."""
+    torch = _torch()
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(stream.cuda_stream, device=device)
+    with torch.cuda.stream(stream):
+        t = torch.empty(shape, dtype=dtype, device=device)
+    t.record_stream(torch.cuda.current_stream(device))
+    return t
+
+
 def _dptr(t) -> ctypes.c_void_p:
     return ctypes.c_void_p(t.data_ptr())
 

@@ -14,11 +14,16 @@ linear-attention layers of a hybrid model over it:
 model's type or in e4m3 with scales.
 
 torch is used only for device memory and streams, as in `device_pool`.
+
+With `stream=`, what a call allocates is that stream's memory. Operands of
+another stream's have to be ready there, and to be kept (or noted with
+`record_stream`) until it has passed the call, as with any work on a second stream.
 """
 from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
+from functools import partial
 
 import numpy as np
 
@@ -30,6 +35,7 @@ from .device_pool import (
     BackendError,
     DeviceIndexError,
     _dptr,
+    _empty_on,
     _host_i32,
     _host_u32,
     _i32p,
@@ -191,7 +197,7 @@ class DeviceStatePool:
         _check(dst, self.device, (n,), torch.int32, "dst")
         _raise(self._lib.mkv_state_copy(self._h, _dptr(src), _dptr(dst), n, sh))
 
-    def _rows(self, q, k, v, log_decay, out, scale, lead=()):
+    def _rows(self, q, k, v, log_decay, out, scale, lead=(), stream=None):
         """Checks a call's rows ([*lead, tokens, heads, dim]) and returns
         (tokens, out, scale, flags). log_decay: f32 [*lead, tokens, Hv], or
         [*lead, Hv] for one decay per head."""
@@ -209,7 +215,7 @@ class DeviceStatePool:
         _check(log_decay, self.device, lead + ((d.num_v_heads,) if per_head else (n, d.num_v_heads)), torch.float32,
                "log_decay")
         if out is None:
-            out = torch.empty_like(v)
+            out = _empty_on(stream, v.shape, dt, v.device)
         _check(out, self.device, lead + (n, d.num_v_heads, d.v_dim), dt, "out")
         return n, out, d.k_dim ** -0.5 if scale is None else scale, LINEAR_HEAD_DECAY if per_head else 0
 
@@ -236,7 +242,7 @@ class DeviceStatePool:
         (default: slots[b]; STATE_NONE, or -1 in a device tensor: zeros) on
         and leaves it in slots[b]. Slots: host u32 (validated, copied) or
         device int32. Returns o [B, Hv, v_dim]."""
-        n, out, scale, flags = self._rows(q, k, v, log_decay, out, scale)
+        n, out, scale, flags = self._rows(q, k, v, log_decay, out, scale, stream=stream)
         B, dst, src, host, _ = self._slots(slots, src_slots)
         if B != n:
             raise _bad(f"{n} rows for {B} slots")
@@ -250,7 +256,7 @@ class DeviceStatePool:
         """A chunk of q_lens[b] tokens per sequence, its rows one after
         another; slots as in linear_step. Host q_lens and slots (validated,
         copied). Returns o [tokens, Hv, v_dim]."""
-        n, out, scale, flags = self._rows(q, k, v, log_decay, out, scale)
+        n, out, scale, flags = self._rows(q, k, v, log_decay, out, scale, stream=stream)
         lens, slots, src_slots = self._extend_meta(n, q_lens, slots, src_slots)
         _raise(self._lib.mkv_linear_extend_host(
             self._h, layer, _dptr(q), _dptr(k), _dptr(v), _dptr(log_decay), _dptr(out), _i32p(lens),
@@ -285,7 +291,7 @@ class DeviceStatePool:
         graph. workspace: a device tensor of linear_extend_workspace_size
         bytes, or None for the pool's own."""
         torch = _torch()
-        n, out, scale, flags = self._rows(q, k, v, log_decay, out, scale)
+        n, out, scale, flags = self._rows(q, k, v, log_decay, out, scale, stream=stream)
         if _is_host(slots):
             raise _bad("slots must be a device tensor")
         B, dst, src, _, _ = self._slots(slots, src_slots)
@@ -318,7 +324,7 @@ class DeviceStatePool:
     def _bind(self, q, k, v, log_decay, q_lens, slots, out, src_slots, scale, stream):
         L = self.desc.num_layers
         lead = (L,) if q.dim() == 4 else ()
-        n, out, scale, flags = self._rows(q, k, v, log_decay, out, scale, lead)
+        n, out, scale, flags = self._rows(q, k, v, log_decay, out, scale, lead, stream)
         # (The lengths are checked against q's rows here, and here only.)
         q_lens, slots, src_slots = (_host_copy(x) for x in (q_lens, slots, src_slots))
         if q_lens is None:
@@ -378,15 +384,16 @@ def add_rms_norm(x, weight, eps: float, residual=None, residual_out=None, out=No
             weight.dim() != 1 or weight.shape[0] != dim or not weight.is_contiguous():
         _check(weight, dev, (dim,), torch.float32, "weight")
     if residual is not None and residual_out is None:
-        residual_out = torch.empty_like(x)
+        residual_out = torch.empty_like(x) if stream is None else _empty_on(stream, shape, dt, device)
     if out is None and (both or not fp8):
-        out = torch.empty_like(x)
+        out = torch.empty_like(x) if stream is None else _empty_on(stream, shape, dt, device)
     q8 = scales = None
     if fp8:
         if group < 0 or (group and dim % group):
             raise _bad(f"group ({group}) does not divide dim ({dim})")
-        q8 = torch.empty((rows, dim), dtype=torch.float8_e4m3fn, device=device)
-        scales = torch.empty((rows, dim // group if group else 1), dtype=torch.float32, device=device)
+        new = torch.empty if stream is None else partial(_empty_on, stream)
+        q8 = new((rows, dim), dtype=torch.float8_e4m3fn, device=device)
+        scales = new((rows, dim // group if group else 1), dtype=torch.float32, device=device)
     elif group:
         raise _bad("group is for an e4m3 output")
     st = _lib.device_lib().mkv_add_rms_norm(
