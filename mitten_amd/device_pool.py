@@ -351,7 +351,6 @@ class DeviceKvPool:
                out_k=None, out_v=None, total_tokens: int | None = None, stream=None):
         """Returns (k, v), each flat [sum(ctx) * Hkv * D]: sequence b occupies
         [Hkv][ctx_b][D] starting at element ctx_indptr[b]*Hkv*D."""
-        torch = _torch()
         d = self.desc
         B = ctx_indptr.shape[0] - 1
         self._i32(block_indptr, "block_indptr", B + 1)
@@ -361,9 +360,9 @@ class DeviceKvPool:
             total_tokens = int(ctx_indptr[-1].item())
         n = total_tokens * d.num_kv_heads * d.head_dim
         if out_k is None:
-            out_k = torch.empty(n, dtype=self.torch_dtype, device=ctx_indptr.device)
+            out_k = _empty_on(stream, n, self.torch_dtype, ctx_indptr.device)
         if out_v is None:
-            out_v = torch.empty(n, dtype=self.torch_dtype, device=ctx_indptr.device)
+            out_v = _empty_on(stream, n, self.torch_dtype, ctx_indptr.device)
         self._check_tensor(out_k, None, "out_k")
         self._check_tensor(out_v, None, "out_v")
         if out_k.numel() < n or out_v.numel() < n:
@@ -388,9 +387,9 @@ class DeviceKvPool:
         n = int(cl.astype(np.int64).sum()) * d.num_kv_heads * d.head_dim
         dev = torch.device(f"cuda:{self.device}")
         if out_k is None:
-            out_k = torch.empty(max(n, 1), dtype=self.torch_dtype, device=dev)
+            out_k = _empty_on(stream, max(n, 1), self.torch_dtype, dev)
         if out_v is None:
-            out_v = torch.empty(max(n, 1), dtype=self.torch_dtype, device=dev)
+            out_v = _empty_on(stream, max(n, 1), self.torch_dtype, dev)
         self._check_tensor(out_k, None, "out_k")
         self._check_tensor(out_v, None, "out_v")
         cap = min(out_k.numel(), out_v.numel()) // (d.num_kv_heads * d.head_dim)
@@ -423,7 +422,6 @@ class DeviceKvPool:
                          split_tokens: int = 0, workspace=None, kernel: str | None = None,
                          stream=None):
         """q: [B, Hq, D] in the pool dtype. Returns o: [B, Hq, D]."""
-        torch = _torch()
         d = self.desc
         B = q.shape[0]
         self._check_tensor(q, (B, d.num_q_heads, d.head_dim), "q")
@@ -431,7 +429,7 @@ class DeviceKvPool:
         self._i32(block_ids, "block_ids")
         self._i32(ctx_lens, "ctx_lens", B)
         if out is None:
-            out = torch.empty_like(q)
+            out = _empty_on(stream, q.shape, q.dtype, q.device)
         self._check_tensor(out, (B, d.num_q_heads, d.head_dim), "out")
         if scale is None:
             scale = float(np.float32(d.head_dim ** -0.5))
@@ -457,7 +455,6 @@ class DeviceKvPool:
                                 split_tokens: int = 0, kernel: str | None = None, stream=None):
         """decode_attention with its split-K partials in the library's static
         device scratch (mkv_decode_attention_static): nothing is allocated."""
-        torch = _torch()
         d = self.desc
         B = q.shape[0]
         self._check_tensor(q, (B, d.num_q_heads, d.head_dim), "q")
@@ -465,7 +462,7 @@ class DeviceKvPool:
         self._i32(block_ids, "block_ids")
         self._i32(ctx_lens, "ctx_lens", B)
         if out is None:
-            out = torch.empty_like(q)
+            out = _empty_on(stream, q.shape, q.dtype, q.device)
         self._check_tensor(out, (B, d.num_q_heads, d.head_dim), "out")
         if scale is None:
             scale = float(np.float32(d.head_dim ** -0.5))
@@ -488,7 +485,6 @@ class DeviceKvPool:
         """Causal attention of each sequence's newest tokens (chunked prefill):
         q, out: [q_indptr[-1], Hq, D]; sequence b's n_b = q_indptr[b+1] - q_indptr[b]
         queries sit at positions [ctx_b - n_b, ctx_b) and attend keys 0..p."""
-        torch = _torch()
         d = self.desc
         B = q_indptr.shape[0] - 1
         self._i32(q_indptr, "q_indptr", B + 1)
@@ -498,7 +494,7 @@ class DeviceKvPool:
         T = q.shape[0]
         self._check_tensor(q, (T, d.num_q_heads, d.head_dim), "q")
         if out is None:
-            out = torch.empty_like(q)
+            out = _empty_on(stream, q.shape, q.dtype, q.device)
         self._check_tensor(out, (T, d.num_q_heads, d.head_dim), "out")
         if scale is None:
             scale = float(np.float32(d.head_dim ** -0.5))
@@ -512,14 +508,13 @@ class DeviceKvPool:
                               scale: float | None = None, zero_sink: bool = False, stream=None):
         """extend_attention with host metadata (mkv_extend_attention_host):
         sequence b's q_lens[b] query rows follow sequence b-1's in q."""
-        torch = _torch()
         d = self.desc
         ql, cl = _host_i32(q_lens, "q_lens"), _host_i32(ctx_lens, "ctx_lens")
         ip, ix = _host_u32(block_indptr, "block_indptr"), _host_u32(block_ids, "block_ids")
         T = int(ql.astype(np.int64).sum())
         self._check_tensor(q, (T, d.num_q_heads, d.head_dim), "q")
         if out is None:
-            out = torch.empty_like(q)
+            out = _empty_on(stream, q.shape, q.dtype, q.device)
         self._check_tensor(out, (T, d.num_q_heads, d.head_dim), "out")
         if ql.size != cl.size or ip.size != cl.size + 1:
             raise BackendError(MKV_ERR_INVALID_ARGUMENT, "q_lens, ctx_lens and block_indptr disagree on num_seqs")
@@ -570,7 +565,7 @@ class DeviceKvPool:
             self._check_tensor(inv_freq, None, "inv_freq", dtype=torch.float32)
             rd = 2 * inv_freq.shape[0]
         if out is None:
-            out = torch.empty((n, d.num_q_heads, d.head_dim), dtype=self.torch_dtype, device=q.device)
+            out = _empty_on(stream, (n, d.num_q_heads, d.head_dim), self.torch_dtype, q.device)
         self._check_tensor(out, (n, d.num_q_heads, d.head_dim), "out")
         nul = ctypes.c_void_p(0)
         fn = self._lib.mkv_qk_norm_rope_append_host if host else self._lib.mkv_qk_norm_rope_append
@@ -603,9 +598,9 @@ class DeviceKvPool:
         dev = torch.device(f"cuda:{self.device}")
         nbytes = n * self.wire_block_bytes(nl)
         if payload is None:
-            payload = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            payload = _empty_on(stream, nbytes, torch.uint8, dev)
         if checksums is None:
-            checksums = torch.empty(n, dtype=torch.int64, device=dev)
+            checksums = _empty_on(stream, n, torch.int64, dev)
         self._check_tensor(payload, (nbytes,), "payload", dtype=torch.uint8)
         self._check_tensor(checksums, (n,), "checksums", dtype=torch.int64)
         if host:
@@ -633,7 +628,7 @@ class DeviceKvPool:
         if expected is not None:
             self._check_tensor(expected, (n,), "expected", dtype=torch.int64)
         if checksums is None:
-            checksums = torch.empty(n, dtype=torch.int64, device=payload.device)
+            checksums = _empty_on(stream, n, torch.int64, payload.device)
         self._check_tensor(checksums, (n,), "checksums", dtype=torch.int64)
         fn = self._lib.mkv_wire_import_host if host else self._lib.mkv_wire_import
         _raise(fn(self._h, _u32p(block_ids) if host else _dptr(block_ids), n, layer_begin, nl, _dptr(payload),
@@ -677,7 +672,8 @@ class DeviceKvPool:
         d = self.desc
         if not getattr(plan, "suffixes", False):
             raise BackendError(MKV_ERR_INVALID_ARGUMENT, "the plan must come from plan_suffixes")
-        out, scale, flags = self._planned_args(plan, q, block_indptr, block_ids, out, scale, zero_sink, kernel)
+        out, scale, flags = self._planned_args(plan, q, block_indptr, block_ids, out, scale, zero_sink, kernel,
+                                               stream=stream)
         if prefix_ids is not None:
             self._i32(prefix_ids, "prefix_ids")
         elif not plan.has_prefix:
@@ -695,7 +691,8 @@ class DeviceKvPool:
             flags, _stream_handle(stream)))
         return out
 
-    def _planned_args(self, plan, q, block_indptr, block_ids, out, scale, zero_sink, kernel, cached_loads=False):
+    def _planned_args(self, plan, q, block_indptr, block_ids, out, scale, zero_sink, kernel, cached_loads=False,
+                      stream=None):
         d = self.desc
         if plan.pool is not self:
             raise BackendError(MKV_ERR_INVALID_ARGUMENT, "plan belongs to another pool")
@@ -709,9 +706,8 @@ class DeviceKvPool:
         else:
             self._i32(block_indptr, "block_indptr", B + 1)
             self._i32(block_ids, "block_ids")
-        torch = _torch()
         if out is None:
-            out = torch.empty_like(q)
+            out = _empty_on(stream, q.shape, q.dtype, q.device)
         self._check_tensor(out, (B, d.num_q_heads, d.head_dim), "out")
         if scale is None:
             scale = float(np.float32(d.head_dim ** -0.5))
@@ -734,7 +730,7 @@ class DeviceKvPool:
         """cached_loads: K/V loads through the caches (MKV_ATTN_CACHED_LOADS),
         for batches whose tables share blocks."""
         out, scale, flags = self._planned_args(plan, q, block_indptr, block_ids, out, scale, zero_sink, kernel,
-                                               cached_loads)
+                                               cached_loads, stream)
         _raise(self._lib.mkv_decode_attention_planned(
             self._h, plan._h, layer, _dptr(q), _dptr(out), _tptr(block_indptr), _tptr(block_ids),
             scale, flags, _stream_handle(stream)))
@@ -749,7 +745,7 @@ class DeviceKvPool:
         block-table gather (mkv_decode_step_gather)."""
         d = self.desc
         out, scale, flags = self._planned_args(plan, q, block_indptr, block_ids, out, scale, zero_sink, kernel,
-                                               cached_loads)
+                                               cached_loads, stream)
         B = plan.num_seqs
         self._check_tensor(k_new, (B, d.num_kv_heads, d.head_dim), "k_new")
         self._check_tensor(v_new, (B, d.num_kv_heads, d.head_dim), "v_new")

@@ -6,7 +6,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from mitten_amd import DeviceStatePool, StateDesc, add_rms_norm
+from mitten_amd import DeviceKvPool, DeviceStatePool, PoolDesc, StateDesc, add_rms_norm
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +77,39 @@ def test_results_are_right_on_a_given_stream():
         got = add_rms_norm(x, w, 1e-6, stream=side)[1]
         torch.cuda.current_stream().wait_stream(side)
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("kind", ["decode", "planned", "static", "extend", "extend_host", "prep", "gather",
+                                  "gather_host", "wire"])
+def test_kv_pool(kind):
+    import torch
+
+    B, ctx, hq, hkv, d = 64, 256, 8, 2, 128  # results of 512 KiB
+    desc = PoolDesc(num_layers=1, num_kv_heads=hkv, num_q_heads=hq, head_dim=d, num_blocks=B * ctx // 16, dtype="bf16")
+    with DeviceKvPool(desc) as pool:
+        pool.tensor().zero_()
+        q = torch.randn(B * 4, hq, d, device="cuda").bfloat16()
+        kv = torch.randn(B * 4, hkv, d, device="cuda").bfloat16()
+        host_ip, host_ids = np.arange(B + 1) * (ctx // 16), np.arange(B * ctx // 16)
+        ip, ids, cl, qip = (torch.tensor(x, dtype=torch.int32, device="cuda")
+                            for x in (host_ip, host_ids, [ctx] * B, 4 * np.arange(B + 1)))
+        cip = torch.tensor(ctx * np.arange(B + 1), dtype=torch.int32, device="cuda")
+        plan = pool.plan(np.full(B, ctx, np.int32))
+        slots = np.arange(B * 4)
+        torch.cuda.synchronize()
+        out, one = 2 * B * 4 * hq * d, 2 * B * hq * d
+        kvb = 2 * B * ctx * hkv * d
+        call, sizes = {
+            "decode": (lambda s: [pool.decode_attention(0, q[:B], ip, ids, cl, ctx, stream=s)], [one]),
+            "planned": (lambda s: [pool.decode_attention_planned(0, plan, q[:B], ip, ids, stream=s)], [one]),
+            "static": (lambda s: [pool.decode_attention_static(0, q[:B], ip, ids, cl, ctx, stream=s)], [one]),
+            "extend": (lambda s: [pool.extend_attention(0, q, qip, ip, ids, cl, 4, ctx, stream=s)], [out]),
+            "extend_host": (lambda s: [pool.extend_attention_host(0, q, [4] * B, [ctx] * B, host_ip, host_ids,
+                                                                  stream=s)], [out]),
+            "prep": (lambda s: [pool.qk_norm_rope_append(0, q, kv, kv, slots, slots, gated=False, stream=s)], [out]),
+            "gather": (lambda s: pool.gather(0, ip, ids, cip, ctx, total_tokens=B * ctx, stream=s), [kvb, kvb]),
+            "gather_host": (lambda s: pool.gather_host(0, host_ip, host_ids, [ctx] * B, stream=s), [kvb, kvb]),
+            "wire": (lambda s: pool.wire_export(host_ids, stream=s), [2 * kvb, 8 * host_ids.size]),
+        }[kind]
+        check(call, sizes)
+        pool.check()
