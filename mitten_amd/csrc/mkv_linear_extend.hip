@@ -20,6 +20,7 @@ namespace mkv {
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef short i16x4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i16x4s lds_i16x4;
 
@@ -91,6 +92,14 @@ __device__ __forceinline__ float exp2_f(float x) { return __builtin_amdgcn_exp2f
 // stays one).
 __device__ __forceinline__ double log2_decay(float g) {
   return (double)(g < -104.0f ? -104.0f : g) * 1.4426950408889634074;
+}
+
+// Difference of two summed log2 decays of a chunk, each in steps of 2^-17 (64
+// tokens reach -9,603, within 31 bits): off by 2^-17 at most wherever the
+// tokens stand, where f32 sums behind strong decays are off by 2^-10. A NaN is lost
+// here; it reaches the outputs by e^G.
+__device__ __forceinline__ float decay_diff(int a, int b) {
+  return (float)(int)((uint32_t)a - (uint32_t)b) * 7.62939453125e-6f;
 }
 
 // c + 0 * each bf16 of a word: a NaN where one of them is an Inf or a NaN.
@@ -184,10 +193,12 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
   // In this order every read's offset from its lane's part fits an instruction
   // (16 bits) at k_dim 128 (apart, the vectors came last and cost 5 registers).
   struct Tiles {
-    // Per token: summed log2 decay G, scale e^G, the weight e^{G_end - G}, and
-    // e^{G' - G}, G' that of the last of its 16 tokens; then the chunk's whole decay.
-    // Two of each: the next chunk's are made beside this chunk's products.
-    float gs2[2][kChunk], es2[2][kChunk], ws2[2][kChunk], rs2[2][kChunk], gend2[2];
+    // Per token: summed log2 decay G (in 2^-17, decay_diff), scale e^G, the weight
+    // e^{G_end - G}, and e^{G' - G}, G' that of the last of its 16 tokens; then the
+    // chunk's whole decay. Two of each: the next chunk's are made beside this
+    // chunk's products.
+    int gs2[2][kChunk];
+    float es2[2][kChunk], ws2[2][kChunk], rs2[2][kChunk], gend2[2];
     int odd, pad;  // the last chunk (counted from 1) with an Inf or NaN in k or v
     uint8_t vt[kChunk * VRB];
     uint8_t pt[OUT ? 2 * kPlane : 16];  // the scores' two parts
@@ -195,7 +206,8 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
   };
   static_assert(offsetof(Tiles, vt) % 16 == 0, "tiles are read 16 bytes at a time");
   __shared__ __attribute__((aligned(16))) Tiles lds;
-  auto &gs2 = lds.gs2, &es2 = lds.es2, &ws2 = lds.ws2, &rs2 = lds.rs2;
+  auto &gs2 = lds.gs2;
+  auto &es2 = lds.es2, &ws2 = lds.ws2, &rs2 = lds.rs2;
   auto &gend2 = lds.gend2;
   uint8_t *const kt = lds.kt, *const qt = lds.qt, *const pt = lds.pt, *const vt = lds.vt;
   int &odd_s = lds.odd;
@@ -261,7 +273,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
   const int64_t krs = (int64_t)a.Hk * KRB, vrs = (int64_t)a.Hv * a.DV * 2;  // row strides
   u32x4 kr[KL], qr[OUT ? KL : 1], vr[VL];
   uint32_t k_off = tid / KC * (uint32_t)krs + tid % KC * 16, v_off = tid / VC * (uint32_t)vrs + tid % VC * 16;
-  uint32_t o_off = m16 * (uint32_t)vrs + (wave * 16 + 4 * g4) * 2, s_off = lane_off;
+  uint32_t o_off = m16 * (uint32_t)vrs + (wave * 16 + 4 * g4) * 2;
   // The loop has no branch around a load or a store of global memory (the
   // buffers' bounds drop them), so that a wait for the next chunk's rows does not
   // wait for the outputs stored after they were asked for.
@@ -295,10 +307,10 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
   float gr = load_g(t_begin);
   auto vectors = [&](int t0, int buf) {
     const double l = t0 + lane < t_end ? log2_decay(gr) : 0.0, G = wave_scan(l), end = lane_d(G, 63);
-    gs2[buf][lane] = (float)G;
+    gs2[buf][lane] = (int)rint(fmin(fmax(G, -16000.0), 16000.0) * 131072.0);
     es2[buf][lane] = exp2_f((float)G) * a.scale;
     ws2[buf][lane] = exp2_f((float)(end - G));
-    rs2[buf][lane] = exp2_f(__shfl((float)G, lane | 15) - (float)G);
+    rs2[buf][lane] = exp2_f((float)(__shfl(G, lane | 15) - G));
     if (lane == 0) gend2[buf] = exp2_f((float)end);
     return end;
   };
@@ -343,11 +355,12 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
   int t0 = t_begin;
   for (int chunk = 1; t0 < t_end; chunk++) {
     const int nt = min(kChunk, t_end - t0);
-    const float *gs = gs2[(chunk - 1) & 1], *es = es2[(chunk - 1) & 1], *ws = ws2[(chunk - 1) & 1], *rs = rs2[(chunk - 1) & 1];
+    const int *gs = gs2[(chunk - 1) & 1];
+    const float *es = es2[(chunk - 1) & 1], *ws = ws2[(chunk - 1) & 1], *rs = rs2[(chunk - 1) & 1];
     // (Opaque: the addresses made from these are formed where they are used,
     // not kept in registers over the loop.)
     asm volatile("" : "+v"(k_tr), "+v"(v_tr), "+v"(k_row), "+v"(q_row), "+v"(p_row));
-    asm volatile("" : "+v"(k_off), "+v"(v_off), "+v"(o_off), "+v"(s_off));
+    asm volatile("" : "+v"(k_off), "+v"(v_off), "+v"(o_off));
     // (And one of each per 16 tokens: two reads off the same register would be
     // paired across tokens, into registers that no operand has in that order.)
     int q_at[4] = {q_row, q_row, q_row, q_row}, p_at[4] = {p_row, p_row, p_row, p_row};
@@ -376,8 +389,9 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
       auto scores = [&](auto count, int n0, int step) {
         constexpr int N = decltype(count)::value;
         int tq[N], st[N];
-        f32x4 c[N], gk[N], r[N];
-        float gt[N], e[N];
+        f32x4 c[N], r[N];
+        i32x4 gk[N];
+        int gt[N], e[N];
 #pragma unroll
         for (int u = 0; u < N; u++) {  // tiles by rows from the last one: (3, 0) .. (3, 3), (2, 0) .. (0, 0)
           const int n = n0 + step * u;
@@ -385,7 +399,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
           st[u] = n - (n < 4 ? 0 : n < 7 ? 4 : n < 9 ? 7 : 9);
           gt[u] = gs[16 * tq[u] + m16];
           e[u] = gs[16 * st[u] + 15];
-          gk[u] = *reinterpret_cast<const f32x4 *>(&gs[16 * st[u] + 4 * g4]);
+          gk[u] = *reinterpret_cast<const i32x4 *>(&gs[16 * st[u] + 4 * g4]);
           r[u] = *reinterpret_cast<const f32x4 *>(&rs[16 * st[u] + 4 * g4]);
         }
 #pragma unroll
@@ -412,13 +426,13 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
 #pragma unroll
         for (int u = 0; u < N; u++) {
           if (st[u] < tq[u]) {  // e^{G_t - G_end of tile} e^{G_end of tile - G_k}: one exponential per lane
-            const float f = exp2_f(gt[u] - e[u]) * a.scale;
+            const float f = exp2_f(decay_diff(gt[u], e[u])) * a.scale;
 #pragma unroll
             for (int i = 0; i < 4; i++) c[u][i] *= f * r[u][i];
           } else {
 #pragma unroll
             for (int i = 0; i < 4; i++) {  // (selected, not multiplied: past t it may be anything)
-              const float f = exp2_f(gt[u] - gk[u][i]) * a.scale;
+              const float f = exp2_f(decay_diff(gt[u], gk[u][i])) * a.scale;
               c[u][i] = 4 * g4 + i <= m16 ? c[u][i] * f : 0.0f;
             }
           }
@@ -570,6 +584,10 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
 #pragma unroll
     for (int j = 0; j < DK / 16; j++) *reinterpret_cast<f32x4 *>(frag + j * 256) = S[j];
   } else if constexpr (MODE == kWhole) {
+    // (Formed again: not kept in a register over the loop.)
+    int m = m16, g = g4;
+    asm volatile("" : "+v"(m), "+v"(g));
+    const uint32_t s_off = (uint32_t)(4 * g * a.DV + sl * W + 16 * wave + m) * 4;
     const auto to = buffer(a.states + s.dst * plane + hoff, DK * srow);
 #pragma unroll
     for (int j = 0; j < DK / 16; j++)

@@ -56,3 +56,32 @@ def test_bf16_outputs_have_one_rounding(dk, dv, n, whole, rate):
     ref, _, _, _ = reference(*(widen(x) for x in (q, k, v)), g, s0, dk ** -0.5)
     rounding = norm(widen(orc.f32_to_bf16(ref.astype(np.float32))) - ref)
     assert norm(o - ref) <= 1.02 * rounding
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (256, 128)])
+@pytest.mark.parametrize("strong,first", [(60, 61), (40, 44), (40, 61), (62, 62)])
+def test_small_decays_after_strong_ones(dtype, dk, dv, strong, first):
+    """`strong` tokens of a chunk decay by e^-95 to e^-104 each, those after
+    them by 1e-3: the sum is past -5,000 where differences of it decide the
+    scores. Two opposite values, at `first` and the token after, cancel but
+    for the decay between them; q . k is 1 throughout. Per term, bf16: 2^-15
+    (a score's second part is rounded) + 2^-16 (decay differences in steps
+    of 2^-17, the exponential); f32: 2^-18 (f32 operations and their sums)."""
+    n, hv = 64, 32
+    rng = np.random.default_rng(strong + first)
+    q, k, v = (np.zeros((n, h, d), np.float32) for h, d in ((1, dk), (1, dk), (hv, dv)))
+    q[:, :, 3] = k[:, :, 3] = 1
+    v[first] = 2.0 ** rng.integers(-3, 3, (hv, dv))
+    v[first + 1] = -v[first]
+    g = -rng.uniform(95, 104, (n, hv)).astype(np.float32)
+    g[strong:] = -1e-3 * rng.uniform(0.1, 2, (n - strong, hv))
+    if dtype == "bf16":
+        q, k, v = (orc.f32_to_bf16(x) for x in (q, k, v))
+    s0 = np.zeros((hv, dk, dv), np.float32)
+    o, s = extend(q, k, v, g, s0, dtype)
+    scale = float(np.float32(dk ** -0.5))
+    ref, rs, ao, as_ = reference(*(widen(x) for x in (q, k, v)), g, s0, scale)
+    bound = 2.0 ** -8 * np.abs(ref) + (2.0 ** -15 + 2.0 ** -16) * ao if dtype == "bf16" else 2.0 ** -18 * ao
+    assert np.all(np.abs(o - ref) <= bound)
+    assert np.all(np.abs(s - rs) <= 2.0 ** -18 * as_)
