@@ -519,7 +519,8 @@ MKV_API int mkv_state_copy_host(mkv_state_pool *pool, const uint32_t *h_src_slot
  * d_q, d_k: [num_seqs][num_k_heads][k_dim]; d_v, d_o: [num_seqs][num_v_heads][v_dim];
  * in the pool's dtype, 16-byte aligned, d_o overlapping none of the others.
  * d_log_decay: f32 [num_seqs][num_v_heads] (or [num_v_heads] with
- * MKV_LINEAR_HEAD_DECAY), usually <= 0; -inf forgets all before the token.
+ * MKV_LINEAR_HEAD_DECAY), usually <= 0; -inf (or what is 0 in f32, below -104)
+ * forgets all before the token, but for an infinite state, which 0 makes a NaN.
  * All arithmetic is f32 with one rounding per output element.
  * Destinations must be distinct and no sequence's source another's
  * destination (checked by the host form). A slot outside the pool is

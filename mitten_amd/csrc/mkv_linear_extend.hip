@@ -34,7 +34,7 @@ constexpr int kChunk = 64;  // tokens per chunk
 struct LinSegs {
   int32_t nseg, len;
   float *state;  // [B][nseg][Hv][DK * DV]: local states, then the state before each segment
-  float *decay;  // [B][nseg][Hv]: exp of a segment's summed log decays
+  float *decay;  // [B][nseg][Hv]: exp of a segment's summed log decays, -0 with a decay of 0 among them
 };
 
 __device__ __forceinline__ int lin_nseg(const LinSegs &g, int n) {
@@ -85,7 +85,10 @@ __device__ __forceinline__ double lane_d(double v, int lane) {
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
-__device__ __forceinline__ float exp2_f(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float exp2_f(float x) { return __builtin_amdgcn_exp2f(x); }  // below 2^-126: 0
+
+// Whether a decay of that log2 is 0 in f32, as -inf is: it makes an infinity a NaN.
+__device__ __forceinline__ bool decay_is_zero(double l) { return l < -150.0; }
 
 // A token's log decay in base 2. Below e^-104 a decay is 0 in f32 whatever
 // stands beside it: cutting there keeps sums of decays finite at -inf (a NaN
@@ -100,6 +103,11 @@ __device__ __forceinline__ double log2_decay(float g) {
 // here; it reaches the outputs by e^G.
 __device__ __forceinline__ float decay_diff(int a, int b) {
   return (float)(int)((uint32_t)a - (uint32_t)b) * 7.62939453125e-6f;
+}
+
+// A segment's decay for the scan, from its summed log2 (-inf: one of them was 0).
+__device__ __forceinline__ float segment_decay(double total) {
+  return total == -INFINITY ? -0.0f : exp2_f((float)total);
 }
 
 // c + 0 * each bf16 of a word: a NaN where one of them is an Inf or a NaN.
@@ -312,7 +320,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
     ws2[buf][lane] = exp2_f((float)(end - G));
     rs2[buf][lane] = exp2_f((float)(__shfl(G, lane | 15) - G));
     if (lane == 0) gend2[buf] = exp2_f((float)end);
-    return end;
+    return MODE == kLocal && __any(decay_is_zero(l)) ? end - INFINITY : end;  // (a NaN stays one)
   };
   auto stage = [&](int chunk) {  // the loaded rows into the LDS tiles
     float odd[4] = {};
@@ -552,8 +560,8 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
     const int64_t krow = ((int64_t)(s.row0 + t0) * a.Hk + kh) * DK + 4 * g4;
     const int64_t vrow = ((int64_t)(s.row0 + t0) * a.Hv + h) * a.DV + sl * W + 16 * wave + m16;
     const double l = log2_decay(a.g[(int64_t)(s.row0 + t0) * a.g_stride + h]);
-    const float d = exp2_f((float)l);
-    total += l;
+    const float d = exp2f((float)l);
+    total += decay_is_zero(l) ? -INFINITY : l;
     const float v = __uint_as_float((uint32_t)static_cast<const uint16_t *>(a.v)[vrow] << 16);
     float o = 0.0f;
 #pragma unroll
@@ -580,7 +588,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
 
   if constexpr (MODE == kLocal) {
     if (tid == 64 * (NW - 1) && sl == 0)
-      sg.decay[((int64_t)b * sg.nseg + seg) * a.Hv + h] = exp2_f((float)total);
+      sg.decay[((int64_t)b * sg.nseg + seg) * a.Hv + h] = segment_decay(total);
 #pragma unroll
     for (int j = 0; j < DK / 16; j++) *reinterpret_cast<f32x4 *>(frag + j * 256) = S[j];
   } else if constexpr (MODE == kWhole) {
@@ -729,6 +737,7 @@ __global__ void __launch_bounds__(256, DK == 256 ? 1 : 2) linear_chunk_f32_kerne
         ws[lane] = exp2_f((float)(end - G));
       }
       if (lane == 0) gend_s = exp2_f((float)end);
+      if (MODE == kLocal && __any(decay_is_zero(l))) end -= INFINITY;  // (a NaN stays one)
     }
     __syncthreads();
     if (odd_s == chunk) break;  // uniform over the workgroup
@@ -814,8 +823,8 @@ __global__ void __launch_bounds__(256, DK == 256 ? 1 : 2) linear_chunk_f32_kerne
     const int64_t krow = ((int64_t)(s.row0 + t0) * a.Hk + kh) * DK + 4 * g4;
     const int64_t vrow = ((int64_t)(s.row0 + t0) * a.Hv + h) * a.DV + sl * W + 16 * wave + m16;
     const double l = log2_decay(a.g[(int64_t)(s.row0 + t0) * a.g_stride + h]);
-    const float d = exp2_f((float)l), v = static_cast<const float *>(a.v)[vrow];
-    total += l;
+    const float d = exp2f((float)l), v = static_cast<const float *>(a.v)[vrow];
+    total += decay_is_zero(l) ? -INFINITY : l;
     float o = 0.0f;
 #pragma unroll
     for (int j = 0; j < DK / 16; j++) {
@@ -835,7 +844,7 @@ __global__ void __launch_bounds__(256, DK == 256 ? 1 : 2) linear_chunk_f32_kerne
   }
 
   if constexpr (MODE == kLocal) {
-    if (tid == 0 && sl == 0) sg.decay[((int64_t)b * sg.nseg + seg) * a.Hv + h] = exp2_f((float)total);
+    if (tid == 0 && sl == 0) sg.decay[((int64_t)b * sg.nseg + seg) * a.Hv + h] = segment_decay(total);
 #pragma unroll
     for (int j = 0; j < DK / 16; j++) *reinterpret_cast<f32x4 *>(frag + j * 256) = S[j];
   } else if constexpr (MODE == kWhole) {
@@ -883,8 +892,9 @@ __global__ void __launch_bounds__(256) linear_scan_kernel(LinArgs a, LinSegs sg,
     for (int u = 0; u < U; u++) {
       if (j0 + u >= ns) break;
       *reinterpret_cast<f32x4 *>(at + (j0 + u) * plane) = S;
-      // (An infinity stays one under a product of decays that is 0 only by underflow.)
-      const bool gone = d[u] < 1.17549435e-38f;
+      // (An infinity stays one under a product of decays that is 0 only by
+      // underflow; a decay of 0 makes it a NaN.)
+      const bool gone = d[u] < 1.17549435e-38f && !signbit(d[u]);
 #pragma unroll
       for (int i = 0; i < 4; i++) S[i] = (gone && isinf(S[i]) ? S[i] : d[u] * S[i]) + l[u][i];
     }
