@@ -110,11 +110,14 @@ __device__ __forceinline__ float segment_decay(double total) {
   return total == -INFINITY ? -0.0f : exp2_f((float)total);
 }
 
-// c + 0 * each bf16 of a word: a NaN where one of them is an Inf or a NaN.
+// c + the squares of a word's two bf16: not finite where one is an Inf, a NaN, or
+// so large (2^64) that a product of two may pass f32's range.
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ float odd_bf16x2(uint32_t w, float c) {
-  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), bf16x2{}, c, false);
+__device__ __forceinline__ float add_squares(uint32_t w, float c) {
+  const bf16x2 x = __builtin_bit_cast(bf16x2, w);
+  return __builtin_amdgcn_fdot2_f32_bf16(x, x, c, false);
 }
+__device__ __forceinline__ bool not_finite(float x) { return x - x != 0.0f; }
 
 // Buffer resource over `bytes` bytes at p (wave-uniform): loads past the end
 // return zeros and stores past it are dropped, without a branch.
@@ -179,9 +182,10 @@ __device__ __forceinline__ RowParts split_rows(f32x4 x, f32x4 y) {
 //                      by truncation), so that the state keeps f32's accuracy
 // The order of the 32 tokens (or rows) of an operand is (4 g + e, 16 + 4 g + e)
 // throughout, which is how accumulator tiles and transposing reads deliver them.
-// From a chunk with an Inf or NaN in k or v, or a state whose products are not
-// finite, the segment goes on token by token (masked products would carry
-// them to tokens that do not see them).
+// From a chunk with an Inf or NaN in k or v (or a number of 2^64 or more), in its
+// scores or in its products with the state, the segment goes on token by token:
+// masked products would carry them to tokens that do not see them, and what
+// overflows in a product of a chunk is not what does in the recurrence.
 // ===========================================================================
 // kWhole: one segment per sequence, states read and written in their slots.
 // kLocal and kOutputs: the first and the last of the three launches over
@@ -207,7 +211,8 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
     // chunk's products.
     int gs2[2][kChunk];
     float es2[2][kChunk], ws2[2][kChunk], rs2[2][kChunk], gend2[2];
-    int odd, pad;  // the last chunk (counted from 1) with an Inf or NaN in k or v
+    int odd;   // the last chunk (counted from 1) with an Inf, a NaN or 2^64 in k or v
+    int late;  // the chunk with one in its scores, or in its products with the state
     uint8_t vt[kChunk * VRB];
     uint8_t pt[OUT ? 2 * kPlane : 16];  // the scores' two parts
     uint8_t kt[kChunk * KRB], qt[OUT ? kChunk * KRB : 16];
@@ -273,7 +278,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
     }
   }
   double total = 0.0, g_end = 0.0;  // summed log2 decays of the segment so far, and of this chunk (wave NW - 1)
-  if (tid == 0) odd_s = 0;
+  if (tid == 0) odd_s = lds.late = 0;
 
   const uint8_t *kp = static_cast<const uint8_t *>(a.k) + ((int64_t)s.row0 * a.Hk + kh) * KRB;
   const uint8_t *qp = static_cast<const uint8_t *>(a.q) + ((int64_t)s.row0 * a.Hk + kh) * KRB;
@@ -327,7 +332,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
     auto put = [&](const u32x4 &x, uint8_t *tile, int at, bool look) {
       if (look) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) odd[e] = odd_bf16x2(x[e], odd[e]);
+        for (int e = 0; e < 4; e++) odd[e] = add_squares(x[e], odd[e]);
       }
       *reinterpret_cast<uint2 *>(tile + at) = make_uint2(x[0], x[1]);
       *reinterpret_cast<uint2 *>(tile + (at ^ 8)) = make_uint2(x[2], x[3]);
@@ -343,8 +348,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
       const int r = tid / VC + i * (T / VC), c = tid % VC;
       put(vr[i], vt, lin_at(r, c, 0, VC, lin_tr_swz(r, VC)), true);
     }
-    const float any = (odd[0] + odd[1]) + (odd[2] + odd[3]);
-    if (any != any) odd_s = chunk;
+    if (not_finite((odd[0] + odd[1]) + (odd[2] + odd[3]))) odd_s = chunk;
   };
 
   load_k(t_begin);
@@ -383,6 +387,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
     gr = load_g(t0 + 2 * kChunk);
 
     f32x4 acc[4];
+    float bad[2] = {};  // a NaN where a product is an Inf or a NaN
     if constexpr (OUT) {
       // Scores: the ten tiles of 16 tokens (columns) by 16 keys on and below the
       // diagonal, up to three per wave; the two above it that a product of 32
@@ -444,6 +449,8 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
               c[u][i] = 4 * g4 + i <= m16 ? c[u][i] * f : 0.0f;
             }
           }
+#pragma unroll
+          for (int i = 0; i < 4; i++) bad[i & 1] = fmaf(c[u][i], 0.0f, bad[i & 1]);
           uint8_t *at = pt + (p_row ^ (st[u] * 32)) + tq[u] * 16 * 128;
           const uint32_t h0 = upper_bf16x2(c[u][0], c[u][1]), h1 = upper_bf16x2(c[u][2], c[u][3]);
           *reinterpret_cast<uint64_t *>(at) = (uint64_t)h1 << 32 | h0;
@@ -476,9 +483,27 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
         }
       }
 #pragma unroll
-      for (int tt = 0; tt < 4; tt++) acc[tt] *= es[16 * tt + m16];
+      for (int tt = 0; tt < 4; tt++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) bad[i & 1] = fmaf(acc[tt][i], 0.0f, bad[i & 1]);
+        acc[tt] *= es[16 * tt + m16];
+      }
+      if (bad[0] + bad[1] != 0.0f) lds.late = chunk;
       __syncthreads();  // the scores are written
     }
+    const float dend = gend2[(chunk - 1) & 1];
+    if constexpr (!OUT) {
+      // (An Inf in a state without outputs only meets the chunk's decay.)
+      if (__builtin_amdgcn_readfirstlane(__float_as_int(dend)) == 0) {
+#pragma unroll
+        for (int j = 0; j < DK / 16; j++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) bad[i & 1] = fmaf(S[j][i], 0.0f, bad[i & 1]);
+        if (bad[0] + bad[1] != 0.0f) lds.late = chunk;
+        __syncthreads();
+      }
+    }
+    const int late = lds.late;
 
     load_v(t0 + kChunk);
     bf16x8 vf[2];  // [32 tokens][16 columns]
@@ -489,6 +514,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
       const i16x4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(at + 16 * VRB));
       vf[x] = join_b64(__builtin_bit_cast(uint64_t, lo), __builtin_bit_cast(uint64_t, hi));
     }
+    if (late == chunk) break;  // uniform over the workgroup
     if constexpr (OUT) {
       const auto ob = buffer(static_cast<uint8_t *>(a.o) + ((int64_t)(s.row0 + t0) * a.Hv + h) * a.DV * 2 + sl * VRB,
                              (uint32_t)(nt - 1) * (uint32_t)vrs + VRB);
@@ -511,7 +537,6 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
     }
     total += g_end;  // (past the last exit of the loop body)
     g_end = next_end;
-    const float dend = gend2[(chunk - 1) & 1];
 #pragma unroll
     for (int j = 0; j < DK / 16; j++) S[j] *= dend;
 #pragma unroll
@@ -552,7 +577,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 && DK < 256 ? 4 : DK < 256 ? 
     __syncthreads();
   }
 
-  // From the first chunk that holds an Inf or NaN on: token by token, as the
+  // From the first chunk that cannot be computed as one on: token by token, as the
   // recurrence has it. Lane: column m16 of each tile, its rows' share of an
   // output, summed over the four lane groups.
 #pragma unroll 1
@@ -626,7 +651,8 @@ __global__ void __launch_bounds__(256, DK == 256 ? 1 : 2) linear_chunk_f32_kerne
   // Summed log2 decay (two floats), scale e^G, and e^{G_end - G} per token.
   __shared__ __attribute__((aligned(16))) float gh[C], gl[C], es[C], ws[C];
   __shared__ float gend_s;
-  __shared__ int odd_s;  // the last chunk (counted from 1) with an Inf or NaN in k or v
+  __shared__ int odd_s;   // the last chunk (counted from 1) with an Inf, a NaN or 2^64 in k or v
+  __shared__ int late_s;  // the chunk with one in its scores, or in its products with the state
 
   const int slices = a.DV / W, rep = a.Hv / a.Hk;
   const int members = rep * slices, grp = (int)((blockIdx.x >> 3) / members) * 8 + (int)(blockIdx.x & 7);
@@ -666,7 +692,7 @@ __global__ void __launch_bounds__(256, DK == 256 ? 1 : 2) linear_chunk_f32_kerne
     }
   }
   double total = 0.0;  // summed log2 decays of the segment so far (wave 0)
-  if (tid == 0) odd_s = 0;
+  if (tid == 0) odd_s = late_s = 0;
 
   const uint8_t *kp = static_cast<const uint8_t *>(a.k) + ((int64_t)s.row0 * a.Hk + kh) * (DK * 4);
   const uint8_t *qp = static_cast<const uint8_t *>(a.q) + ((int64_t)s.row0 * a.Hk + kh) * (DK * 4);
@@ -716,16 +742,16 @@ __global__ void __launch_bounds__(256, DK == 256 ? 1 : 2) linear_chunk_f32_kerne
       *reinterpret_cast<f32x4 *>(kt + at(r, c, KC)) = kr[i];
       if constexpr (OUT) *reinterpret_cast<f32x4 *>(qt + at(r, c, KC)) = qr[i];
 #pragma unroll
-      for (int e = 0; e < 4; e++) odd = fmaf(kr[i][e], 0.0f, odd);
+      for (int e = 0; e < 4; e++) odd = fmaf(kr[i][e], kr[i][e], odd);
     }
 #pragma unroll
     for (int i = 0; i < VL; i++) {
       const int r = tid / VC + i * (256 / VC), c = tid % VC * 4;
       *reinterpret_cast<f32x4 *>(vt + at(r, c, VC)) = vr[i];
 #pragma unroll
-      for (int e = 0; e < 4; e++) odd = fmaf(vr[i][e], 0.0f, odd);
+      for (int e = 0; e < 4; e++) odd = fmaf(vr[i][e], vr[i][e], odd);
     }
-    if (odd != odd) odd_s = chunk;
+    if (not_finite(odd)) odd_s = chunk;
     double end = 0.0;
     if (wave == 0) {
       const double l = lane < nt ? log2_decay(gr) : 0.0, G = wave_scan(l);
@@ -742,9 +768,9 @@ __global__ void __launch_bounds__(256, DK == 256 ? 1 : 2) linear_chunk_f32_kerne
     __syncthreads();
     if (odd_s == chunk) break;  // uniform over the workgroup
     load(t0 + C);
-    total += end;
 
     f32x4 acc[2];
+    float bad = 0.0f;  // a NaN where a product is an Inf or a NaN
     if constexpr (OUT) {
       // Scores: one tile of 16 tokens (columns) by 16 keys per wave; the one
       // that no column sees comes out as zeros.
@@ -763,6 +789,7 @@ __global__ void __launch_bounds__(256, DK == 256 ? 1 : 2) linear_chunk_f32_kerne
         const int k = 16 * st + 4 * g4 + i;
         const float e = exp2_f((gh[t] - gh[k]) + (gl[t] - gl[k])) * a.scale;
         p[i] = k <= t ? r[i] * e : 0.0f;
+        bad = fmaf(p[i], 0.0f, bad);
       }
       *reinterpret_cast<f32x4 *>(pt + t * C + ((4 * st + g4) ^ (t & 7)) * 4) = p;
       // O^T from the state.
@@ -776,15 +803,34 @@ __global__ void __launch_bounds__(256, DK == 256 ? 1 : 2) linear_chunk_f32_kerne
           for (int i = 0; i < 4; i++)
             o[i & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(S[j][i], qf[i], o[i & 1], 0, 0, 0);
         }
-        acc[tt] = (o[0] + o[1]) * es[16 * tt + m16];
+        acc[tt] = o[0] + o[1];
+#pragma unroll
+        for (int i = 0; i < 4; i++) bad = fmaf(acc[tt][i], 0.0f, bad);
+        acc[tt] *= es[16 * tt + m16];
       }
+      if (bad != 0.0f) late_s = chunk;
       __syncthreads();  // the scores are written
     }
+    const float dend = gend_s;
+    if constexpr (!OUT) {
+      // (An Inf in a state without outputs only meets the chunk's decay.)
+      if (__builtin_amdgcn_readfirstlane(__float_as_int(dend)) == 0) {
+#pragma unroll
+        for (int j = 0; j < DK / 16; j++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) bad = fmaf(S[j][i], 0.0f, bad);
+        if (bad != 0.0f) late_s = chunk;
+        __syncthreads();
+      }
+    }
+    const int late = late_s;
     float vf[2][4];  // [16 tokens][4 g + i] of the wave's columns
 #pragma unroll
     for (int st = 0; st < 2; st++)
 #pragma unroll
       for (int i = 0; i < 4; i++) vf[st][i] = vt[at(16 * st + 4 * g4 + i, 16 * wave + m16, VC)];
+    if (late == chunk) break;  // uniform over the workgroup
+    total += end;
     if constexpr (OUT) {
       const auto ob = buffer(static_cast<uint8_t *>(a.o) + ((int64_t)(s.row0 + t0) * a.Hv + h) * a.DV * 4 + sl * (W * 4),
                              (uint32_t)(nt - 1) * (uint32_t)vrs + W * 4);
@@ -801,7 +847,6 @@ __global__ void __launch_bounds__(256, DK == 256 ? 1 : 2) linear_chunk_f32_kerne
                                                t * (uint32_t)vrs + (16 * wave + 4 * g4) * 4, 0, 0);
       }
     }
-    const float dend = gend_s;
 #pragma unroll
     for (int j = 0; j < DK / 16; j++) S[j] *= dend;
 #pragma unroll
@@ -816,7 +861,7 @@ __global__ void __launch_bounds__(256, DK == 256 ? 1 : 2) linear_chunk_f32_kerne
       }
   }
 
-  // Token by token from the first chunk with an Inf or NaN on, as the bf16 form.
+  // Token by token from there on, as the bf16 form.
 #pragma unroll 1
   for (; t0 < t_end; t0++) {
     asm volatile("" : "+v"(m16), "+v"(g4));

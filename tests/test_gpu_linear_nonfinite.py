@@ -88,3 +88,56 @@ def test_a_nan_decay_beside_a_zero_one_stays(dtype):
     g[1381, 1], g[1380, 1] = np.nan, -np.inf
     _, s = verify("segments", q, k, v, g, s0, dtype)
     assert np.isnan(s).all()
+
+
+def recurrence32(q, k, v, g, s0, scale):
+    """The recurrence with its state held in f32 (past 3.4e38 it is infinite),
+    in f64 otherwise: (outputs, state, their sums of absolute values)."""
+    top = 3.4028235e38
+    rep = v.shape[1] // k.shape[1]
+    q, k = (np.repeat(x.astype(np.float64), rep, 1) for x in (q, k))
+    v = v.astype(np.float64)
+    S, A = s0.astype(np.float64), np.abs(s0.astype(np.float64))
+    o, Ao = np.zeros(v.shape), np.zeros(v.shape)
+    for t in range(v.shape[0]):
+        d = np.exp(g[t].astype(np.float64))[:, None, None]
+        kv = k[t][:, :, None] * v[t][:, None, :]
+        kv = np.where(np.abs(kv) > top, np.copysign(np.inf, kv), kv)
+        S, A = d * S + kv, d * A + np.abs(kv)
+        S = np.where(np.abs(S) > top, np.copysign(np.inf, S), S)
+        o[t], Ao[t] = scale * np.einsum("hd,hdv->hv", q[t], S), scale * np.einsum("hd,hdv->hv", np.abs(q[t]), A)
+    return np.where(np.abs(o) > top, np.copysign(np.inf, o), o), S, Ao, A
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (256, 64)])
+@pytest.mark.parametrize("form,n", FORMS + [("whole", 64)])
+@pytest.mark.parametrize("what", ["state", "state and decays", "score", "score of two states", "q inf", "q nan"])
+def test_overflow_and_odd_queries(form, n, dk, dv, what, dtype):
+    """Finite rows whose product overflows a state inside a segment ("state"),
+    before decays whose product is 0 ("state and decays"); a q . k past f32's
+    range where the state and the output are within it ("score", with a
+    value of 1e-25; "score of two states": the product of q with a state of 1e30
+    likewise); a query that is not finite."""
+    q, k, v, g, s0 = make(n, dk, dv, dtype, 5)
+    q += np.where(q >= 0, 0.25, -0.25).astype(np.float32)
+    at = n // 3
+    if what.startswith("state"):
+        k[at, 0, 3], v[at, 0, 2], v[at, 1, 5] = 1e30, 1e30, -1e30
+        g[at + 1:] = -2.5 if what == "state and decays" else -1e-3
+    elif what == "score":
+        k[at, 0, 3], q[at:at + 9, 0, 3], v[at] = 1e25, 1e20, 1e-25
+    elif what == "score of two states":
+        s0[0, 3, 2], g[0, 0], q[at:at + 9, 0, 3] = 1e30, -100, 1e10
+    else:
+        q[at, 0, 3] = np.inf if what == "q inf" else np.nan
+    if dtype == "bf16":
+        q, k, v = (widen(orc.f32_to_bf16(x)) for x in (q, k, v))
+    o, s = run(form, q, k, v, g, s0, dtype)
+    with np.errstate(all="ignore"):
+        ro, rs, ao, as_ = recurrence32(q, k, v, g, s0, dk ** -0.5)
+    for got, ref, bound in ((o, ro, out_bound(n, dk, dtype, ro, ao)), (s, rs, f32_bound(n, dk, as_))):
+        fine = np.isfinite(ref)
+        assert np.array_equal(np.isnan(ref), np.isnan(got))
+        assert np.array_equal(ref[np.isinf(ref)], got[np.isinf(ref)])
+        assert np.all(np.abs(got[fine] - ref[fine]) <= bound[fine])
