@@ -985,7 +985,8 @@ static LinPlan plan_extend(const StatePool *p, int64_t num_seqs, int64_t num_tok
                            uint64_t ws_bytes) {
   const mkv_state_desc &d = p->desc;
   const bool f32 = d.dtype == MKV_DTYPE_F32;
-  const int64_t longest = std::max<int64_t>(1, (max_q_len + kChunk - 1) / kChunk);  // chunks
+  // Chunks of the longest sequence (max_q_len may be a loose bound).
+  const int64_t longest = std::max<int64_t>(1, (std::min(max_q_len, num_tokens) + kChunk - 1) / kChunk);
   const int64_t chunks = std::min(num_seqs * longest, num_tokens / kChunk + num_seqs);
   const int cols = f32 || d.v_dim == 64 ? 64 : 128;  // of a workgroup over segments
   const double load = (double)chunks * d.num_v_heads * d.v_dim / (f32 ? 64 : 128) / p->cus;
@@ -995,8 +996,7 @@ static LinPlan plan_extend(const StatePool *p, int64_t num_seqs, int64_t num_tok
   LinPlan r = {cols / 16, 1, INT_MAX & ~(kChunk - 1)};
   double best = std::max(lone * longest, full * load);
   for (int64_t want = 1; want < longest && want * segs < best; want += 1 + want / 64) {
-    // Chunks of a segment, to 2%: max_q_len may be a loose bound, and the steps are
-    // the same whatever the workspace holds.
+    // Chunks of a segment, to 2%; the steps are the same whatever the workspace holds.
     const int64_t nseg = (longest + want - 1) / want;
     const uint64_t bytes = segs_bytes(p, num_seqs, nseg);
     if (bytes > ws_bytes) continue;
