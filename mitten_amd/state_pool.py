@@ -289,20 +289,23 @@ class DeviceStatePool:
         """linear_extend with device metadata (int32 q_indptr [B + 1], slots,
         src_slots), read when the kernels run: it can be captured into a
         graph. workspace: a device tensor of linear_extend_workspace_size
-        bytes, or None for the pool's own."""
+        bytes (with less, of none too, sequences stay whole), or None for the
+        pool's own."""
         torch = _torch()
         n, out, scale, flags = self._rows(q, k, v, log_decay, out, scale, stream=stream)
         if _is_host(slots):
             raise _bad("slots must be a device tensor")
         B, dst, src, _, _ = self._slots(slots, src_slots)
         _check(q_indptr, self.device, (B + 1,), torch.int32, "q_indptr")
-        nws = 0
+        ws, nws = None, 0
         if workspace is not None:
-            _check(workspace, self.device, None, workspace.dtype, "workspace")
+            _check(workspace, self.device, None, getattr(workspace, "dtype", None), "workspace")
             nws = workspace.numel() * workspace.element_size()
+            # (An empty tensor has no address, and no address is the pool's own.)
+            ws = workspace.data_ptr() or self.data_ptr
         _raise(self._lib.mkv_linear_extend(
             self._h, layer, _dptr(q), _dptr(k), _dptr(v), _dptr(log_decay), _dptr(out), _dptr(q_indptr), src, dst, B,
-            n, max_q_len, scale, flags, _tptr(workspace), nws, _stream(stream, self.device)))
+            n, max_q_len, scale, flags, ws, nws, _stream(stream, self.device)))
         return out
 
     def bind_linear_step(self, q, k, v, log_decay, slots, out, src_slots=None, scale: float | None = None,

@@ -138,3 +138,28 @@ def test_graphs_with_workspaces_of_their_own_beside_each_other():
             for b in range(2):
                 assert torch.equal(outs[b], want[b][0]) and torch.equal(pool.tensor()[0, b], want[b][1])
         pool.check()
+
+
+def test_an_empty_workspace_is_none_of_the_pools():
+    """A workspace of no bytes has no room for segments: the call stays whole, as
+    with one of 16, where the pool's own would have cut it."""
+    import torch
+
+    from mitten_amd import device_pool as dp
+
+    rng = np.random.default_rng(9)
+    hk, hv, dk, dv, n = 1, 2, 128, 128, 2000
+    _, dev, ip = long_prompt(rng, hk, hv, dk, dv, n, "f32")
+    slots, new = (torch.tensor([x], dtype=torch.int32, device="cuda") for x in (0, -1))
+    with DeviceStatePool(StateDesc(1, hk, hv, dk, dv, 1, "f32")) as pool:
+        got = []
+        for ws in (None, torch.empty(16, device="cuda"), torch.empty(0, device="cuda")):
+            o = pool.linear_extend_device(0, *dev, ip, slots, n, src_slots=new, workspace=ws)
+            got.append((o, pool.tensor().clone()))
+        pool.check()
+        assert not torch.equal(got[0][1], got[1][1])  # (summed in another order)
+        assert torch.equal(got[1][0], got[2][0]) and torch.equal(got[1][1], got[2][1])
+        for bad, msg in ((np.zeros(1 << 20), "tensor"), (torch.empty(64), "cuda:0")):
+            with pytest.raises(dp.BackendError) as ei:
+                pool.linear_extend_device(0, *dev, ip, slots, n, workspace=bad)
+            assert msg in str(ei.value)
