@@ -85,3 +85,23 @@ def test_small_decays_after_strong_ones(dtype, dk, dv, strong, first):
     bound = 2.0 ** -8 * np.abs(ref) + (2.0 ** -15 + 2.0 ** -16) * ao if dtype == "bf16" else 2.0 ** -18 * ao
     assert np.all(np.abs(o - ref) <= bound)
     assert np.all(np.abs(s - rs) <= 2.0 ** -18 * as_)
+
+
+STATE_REL = 1.5e-6  # norm of a state's error, relative (test_linear_state_parts.py)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("dk,dv", LONG)
+@pytest.mark.parametrize("n,whole", [(2, True), (64, True), (200, True), (1500, True), (1500, False)])
+def test_states_keep_f32s_accuracy(dk, dv, n, whole, dtype):
+    """w V against K in three bf16 parts (24 bits): the norm of a state's error
+    is that of f32 sums, some 2^-24 for each of the operations that an element
+    takes, in a random order of signs: 2^-24 sqrt(2 x 64) = 7e-7 over the tokens
+    that a state remembers here (rates of 1e-1 to 1, so few). Two parts leave
+    1e-5."""
+    rng = np.random.default_rng(dk * dv + n)
+    q, k, v, g = inputs(rng, n, 1, 2, dk, dv, dtype, 0.3)
+    s0 = (0.3 * rng.standard_normal((2, dk, dv))).astype(np.float32)
+    _, s = extend(q, k, v, g, s0, dtype, whole)
+    _, ref, _, _ = reference(*(widen(x) for x in (q, k, v)), g, s0, dk ** -0.5)
+    assert norm(s - ref) <= STATE_REL * norm(ref)
