@@ -971,16 +971,16 @@ struct LinPlan {
 };
 
 // The costs are measured ones in microseconds at a k_dim of 128 (f32: 64) on 256
-// CUs: whole sequences, `lone` per chunk of 64 tokens of the longest or `full`
-// per chunk and CU (of 128 columns; f32: 64); segments, `seg` per chunk of one
-// round of workgroups or `segs` of each of several, 12 for three launches, and
-// the states between them, written, scanned and read at 5 TB/s. A chunk's
-// products grow with k_dim, its latency (most of `lone`) less. Measured against
-// the other way: 2,000 tokens of 32 heads of 128 in segments 52 us (whole 134),
-// 600 tokens 34 (47), 300 tokens whole 21 (28), 8 prompts of 300-1,500 tokens of
-// 28 heads whole 69 (108), 2 of 1,000-2,000 of 8 heads of 256 in segments 64
-// (155); f32 2,000 tokens of 14 heads of 64 37 (201), 2 of 500-1,000 of 16 heads
-// of 128 65 (133; 89 in the segments that costs without k_dim choose).
+// CUs: whole sequences, 4.5 (f32: 2.5) and `lone` per chunk of 64 tokens of the
+// longest, or `full` per chunk and CU (of 128 columns; f32: 64); segments, `seg`
+// per chunk of one round of workgroups or `segs` of each of several, 14 for three
+// launches, and the states between them, written, scanned and read at 5 TB/s. A
+// chunk's products grow with k_dim, its latency less. Measured against the other
+// way: 1,000 tokens of 32 heads of 128 in segments 38 us (whole 54), 4,000 80
+// (199), 2 prompts of 800 of 28 heads whole 47 (57), 4 of 600 of 8 heads of 256 in
+// segments 48 (61), 8 of 300 of 2 heads of 64 whole 17 (20); f32 1,000 tokens of 14
+// heads of 64 in segments 28 (113), 8 of 300 whole 40 (44), 2 of 800 of 32 heads of
+// 128 in segments 124 (136).
 static LinPlan plan_extend(const StatePool *p, int64_t num_seqs, int64_t num_tokens, int64_t max_q_len,
                            uint64_t ws_bytes) {
   const mkv_state_desc &d = p->desc;
@@ -991,18 +991,22 @@ static LinPlan plan_extend(const StatePool *p, int64_t num_seqs, int64_t num_tok
   const int cols = f32 || d.v_dim == 64 ? 64 : 128;  // of a workgroup over segments
   const double load = (double)chunks * d.num_v_heads * d.v_dim / (f32 ? 64 : 128) / p->cus;
   const double dim = d.k_dim / (f32 ? 64.0 : 128.0);
-  const double lone = (f32 ? 6.8 : 3.6) * std::min(dim, (1.0 + dim) / 2), full = (f32 ? 5.6 : 3.3) * dim;
-  const double seg = (f32 ? 8.4 : 7.4) * dim, segs = (f32 ? 6.0 : 6.2) * dim;
+  const double grown = f32 ? dim : std::max(0.56 + 0.44 * dim, 0.23 + 0.77 * dim);
+  const double lone = f32 ? 6.8 * std::min(dim, (1.0 + dim) / 2) : 3.1 * grown, full = (f32 ? 5.6 : 3.3) * dim;
+  const double seg = (f32 ? 8.4 : 7.4) * grown, segs = (f32 ? 6.0 : 6.2) * grown;
   LinPlan r = {cols / 16, 1, INT_MAX & ~(kChunk - 1)};
-  double best = std::max(lone * longest, full * load);
+  double best = std::max((f32 ? 2.5 : 4.5) + lone * longest, full * load);
   for (int64_t want = 1; want < longest && want * segs < best; want += 1 + want / 64) {
     // Chunks of a segment, to 2%; the steps are the same whatever the workspace holds.
     const int64_t nseg = (longest + want - 1) / want;
     const uint64_t bytes = segs_bytes(p, num_seqs, nseg);
     if (bytes > ws_bytes) continue;
-    const double wgs = (double)chunks / want * d.num_v_heads * (d.v_dim / cols);
-    const double rounds = std::max(1.0, std::ceil(wgs / p->cus - 0.05));
-    const double t = 12.0 + 3.0 * (double)bytes / 5e6 + want * (rounds > 1.0 ? segs * rounds : seg);
+    // Workgroups of the fullest XCD, which has whole key heads' (5 segments each of 2
+    // prompts, 28 heads over 4: 35 on 32 CUs, 57 us against 47 whole).
+    const double heads = std::ceil(std::ceil((double)chunks / want) * d.num_k_heads / 8);
+    const double wgs = heads * (d.num_v_heads / d.num_k_heads) * (d.v_dim / cols);
+    const double rounds = std::max(1.0, std::ceil(wgs * 8 / p->cus - 0.05));
+    const double t = 14.0 + 3.0 * (double)bytes / 5e6 + want * (rounds > 1.0 ? segs * rounds : seg);
     if (t < best) {
       best = t;
       r.nseg = (int)nseg;

@@ -163,3 +163,14 @@ def test_an_empty_workspace_is_none_of_the_pools():
             with pytest.raises(dp.BackendError) as ei:
                 pool.linear_extend_device(0, *dev, ip, slots, n, workspace=bad)
             assert msg in str(ei.value)
+
+
+def test_segments_that_overfill_an_xcd_are_counted():
+    """28 value heads over 4: whole key heads go to one XCD, 5 segments each of 2
+    prompts would leave 35 workgroups on its 32 CUs, two rounds of three
+    launches (57 us; whole 47). 16 key heads of 2 fill every XCD evenly."""
+    with DeviceStatePool(StateDesc(1, 4, 28, 128, 128, 1, "bf16")) as pool:
+        assert pool.linear_extend_workspace_size(2, 1600, 800) == 0
+        assert pool.linear_extend_workspace_size(1, 4000, 4000) > 0
+    with DeviceStatePool(StateDesc(1, 16, 32, 128, 128, 1, "bf16")) as pool:
+        assert pool.linear_extend_workspace_size(1, 1000, 1000) > 0
