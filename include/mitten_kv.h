@@ -517,7 +517,7 @@ MKV_API int mkv_state_copy_host(mkv_state_pool *pool, const uint32_t *h_src_slot
  * and written to slot dst[b]; o[b] is its output. src NULL: src = dst, in
  * place. A source other than dst[b] is a fork: it stays as it is.
  * d_q, d_k: [num_seqs][num_k_heads][k_dim]; d_v, d_o: [num_seqs][num_v_heads][v_dim];
- * in the pool's dtype, 16-byte aligned, d_o overlapping none of the others.
+ * in the pool's dtype, 16-byte aligned, d_o overlapping none of the others (refused).
  * d_log_decay: f32 [num_seqs][num_v_heads] (or [num_v_heads] with
  * MKV_LINEAR_HEAD_DECAY), usually <= 0; -inf (or what is 0 in f32, below -104)
  * forgets all before the token, but for an infinite state, which 0 makes a NaN.

@@ -131,6 +131,12 @@ struct DeviceGuard {
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Whether two buffers, neither of them null, share a byte.
+inline bool overlap(const void *a, uint64_t an, const void *b, uint64_t bn) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x && y && (x < y ? y - x < an : x - y < bn);
+}
+
 #define MKV_CHECK_HIP(expr)                      \
   do {                                           \
     hipError_t e_ = (expr);                      \

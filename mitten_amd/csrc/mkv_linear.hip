@@ -166,6 +166,13 @@ int lin_args(StatePool *p, int32_t layer, const void *d_q, const void *d_k, cons
     return set_error(MKV_ERR_INVALID_ARGUMENT, "NULL device pointer");
   if (!aligned16(d_q) || !aligned16(d_k) || !aligned16(d_v) || !aligned16(d_o))
     return set_error(MKV_ERR_INVALID_ARGUMENT, "q, k, v and o must be 16-byte aligned");
+  // (Heads that share q and k, and columns that share a row, are computed apart.)
+  const uint64_t es = d.dtype == MKV_DTYPE_F32 ? 4 : 2, n = (uint64_t)num_tokens;
+  const uint64_t kb = n * d.num_k_heads * d.k_dim * es, vb = n * d.num_v_heads * d.v_dim * es;
+  const uint64_t gb = (flags & MKV_LINEAR_HEAD_DECAY ? 1 : n) * d.num_v_heads * 4;
+  if (n && (overlap(d_o, vb, d_q, kb) || overlap(d_o, vb, d_k, kb) || overlap(d_o, vb, d_v, vb) ||
+            overlap(d_o, vb, d_g, gb)))
+    return set_error(MKV_ERR_INVALID_ARGUMENT, "o overlaps q, k, v or the decays");
   a = LinArgs{};
   a.q = d_q;
   a.k = d_k;

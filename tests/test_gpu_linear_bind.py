@@ -121,3 +121,30 @@ def test_a_call_bound_before_a_capture_is_captured():
             torch.cuda.synchronize()
             assert torch.equal(out, o) and torch.equal(pool.tensor(), s)
         pool.check()
+
+
+@pytest.mark.parametrize("form", ["step", "step_device", "extend", "extend_device", "bind"])
+def test_an_output_over_an_operand_is_refused(form):
+    import torch
+
+    n, h, d = 8, 2, 64
+    with DeviceStatePool(StateDesc(1, h, h, d, d, n, "f32")) as pool:
+        pool.tensor().zero_()
+        # q, k, v and room for two outputs one after another; decays in the last of them.
+        flat = torch.zeros(5 * n * h * d, device="cuda")
+        q, k, v, o, p = (x.view(n, h, d) for x in flat.chunk(5))
+        g = p.view(-1)[: n * h].view(n, h)
+        slots = torch.arange(n, dtype=torch.int32, device="cuda")
+        ip = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+        call = {"step": lambda o: pool.linear_step(0, q, k, v, g, list(range(n)), out=o),
+                "step_device": lambda o: pool.linear_step(0, q, k, v, g, slots, out=o),
+                "extend": lambda o: pool.linear_extend(0, q, k, v, g, [n], [0], out=o),
+                "extend_device": lambda o: pool.linear_extend_device(0, q, k, v, g, ip, slots[:1], n, out=o),
+                "bind": lambda o: pool.bind_linear_step(q, k, v, g, slots, o)(0)}[form]
+        near = [flat[x:x + n * h * d].view(n, h, d) for x in (4, n * h * d - 4, 3 * n * h * d - 4)]
+        for bad in (q, k, v, p, *near):
+            with pytest.raises(dp.BackendError) as ei:
+                call(bad)
+            assert "overlaps" in str(ei.value)
+        call(o)  # right behind v and before the decays
+        pool.check()
