@@ -579,7 +579,8 @@ MKV_API int mkv_linear_extend_host(mkv_state_pool *pool, int32_t layer, const vo
  * stored), one rounding per output element. num_rows below 2^24; dim: a multiple of 8, at most
  * 16384; group: a multiple of 8 that divides it. Device pointers 16-byte
  * aligned (d_scales: 4). d_sum or d_out may be d_x or d_residual, in place
- * (not both the same: refused). Squares are summed in f32: a row whose sum
+ * (not both the same); an output that overlaps another buffer otherwise is
+ * refused. Squares are summed in f32: a row whose sum
  * of squares passes 3.4e38 comes out as zeros.
  * Replaces the residual add and RmsNorm::forward around a layer's blocks
  * (inference-model-qwen/src/model.rs:84-109,348-365). */

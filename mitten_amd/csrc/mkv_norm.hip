@@ -188,6 +188,18 @@ extern "C" int mkv_add_rms_norm(int device, const void *d_x, const void *d_resid
     return set_error(MKV_ERR_INVALID_ARGUMENT,
                      "group (%d) must be 0 (one scale per row) or a multiple of 8 that divides dim (%d), with an e4m3 output",
                      group, dim);
+  // Outputs share no byte with anything else, but for the sum and the output in
+  // place of x or of the residual (an element is read and written by one thread).
+  const uint64_t n = (uint64_t)num_rows * dim, nb = n * (dtype == MKV_DTYPE_F32 ? 4 : 2);
+  const struct {
+    const void *p;
+    uint64_t bytes;
+  } bufs[] = {{d_sum, nb},   {d_out, nb}, {d_fp8, n},        {d_scales, (group ? n / group : num_rows) * 4ull},
+              {d_weight, (uint64_t)dim * 4}, {d_x, nb}, {d_residual, nb}};
+  for (int i = 0; i < 4; i++)
+    for (int j = i + 1; j < 7; j++)
+      if (overlap(bufs[i].p, bufs[i].bytes, bufs[j].p, bufs[j].bytes) && !(i < 2 && j >= 5 && bufs[i].p == bufs[j].p))
+        return set_error(MKV_ERR_INVALID_ARGUMENT, "an output overlaps another buffer");
   int ndev = 0;
   if (hipGetDeviceCount(&ndev) != hipSuccess || ndev == 0) {
     (void)hipGetLastError();

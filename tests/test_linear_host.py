@@ -70,3 +70,19 @@ def test_norm_refuses_one_buffer_for_two_outputs():
     p = ctypes.c_void_p
     st = lib.mkv_add_rms_norm(0, p(64), p(96), p(80), 1e-6, 4, 64, 1, p(16), p(16), None, None, 0, None)
     assert st == 1 and "same" in lib.mkv_last_error().decode()
+
+
+@pytest.mark.parametrize("place", [
+    dict(fp8="x"), dict(fp8="residual"), dict(fp8="out"), dict(fp8="sum"), dict(fp8="weight"), dict(scales="x"),
+    dict(scales="fp8"), dict(scales="weight"), dict(out="weight"), dict(sum="weight"), dict(out=("x", 16)),
+    dict(out=("x", -16)), dict(sum=("residual", 512 - 16)), dict(sum=("out", 16)), dict(fp8=("scales", -240)),
+])
+def test_norm_refuses_outputs_over_other_buffers(place):
+    """4 rows of 64 bf16: 512 bytes each, 256 of e4m3, 16 of scales (256 bytes after the e4m3 rows' end)."""
+    at = dict(x=1 << 20, residual=2 << 20, weight=3 << 20, sum=4 << 20, out=5 << 20, fp8=6 << 20, scales=7 << 20)
+    for k, v in place.items():
+        at[k] = at[v] if isinstance(v, str) else at[v[0]] + v[1]
+    lib, p = _lib.device_lib(), ctypes.c_void_p
+    st = lib.mkv_add_rms_norm(0, p(at["x"]), p(at["residual"]), p(at["weight"]), 1e-6, 4, 64, 1, p(at["sum"]),
+                              p(at["out"]), p(at["fp8"]), p(at["scales"]), 0, None)
+    assert st == 1 and "overlaps" in lib.mkv_last_error().decode()
