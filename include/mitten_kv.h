@@ -461,13 +461,20 @@ MKV_API int mkv_qk_norm_rope_append(mkv_pool *pool, int32_t layer, const void *d
 /* ---- linear-attention states ----------------------------------------------- */
 
 /* A linear-attention layer keeps one f32 matrix per value head and sequence
- * in place of K/V rows (the DeltaNet variant of KVCacheState,
- * inference-model-common/src/lib.rs:5-13). For one sequence and value head,
- * with q and k of key head h / (num_v_heads / num_k_heads):
- *   S_t = exp(g_t) S_{t-1} + k_t v_t^T,   o_t = scale * S_t^T q_t,
- * g_t the log decay of token t and head h. A state pool holds the matrices of
- * num_slots sequences in every linear layer:
+ * in place of K/V rows. A state pool holds the matrices of num_slots
+ * sequences in every linear layer:
  *   [num_layers][num_slots][num_v_heads][k_dim][v_dim], f32.
+ * The pool, its slots, forks and copies fit any layer with such a state (the
+ * DeltaNet variant of KVCacheState, inference-model-common/src/lib.rs:5-13,
+ * among them). linear_extend and linear_step compute one recurrence, that of a
+ * scalar decay per head: for one sequence and value head, with q and k of key
+ * head h / (num_v_heads / num_k_heads),
+ *   S_t = exp(g_t) S_{t-1} + k_t v_t^T,   o_t = scale * S_t^T q_t,
+ * g_t the log decay of token t and head h, as retention and scalar-decay
+ * state-space layers have it. The (gated) delta rule is another one: its
+ * S_t = a_t (I - b_t k_t k_t^T) S_{t-1} + b_t k_t v_t^T has a write strength
+ * and an erase term that these calls do not have, so GatedDeltaNet layers
+ * (inference-model-qwen/src/model.rs:425-501) cannot run on them.
  * A slot is to a sequence what its page table is to the K/V pool; slots are
  * handed out by the caller (KvCachePool of mitten_kv_host.h does). */
 typedef struct mkv_state_pool mkv_state_pool;
@@ -549,9 +556,11 @@ MKV_API int mkv_linear_step_host(mkv_state_pool *pool, int32_t layer, const void
  * states between segments 2^-14), and the output is rounded once.
  * Where few long sequences would leave the device idle, their chunks are cut
  * into segments (three launches) whose states stand in d_workspace
- * (mkv_linear_extend_workspace_size bytes, 16-byte aligned; with less, the
- * sequences stay whole), or in a workspace of the pool's own, allocated with
- * it (64 MiB) when d_workspace is NULL. Calls that use the pool's own follow
+ * (mkv_linear_extend_workspace_size bytes, 16-byte aligned; with less, there
+ * are fewer segments, or the sequences stay whole), or in a workspace of the
+ * pool's own, allocated with it (64 MiB) when d_workspace is NULL. (That holds
+ * what the calls want up to 4 segments of 32 heads of 256 x 256 each; more heads
+ * of that size fill the device whole, and ask for none.) Calls that use the pool's own follow
  * one another across streams; a captured one must not be replayed beside
  * another call or graph that uses it (give each a workspace). */
 MKV_API int mkv_linear_extend_workspace_size(const mkv_state_pool *pool, int32_t num_seqs, int32_t num_tokens,

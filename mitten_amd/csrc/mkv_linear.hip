@@ -2,8 +2,8 @@
 // the step that moves each sequence's on by one token.
 //
 // A linear-attention layer keeps, instead of K/V rows, one matrix per value
-// head and sequence (the DeltaNet variant of KVCacheState,
-// inference-model-common/src/lib.rs:5-13):
+// head and sequence. The recurrence here is that of a scalar decay per head
+// (the delta rule, which also erases along k_t, is another):
 //   S_t = exp(g_t) S_{t-1} + k_t v_t^T,   o_t = scale * S_t^T q_t.
 #include <algorithm>
 #include <climits>

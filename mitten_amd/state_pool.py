@@ -1,9 +1,9 @@
 """Linear-attention states and the step between layers, in Python.
 
 `DeviceStatePool` owns one libmitten_kv state pool (HBM, f32, layout
-[num_layers][num_slots][num_v_heads][k_dim][v_dim]: the DeltaNet variant of
-KVCacheState, inference-model-common/src/lib.rs:5-13) and runs the
-linear-attention layers of a hybrid model over it:
+[num_layers][num_slots][num_v_heads][k_dim][v_dim]) and runs linear attention
+with a scalar decay per head over it (S_t = exp(g_t) S_{t-1} + k_t v_t^T, o_t =
+scale S_t^T q_t; not the delta rule, which also erases):
 
     linear_extend(layer, q, k, v, log_decay, q_lens, slots)    ragged prompts
     linear_step(layer, q, k, v, log_decay, slots)              one token per sequence
@@ -120,7 +120,10 @@ def _torch_type(name: str):
 
 
 class DeviceStatePool:
-    """The states of a hybrid model's linear-attention layers."""
+    """The states of a hybrid model's linear-attention layers. Pool, forks and
+    copies fit any layer with one matrix per head (the DeltaNet variant of
+    KVCacheState, inference-model-common/src/lib.rs:5-13, too); linear_extend and
+    linear_step compute the scalar-decay recurrence only."""
 
     def __init__(self, desc: StateDesc, device: int = 0):
         self.desc = desc

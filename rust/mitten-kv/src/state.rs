@@ -1,6 +1,11 @@
-//! The states of a hybrid model's linear-attention layers: the `DeltaNet`
-//! variant of `KVCacheState` (`inference-model-common/src/lib.rs:5-13`) as a
-//! pool of slots beside the K/V pool, and the residual + norm between layers.
+//! The states of a hybrid model's linear-attention layers as a pool of slots
+//! beside the K/V pool, linear attention with a scalar decay per head over them,
+//! and the residual + norm between layers.
+//!
+//! Slots, forks and copies fit the `DeltaNet` variant of `KVCacheState`
+//! (`inference-model-common/src/lib.rs:5-13`) as well; `linear_extend` and
+//! `linear_step` do not compute its recurrence (the delta rule has a write
+//! strength and an erase term, which they lack).
 //!
 //! A request holds one slot instead of a page table; slots come from the same
 //! host allocator as pages (`KvCachePool`, one "page" per slot). A request
