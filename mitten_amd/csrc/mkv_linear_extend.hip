@@ -1014,7 +1014,7 @@ static LinPlan plan_extend(const StatePool *p, int64_t num_seqs, int64_t num_tok
     }
   }
   // Whole sequences of bf16 take 64 columns a workgroup while two to a CU hold
-  // them all (8 prompts of 300-1,500 tokens, 28 heads: 69 us against 85 with
+  // them all (8 prompts of 300-1,500 tokens, 28 heads: 78 us against 88 with
   // 128), else 128, which form the scores once for twice the columns.
   if (r.nseg == 1 && num_seqs * d.num_v_heads * (d.v_dim / 64) <= 2 * p->cus) r.waves = 4;
   return r;

@@ -76,6 +76,10 @@ __device__ __forceinline__ uint32_t abs_bits(float f) { return __float_as_uint(f
 // which bounds it (16,384 rows of 3,584 bf16 with a residual, sum and e4m3 out:
 // 81 us, 5.1 TB/s, what a copy of that size reaches; 64 rows: 4.5 us, the
 // launch and two trips to memory).
+// A group's maximum is taken by each of its threads from the maxima of its
+// chunks: nothing for groups of 64 or 128 columns, but reads that grow with the
+// square of a large group (4,096 rows of 16,384 with groups of 512 columns 110 us,
+// 2,048 152, 8,192 480; one scale per row, which goes by shuffles, 94).
 template <int W, int NC, bool BF16>
 __global__ void __launch_bounds__(64 * W) add_rms_norm_kernel(NormArgs a) {
   __shared__ float red_f[W];
