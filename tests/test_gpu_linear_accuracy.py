@@ -105,3 +105,29 @@ def test_states_keep_f32s_accuracy(dk, dv, n, whole, dtype):
     _, s = extend(q, k, v, g, s0, dtype, whole)
     _, ref, _, _ = reference(*(widen(x) for x in (q, k, v)), g, s0, dk ** -0.5)
     assert norm(s - ref) <= STATE_REL * norm(ref)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("dk,dv", [(64, 128), (128, 128), (128, 256), (256, 128)])
+def test_many_sequences_are_as_accurate(dk, dv, dtype):
+    """Enough of them for workgroups of 128 columns: one rounding per bf16
+    output, states as f32 sums leave them."""
+    import torch
+
+    rng = np.random.default_rng(dk + dv)
+    B, n, hk, hv = 70, 130, 2, 8
+    q, k, v, g = inputs(rng, B * n, hk, hv, dk, dv, dtype, 0.3)
+    s0 = (0.3 * rng.standard_normal((1, B, hv, dk, dv))).astype(np.float32)
+    with DeviceStatePool(StateDesc(1, hk, hv, dk, dv, B, dtype)) as pool:
+        pool.tensor().copy_(torch.from_numpy(s0))
+        o = pool.linear_extend(0, *(to_device(x) for x in (q, k, v, g)), [n] * B, np.arange(B))
+        pool.check()
+        o, s = widen(to_host(o)).astype(np.float64), pool.tensor().cpu().numpy()[0]
+    for b in (0, 33, B - 1):
+        r = slice(b * n, (b + 1) * n)
+        ref, rs, _, _ = reference(*(widen(x[r]) for x in (q, k, v)), g[r], s0[0, b], dk ** -0.5)
+        if dtype == "bf16":
+            assert norm(o[r] - ref) <= 1.02 * norm(widen(orc.f32_to_bf16(ref.astype(np.float32))) - ref)
+        else:
+            assert norm(o[r] - ref) <= STATE_REL * norm(ref)
+        assert norm(s[b] - rs) <= STATE_REL * norm(rs)

@@ -16,14 +16,22 @@ pytestmark = pytest.mark.gpu
 
 def run(form, q, k, v, g, s0, dtype):
     """(outputs, state) of one sequence: "step" token by token, "whole" (a
-    workspace with no room), "segments" (as planned)."""
+    workspace with no room), "segments" (as planned), "many" (with 140 others like
+    it, which take workgroups of 128 columns where v has them)."""
     import torch
 
     hk, dk, (n, hv, dv) = q.shape[1], q.shape[2], v.shape
     dev = [to_device(orc.f32_to_bf16(x) if dtype == "bf16" else x) for x in (q, k, v)] + [to_device(g)]
-    with DeviceStatePool(StateDesc(1, hk, hv, dk, dv, 1, dtype)) as pool:
+    many = 141 if form == "many" else 1
+    with DeviceStatePool(StateDesc(1, hk, hv, dk, dv, many, dtype)) as pool:
         pool.tensor().copy_(torch.from_numpy(s0[None, None]))
-        if form == "step":
+        if form == "many":
+            o = pool.linear_extend(0, *(torch.cat([x] * many) for x in dev), [n] * many, np.arange(many))
+            o, states = o.view(many, n, hv, dv), pool.tensor()[0]
+            bits = [x.view(torch.int16 if x.dtype == torch.bfloat16 else torch.int32) for x in (o, states)]
+            assert all(bool((x == x[:1]).all()) for x in bits), "equal sequences differ"
+            o = o[0]
+        elif form == "step":
             o = torch.cat([pool.linear_step(0, *(x[t:t + 1] for x in dev), [0]) for t in range(n)])
         else:
             assert form == "whole" or pool.linear_extend_workspace_size(1, n, n) > 0
@@ -56,11 +64,11 @@ def make(n, dk, dv, dtype, seed):
     return q, k, v, g, rng.standard_normal((2, dk, dv)).astype(np.float32)
 
 
-FORMS = [("step", 20), ("whole", 20), ("whole", 200), ("segments", 1400)]
+FORMS = [("step", 20), ("whole", 20), ("whole", 200), ("segments", 1400), ("many", 150)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (256, 64)])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (64, 128), (128, 128), (256, 64), (256, 128)])
 @pytest.mark.parametrize("form,n", FORMS)
 @pytest.mark.parametrize("decay", [-np.inf, -200.0, -95.0, -3.0])
 def test_an_infinite_state_behind_a_decay(form, n, dk, dv, decay, dtype):
@@ -110,7 +118,7 @@ def recurrence32(q, k, v, g, s0, scale):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (256, 64)])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (64, 128), (128, 128), (256, 64), (256, 128)])
 @pytest.mark.parametrize("form,n", FORMS + [("whole", 64)])
 @pytest.mark.parametrize("what", ["state", "state and decays", "score", "score of two states", "q inf", "q nan"])
 def test_overflow_and_odd_queries(form, n, dk, dv, what, dtype):
