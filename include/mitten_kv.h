@@ -553,7 +553,10 @@ MKV_API int mkv_linear_step_host(mkv_state_pool *pool, int32_t layer, const void
  * skipped. Slots, types and forms as in mkv_linear_step; sums, decays and
  * states are f32 or wider; with bf16 rows the scores, and the state where an
  * output reads it, enter products in 16 bits (2^-15 of a term; a term of the
- * states between segments 2^-14), and the output is rounded once.
+ * states between segments 2^-14), and the output is rounded once. Infinities,
+ * NaN and overflows are the recurrence's: from a chunk of tokens with one of
+ * them, or with a number of 2^64 or more in k or v, the sequence (or its segment)
+ * is computed token by token, which is slower.
  * Where few long sequences would leave the device idle, their chunks are cut
  * into segments (three launches) whose states stand in d_workspace
  * (mkv_linear_extend_workspace_size bytes, 16-byte aligned; with less, there

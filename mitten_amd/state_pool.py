@@ -329,7 +329,9 @@ class DeviceStatePool:
 
     def _bind(self, q, k, v, log_decay, q_lens, slots, out, src_slots, scale, stream):
         L = self.desc.num_layers
-        lead = (L,) if q.dim() == 4 else ()
+        if out is None:
+            raise _bad("a bound call needs out")
+        lead = (L,) if getattr(q, "ndim", 0) == 4 else ()
         n, out, scale, flags = self._rows(q, k, v, log_decay, out, scale, lead, stream)
         # (The lengths are checked against q's rows here, and here only.)
         q_lens, slots, src_slots = (_host_copy(x) for x in (q_lens, slots, src_slots))
@@ -352,6 +354,8 @@ class DeviceStatePool:
         device = self.device
 
         def run(layer: int) -> None:
+            if not 0 <= layer < L:
+                raise _bad(f"layer {layer} out of range [0, {L})")
             # (self._h is None after close(), which the library refuses.)
             st = fn(self._h, *args[layer], _raw_stream(stream, device))
             if st:

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from mitten_amd import STATE_NONE, DeviceStatePool, StateDesc, state_pool
+from mitten_amd import STATE_NONE, BackendError, DeviceStatePool, StateDesc, state_pool
 
 
 class Recorder:
@@ -95,3 +95,20 @@ def test_a_run_after_close_has_no_pool(pool, step):
     pool._h = None
     run(0)
     assert [h for h, _ in pool._lib.at] == [77, None]
+
+
+@pytest.mark.parametrize("step", [False, True])
+def test_a_bound_call_needs_out_and_a_layer_of_the_pool(pool, step):
+    """(Layer -1 would be the last one of the list of calls.)"""
+    io, out = rows(3)
+    bind, more = (pool.bind_linear_step, ()) if step else (pool.bind_linear_extend, ([1, 1, 1],))
+    with pytest.raises(BackendError):
+        bind(*io, *more, [1, 2, 3], None, stream=pool.stream)
+    with pytest.raises(BackendError):
+        bind(None, *io[1:], *more, [1, 2, 3], out, stream=pool.stream)
+    run = bind(*io, *more, [1, 2, 3], out, stream=pool.stream)
+    for layer in (-1, 2):
+        with pytest.raises(BackendError) as ei:
+            run(layer)
+        assert f"layer {layer} out of range" in str(ei.value)
+    assert not pool._lib.calls
