@@ -789,19 +789,22 @@ class DeviceKvPool:
                                              kernel, cached_loads)
         fn = self._lib.mkv_decode_step if gather_out is None else self._lib.mkv_decode_step_gather
         gx = () if gather_out is None else self._gather_outputs(gather_out)
-        h, ph = self._h, plan._h
         sh = _stream_handle(stream)
         kv_stride = B * d.num_kv_heads * d.head_dim * d.elem_bytes
         qo_stride = B * d.num_q_heads * d.head_dim * d.elem_bytes
         kb, vb, qb, ob = k_new.data_ptr(), v_new.data_ptr(), q.data_ptr(), out.data_ptr()
         ip, ix = _tptr(block_indptr), _tptr(block_ids)
-        args = [(h, ph, layer, ctypes.c_void_p(kb + layer * kv_stride), ctypes.c_void_p(vb + layer * kv_stride),
+        args = [(layer, ctypes.c_void_p(kb + layer * kv_stride), ctypes.c_void_p(vb + layer * kv_stride),
                  ctypes.c_void_p(qb + layer * qo_stride), ctypes.c_void_p(ob + layer * qo_stride), ip, ix)
                 + gx + (scale, flags, sh) for layer in range(L)]
         keep = (k_new, v_new, q, out, block_indptr, block_ids, gather_out)
 
         def run(layer: int) -> None:
-            st = fn(*args[layer])
+            # (Either handle is None after close(), which the library refuses. A plan
+            # may be built again between runs, for as many sequences.)
+            if plan.num_seqs != B:
+                raise BackendError(MKV_ERR_INVALID_ARGUMENT, f"bound for {B} sequences, the plan has {plan.num_seqs}")
+            st = fn(self._h, plan._h, *args[layer])
             if st:
                 _raise(st)
 
@@ -831,13 +834,17 @@ class DeviceKvPool:
         kb, vb, qb, ob = k_new.data_ptr(), v_new.data_ptr(), q.data_ptr(), out.data_ptr()
         pre, npre = _tptr(prefix_ids), 0 if prefix_ids is None else int(prefix_ids.shape[0])
         ip, ix, sh = _tptr(block_indptr), _tptr(block_ids), _stream_handle(stream)
-        args = [(self._h, plan._h, layer, ctypes.c_void_p(kb + layer * kv_stride),
+        args = [(layer, ctypes.c_void_p(kb + layer * kv_stride),
                  ctypes.c_void_p(vb + layer * kv_stride), ctypes.c_void_p(qb + layer * qo_stride),
                  ctypes.c_void_p(ob + layer * qo_stride), pre, npre, ip, ix, scale, flags, sh) for layer in range(L)]
         keep = (k_new, v_new, q, out, prefix_ids, block_indptr, block_ids)
 
         def run(layer: int) -> None:
-            st = fn(*args[layer])
+            # (Either handle is None after close(), which the library refuses. A plan
+            # may be built again between runs, for as many sequences.)
+            if plan.num_seqs != B:
+                raise BackendError(MKV_ERR_INVALID_ARGUMENT, f"bound for {B} sequences, the plan has {plan.num_seqs}")
+            st = fn(self._h, plan._h, *args[layer])
             if st:
                 _raise(st)
 
