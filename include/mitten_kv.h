@@ -22,6 +22,10 @@
  *   state_copy        copies of states between slots (fork, compaction)
  *   add_rms_norm      residual + RMSNorm, output in the model's type or e4m3
  *
+ * A pool of a second type holds the K/V rows in 8 bits (mkv_kv8_*: append,
+ * qk_norm_rope_append, gather, copy_blocks, decode_step, decode_attention and
+ * extend_attention over e4m3 tiles with a power-of-two scale per block and head).
+ *
  * Pool layout in HBM (design/rust-inference-engine-design.md:1380-1387):
  *   [num_layers][2 (K then V)][num_blocks][page_size][num_kv_heads][head_dim]
  * A slot id is block * page_size + offset_in_block.
@@ -110,7 +114,8 @@ enum {
 /* qk_norm_rope_append flags. */
 enum {
   MKV_PREP_PLAIN_Q = 1u << 0, /* d_q is [n][num_q_heads][head_dim] (no gate half) */
-  MKV_PREP_NO_NORM = 1u << 1  /* skip the RMSNorm (RoPE and append only) */
+  MKV_PREP_NO_NORM = 1u << 1, /* skip the RMSNorm (RoPE and append only) */
+  MKV_PREP_INTERLEAVED = 1u << 2 /* 8-bit pools: pairs are dims (2i, 2i + 1), not (i, i + rotary_dim/2) */
 };
 
 typedef struct mkv_pool mkv_pool;
@@ -601,6 +606,147 @@ MKV_API int mkv_linear_extend_host(mkv_state_pool *pool, int32_t layer, const vo
 MKV_API int mkv_add_rms_norm(int device, const void *d_x, const void *d_residual, const float *d_weight, float eps,
                              int32_t num_rows, int32_t dim, int32_t dtype, void *d_sum, void *d_out, void *d_fp8,
                              float *d_scales, int32_t group, void *stream);
+
+/* ---- the K/V cache in 8 bits --------------------------------------------------- */
+
+/* A second pool type beside mkv_pool: the rows of each (layer, K or V, block of
+ * 16 tokens, KV head) are one tile of 16 * head_dim OCP e4m3 bytes with one
+ * exponent e; a byte stands for its e4m3 value times 2^e. It holds twice the
+ * tokens of a bf16 pool, and attention reads half the bytes.
+ *   tiles:     [num_layers][2 (K then V)][num_blocks][num_kv_heads][16 * head_dim] bytes
+ *   exponents: [num_layers][2][num_blocks][num_kv_heads] int8
+ * A tile is in the order in which the matrix instructions read it:
+ *   K: [head_dim / 16][16 tokens][16 dims]
+ *   V: [head_dim / 64][4 token quads][16 dim quads][4 dims][4 tokens]
+ * mkv_pool_desc describes it, with head_dim 64, 128 or 256 and dtype the type of
+ * the rows that go in and out (k, v, q, o).
+ *
+ * A tile's exponent is the least e >= -100 with max |x| <= 448 * 2^e over the
+ * finite values written; a NaN or an infinity is held as NaN. The new rows of a
+ * sequence are positions ctx - n .. ctx - 1. A tile whose row 0 is among them
+ * starts afresh: its other rows become zeros, its exponent is the new rows'. In
+ * any other tile e becomes the greater of its own and the new rows'; if that is
+ * greater than before, its other rows are expressed under it, rounded to nearest
+ * (which changes only values below 2^-6 of the new scale). Rows of a sequence
+ * that is cut back (ctx falls) may be written again; the exponent stays.
+ *
+ * Every call names the sequences by their page tables, as extend_attention does:
+ * a block that a call writes must not be in another sequence's part of the same
+ * call (the host forms refuse it, and a table with an id outside the pool). In
+ * the device forms a sequence whose numbers do not fit is skipped and reported as
+ * by mkv_extend_attention (its rows of o stay as they are); ctx 0 is a padding
+ * sequence: nothing is written for it but zeros in its row of o. Rows behind the last
+ * sequence stay as they are. */
+typedef struct mkv_kv8_pool mkv_kv8_pool;
+
+/* Bytes of the tiles and of the exponents. */
+MKV_API int mkv_kv8_required_bytes(const mkv_pool_desc *desc, uint64_t *out_tile_bytes, uint64_t *out_exponent_bytes);
+/* Allocate the pool and its workspace (64 MiB) on `device` (hipMalloc; contents
+ * uninitialised). MKV_ERR_OUT_OF_MEMORY if HBM cannot hold them. */
+MKV_API int mkv_kv8_pool_create(const mkv_pool_desc *desc, int device, mkv_kv8_pool **out_pool);
+MKV_API int mkv_kv8_pool_destroy(mkv_kv8_pool *pool);
+MKV_API int mkv_kv8_pool_get_desc(const mkv_kv8_pool *pool, mkv_pool_desc *out_desc);
+MKV_API int mkv_kv8_pool_buffers(const mkv_kv8_pool *pool, void **out_tiles, uint64_t *out_tile_bytes,
+                                 void **out_exponents, uint64_t *out_exponent_bytes);
+/* As mkv_pool_check, for this pool's device error word. */
+MKV_API int mkv_kv8_pool_check(mkv_kv8_pool *pool, void *stream, uint32_t *out_bits);
+
+/* Quantise and write the new rows d_k, d_v: [num_tokens][num_kv_heads][head_dim],
+ * sequence b's n_b = d_q_indptr[b+1] - d_q_indptr[b] rows at d_q_indptr[b], for
+ * positions d_ctx_lens[b] - n_b .. d_ctx_lens[b] - 1 of the table
+ * d_block_ids[d_block_indptr[b] ..). max_q_len sizes the launch (a longer chunk is
+ * written all the same). num_seqs at most 65535. */
+MKV_API int mkv_kv8_append(mkv_kv8_pool *pool, int32_t layer, const void *d_k, const void *d_v,
+                           const int32_t *d_q_indptr, const int32_t *d_block_indptr, const int32_t *d_block_ids,
+                           const int32_t *d_ctx_lens, int32_t num_seqs, int32_t num_tokens, int32_t max_q_len,
+                           void *stream);
+MKV_API int mkv_kv8_append_host(mkv_kv8_pool *pool, int32_t layer, const void *d_k, const void *d_v,
+                                const int32_t *h_q_lens, const int32_t *h_ctx_lens, const uint32_t *h_block_indptr,
+                                const uint32_t *h_block_ids, int32_t num_seqs, void *stream);
+
+/* The step before attention, fused with that append: RMSNorm(1 + w) of every q
+ * and k head (or MKV_PREP_NO_NORM), rotary positions on dims [0, rotary_dim), k
+ * and v quantised and written, q to d_q_out [num_tokens][num_q_heads][head_dim].
+ * Pairs of dims (i, i + rotary_dim/2), or (2i, 2i + 1) with MKV_PREP_INTERLEAVED;
+ * pair i of the token at position p turns by the angle p * d_inv_freq[i], formed
+ * in f64 (p up to 2^31 - 1), and is multiplied by rope_factor (1 for plain RoPE;
+ * methods that stretch the context scale cos and sin by one). d_positions: int32
+ * per token, or NULL for the positions in the sequence. d_q: gated
+ * [num_tokens][num_q_heads][2][head_dim], or [..][num_q_heads][head_dim] with
+ * MKV_PREP_PLAIN_Q. rotary_dim: a multiple of 8, 0 to head_dim. All in f32, one
+ * rounding per value of q and per byte. d_q_out must not overlap d_q, d_k or d_v,
+ * but may be d_q itself with MKV_PREP_PLAIN_Q. */
+MKV_API int mkv_kv8_qk_norm_rope_append(mkv_kv8_pool *pool, int32_t layer, const void *d_q, const void *d_k,
+                                        const void *d_v, const float *d_q_norm_w, const float *d_k_norm_w,
+                                        const float *d_inv_freq, int32_t rotary_dim, float eps, float rope_factor,
+                                        const int32_t *d_positions, const int32_t *d_q_indptr,
+                                        const int32_t *d_block_indptr, const int32_t *d_block_ids,
+                                        const int32_t *d_ctx_lens, int32_t num_seqs, int32_t num_tokens,
+                                        int32_t max_q_len, void *d_q_out, uint32_t flags, void *stream);
+MKV_API int mkv_kv8_qk_norm_rope_append_host(mkv_kv8_pool *pool, int32_t layer, const void *d_q, const void *d_k,
+                                             const void *d_v, const float *d_q_norm_w, const float *d_k_norm_w,
+                                             const float *d_inv_freq, int32_t rotary_dim, float eps,
+                                             float rope_factor, const int32_t *h_positions, const int32_t *h_q_lens,
+                                             const int32_t *h_ctx_lens, const uint32_t *h_block_indptr,
+                                             const uint32_t *h_block_ids, int32_t num_seqs, void *d_q_out,
+                                             uint32_t flags, void *stream);
+
+/* Read back: as mkv_gather, the rows in the pool's dtype (a bf16 row is exact
+ * but where 2^e carries a value out of its range). d_ctx_lens in place of a token indptr: sequence b's
+ * rows start at element (sum of the earlier lengths) * Hkv * D. A sequence that
+ * would pass out_capacity_tokens is skipped and reported (MKV_DEVERR_CTX). */
+MKV_API int mkv_kv8_gather(mkv_kv8_pool *pool, int32_t layer, const int32_t *d_block_indptr,
+                           const int32_t *d_block_ids, const int32_t *d_ctx_lens, int32_t num_seqs,
+                           int32_t max_ctx_len, void *d_out_k, void *d_out_v, int64_t out_capacity_tokens,
+                           void *stream);
+MKV_API int mkv_kv8_gather_host(mkv_kv8_pool *pool, int32_t layer, const uint32_t *h_block_indptr,
+                                const uint32_t *h_block_ids, const int32_t *h_ctx_lens, int32_t num_seqs,
+                                void *d_out_k, void *d_out_v, int64_t out_capacity_tokens, void *stream);
+
+/* Whole blocks with their exponents, all layers, as mkv_copy_blocks (_host). */
+MKV_API int mkv_kv8_copy_blocks(mkv_kv8_pool *pool, const int32_t *d_src_blocks, const int32_t *d_dst_blocks,
+                                int32_t num_pairs, void *stream);
+MKV_API int mkv_kv8_copy_blocks_host(mkv_kv8_pool *pool, const uint32_t *h_src_blocks, const uint32_t *h_dst_blocks,
+                                     int32_t num_pairs, void *stream);
+
+/* One query row per sequence over its first d_ctx_lens[b] tokens, as
+ * mkv_decode_attention; with d_k_new, d_v_new ([num_seqs][num_kv_heads][head_dim],
+ * both or neither) the row is first appended at position ctx - 1 and attended as
+ * the tile holds it. max_ctx_len bounds the lengths (a longer one is reported,
+ * MKV_DEVERR_CTX, and skipped) and sizes the launch; lengths and tables are read
+ * when the kernels run. Long contexts are cut into equal pieces over all
+ * sequences, whose partials (f32) stand in d_workspace
+ * (mkv_kv8_workspace_size bytes, 16-byte aligned; with less there are fewer
+ * pieces) or, when it is NULL, in the pool's own. Calls that use the pool's own
+ * follow one another across streams; a captured one must not be replayed beside
+ * another call or graph that uses it (give each a workspace). Scores, sums and
+ * partials are f32; weights enter the product with V in 11 bits (bf16 rows) or
+ * 22 (f32 rows). Flags: MKV_ATTN_ZERO_SINK. num_seqs at most 65535. */
+MKV_API int mkv_kv8_decode_attention(mkv_kv8_pool *pool, int32_t layer, const void *d_k_new, const void *d_v_new,
+                                     const void *d_q, void *d_o, const int32_t *d_block_indptr,
+                                     const int32_t *d_block_ids, const int32_t *d_ctx_lens, int32_t num_seqs,
+                                     int32_t max_ctx_len, float scale, uint32_t flags, void *d_workspace,
+                                     uint64_t workspace_bytes, void *stream);
+MKV_API int mkv_kv8_decode_attention_host(mkv_kv8_pool *pool, int32_t layer, const void *d_k_new,
+                                          const void *d_v_new, const void *d_q, void *d_o,
+                                          const int32_t *h_ctx_lens, const uint32_t *h_block_indptr,
+                                          const uint32_t *h_block_ids, int32_t num_seqs, float scale, uint32_t flags,
+                                          void *stream);
+/* Bytes with which no decode or extend call of this pool is held back. */
+MKV_API int mkv_kv8_workspace_size(const mkv_kv8_pool *pool, uint64_t *out_bytes);
+
+/* Causal attention of each sequence's newest tokens, as mkv_extend_attention, the
+ * chunk's rows written before by an append. Few short chunks over long contexts
+ * split their key ranges (two launches), with partials in the workspace as above. */
+MKV_API int mkv_kv8_extend_attention(mkv_kv8_pool *pool, int32_t layer, const void *d_q, void *d_o,
+                                     const int32_t *d_q_indptr, const int32_t *d_block_indptr,
+                                     const int32_t *d_block_ids, const int32_t *d_ctx_lens, int32_t num_seqs,
+                                     int32_t num_tokens, int32_t max_q_len, int32_t max_ctx_len, float scale,
+                                     uint32_t flags, void *d_workspace, uint64_t workspace_bytes, void *stream);
+MKV_API int mkv_kv8_extend_attention_host(mkv_kv8_pool *pool, int32_t layer, const void *d_q, void *d_o,
+                                          const int32_t *h_q_lens, const int32_t *h_ctx_lens,
+                                          const uint32_t *h_block_indptr, const uint32_t *h_block_ids,
+                                          int32_t num_seqs, float scale, uint32_t flags, void *stream);
 
 /* ---- KV block wire format --------------------------------------------------- */
 

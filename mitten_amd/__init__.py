@@ -8,6 +8,10 @@ Device side (libmitten_kv.so, hand-written gfx950 HIP):
     DeviceStatePool   the states of linear-attention layers (linear_extend,
                       linear_step, copy_states), beside add_rms_norm, the
                       residual + norm between layers
+    DeviceKv8Pool     the K/V pool in 8 bits: e4m3 tiles with a power-of-two
+                      scale per block and head, the steps that write it
+                      (append, qk_norm_rope_append), gather, copy_blocks and
+                      attention over it (decode_step, extend_attention)
 Host side (libmitten_kvhost.so, C++):
     KvCachePool, PageTable, RadixCache, BlockManager
                       the engine's page allocator, radix prefix cache and
@@ -25,6 +29,12 @@ from .device_pool import (  # noqa: F401
     validate_block_tables,
     validate_copy_pairs,
     validate_slots,
+)
+from .kv8_pool import (  # noqa: F401
+    KV8_MIN_EXP,
+    DeviceKv8Pool,
+    kv8_required_bytes,
+    rope_scaled_inv_freq,
 )
 from .state_pool import (  # noqa: F401
     STATE_NONE,

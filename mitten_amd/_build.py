@@ -21,7 +21,7 @@ DEVICE_LIB = os.path.join(LIBDIR, "libmitten_kv.so")
 HOST_LIB = os.path.join(LIBDIR, "libmitten_kvhost.so")
 
 DEVICE_SOURCES = ["mkv_pool.hip", "mkv_attention.hip", "mkv_extend.hip", "mkv_prep.hip", "mkv_wire.hip",
-                  "mkv_linear.hip", "mkv_linear_extend.hip", "mkv_norm.hip"]
+                  "mkv_linear.hip", "mkv_linear_extend.hip", "mkv_norm.hip", "mkv_kv8.hip", "mkv_kv8_attn.hip"]
 HOST_SOURCES = ["host/kv_host.cpp"]
 
 ARCH = "gfx950"

@@ -121,6 +121,28 @@ DEVICE_SIGNATURES = {
     "mkv_linear_extend_workspace_size": (c_int, [P, i32, i32, i32, ctypes.POINTER(u64)]),
     "mkv_linear_extend_host": (c_int, [P, i32, P, P, P, P, P, I32P, U32P, U32P, i32, f32, u32, P]),
     "mkv_add_rms_norm": (c_int, [c_int, P, P, P, f32, i32, i32, i32, P, P, P, P, i32, P]),
+    "mkv_kv8_required_bytes": (c_int, [DESC_P, ctypes.POINTER(u64), ctypes.POINTER(u64)]),
+    "mkv_kv8_pool_create": (c_int, [DESC_P, c_int, ctypes.POINTER(P)]),
+    "mkv_kv8_pool_destroy": (c_int, [P]),
+    "mkv_kv8_pool_get_desc": (c_int, [P, DESC_P]),
+    "mkv_kv8_pool_buffers": (c_int, [P, ctypes.POINTER(P), ctypes.POINTER(u64), ctypes.POINTER(P),
+                                     ctypes.POINTER(u64)]),
+    "mkv_kv8_pool_check": (c_int, [P, P, ctypes.POINTER(u32)]),
+    "mkv_kv8_append": (c_int, [P, i32, P, P, P, P, P, P, i32, i32, i32, P]),
+    "mkv_kv8_append_host": (c_int, [P, i32, P, P, I32P, I32P, U32P, U32P, i32, P]),
+    "mkv_kv8_qk_norm_rope_append": (c_int, [P, i32, P, P, P, P, P, P, i32, f32, f32, P, P, P, P, P, i32, i32, i32, P,
+                                            u32, P]),
+    "mkv_kv8_qk_norm_rope_append_host": (c_int, [P, i32, P, P, P, P, P, P, i32, f32, f32, I32P, I32P, I32P, U32P,
+                                                 U32P, i32, P, u32, P]),
+    "mkv_kv8_gather": (c_int, [P, i32, P, P, P, i32, i32, P, P, i64, P]),
+    "mkv_kv8_gather_host": (c_int, [P, i32, U32P, U32P, I32P, i32, P, P, i64, P]),
+    "mkv_kv8_copy_blocks": (c_int, [P, P, P, i32, P]),
+    "mkv_kv8_copy_blocks_host": (c_int, [P, U32P, U32P, i32, P]),
+    "mkv_kv8_decode_attention": (c_int, [P, i32, P, P, P, P, P, P, P, i32, i32, f32, u32, P, u64, P]),
+    "mkv_kv8_decode_attention_host": (c_int, [P, i32, P, P, P, P, I32P, U32P, U32P, i32, f32, u32, P]),
+    "mkv_kv8_workspace_size": (c_int, [P, ctypes.POINTER(u64)]),
+    "mkv_kv8_extend_attention": (c_int, [P, i32, P, P, P, P, P, P, i32, i32, i32, i32, f32, u32, P, u64, P]),
+    "mkv_kv8_extend_attention_host": (c_int, [P, i32, P, P, I32P, I32P, U32P, U32P, i32, f32, u32, P]),
     "mkv_validate_slots": (c_int, [DESC_P, I32P, i32]),
     "mkv_validate_block_tables": (c_int, [DESC_P, I32P, I32P, I32P, i32, i32]),
     "mkv_validate_copy_pairs": (c_int, [DESC_P, I32P, I32P, i32]),

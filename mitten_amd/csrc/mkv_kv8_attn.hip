@@ -1,0 +1,1190 @@
+// Attention over the K/V pool in 8 bits: one query row per sequence (decode, with
+// the row's append fused in) and chunks of new tokens (extend).
+//
+// For a query row q and the keys it sees, with byte values k', v' and the
+// exponents ek, ev of their tiles:
+//   s_j = scale * log2(e) * q . (k'_j 2^ek),  o = sum_j 2^(s_j - m) v'_j 2^ev / sum_j 2^(s_j - m).
+// S^T = K.Q^T runs on v_mfma_f32_16x16x32_bf16: a byte times its power of two is
+// exact in bf16 (the conversion multiplies). A bf16 q is one operand, an f32 q three
+// (8 + 8 + 8 bits), so the products are exact and the sums f32.
+// O^T = V^T.P^T runs on v_mfma_f32_16x16x32_f16: a byte is exact in f16, and the
+// weight carries the tile's exponent: with E the greatest ev so far and d = ev - E,
+//   p_j = 2^(s_j + d - R),  O = sum_j p_j v'_j,  l = sum_j 2^-d p_j,  o = 2^E O / l,
+// R a running maximum of s_j + d (moved when one passes it by more than kRescaleSlack).
+// p is f16 with 11 bits where it matters: it is held times 2^kBias, so at most
+// 2^15, and a weight 2^-21 below the greatest is still a normal number. (In bf16 its
+// 8 bits would add as much error as the rounding of a bf16 result, 1.41 of it
+// together.) f32 rows take two f16 parts (22 bits).
+//
+// 32 keys (two blocks) per softmax step: the k-slots of lane group g4 in the PV
+// product are keys 4 g4 .. +3 of the first block, then of the second, where S^T
+// left the scores.
+#include "mkv_kv8.h"
+
+namespace mkv {
+
+constexpr float kBias = 15.0f - kRescaleSlack;
+constexpr int kFarExp = 40;  // a tile 2^-40 below the greatest adds nothing to O that f32 keeps
+constexpr int kNoExp = -1000;
+
+template <int D, bool F32>
+struct Kv8Q {
+  static constexpr int QP = F32 ? 3 : 1;
+  bf16x8 op[QP][D / 64][2];
+  // Lane holds q[row of lane % 16][64 r + 16 g4 + 8 half .. +8].
+  __device__ __forceinline__ void load(const void *q, int64_t row, int g4) {
+#pragma unroll
+    for (int r = 0; r < D / 64; r++)
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        const int64_t at = row * D + 64 * r + 16 * g4 + 8 * half;
+        if constexpr (F32) {
+          const f32x4 *p = reinterpret_cast<const f32x4 *>(static_cast<const float *>(q) + at);
+          const f32x4 a = p[0], b = p[1];
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            float x = j < 4 ? a[j & 3] : b[j & 3];
+#pragma unroll
+            for (int part = 0; part < 3; part++) {
+              const __bf16 y = (__bf16)x;
+              op[part][r][half][j] = y;
+              x -= (float)y;
+            }
+          }
+        } else {
+          op[0][r][half] =
+              __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(q) + at));
+        }
+      }
+  }
+};
+
+// Eight bytes of K as an operand, times 2^ek.
+__device__ __forceinline__ bf16x8 kv8_k_operand(uint32_t w0, uint32_t w1, float scale) {
+  union {
+    bf16x2v p[4];
+    bf16x8 v;
+  } u;
+  u.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, false);
+  u.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, true);
+  u.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, false);
+  u.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, true);
+  return u.v;
+}
+// Four bytes of V as f16.
+__device__ __forceinline__ uint2 kv8_v_half(uint32_t w) {
+  const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false);
+  const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true);
+  return make_uint2(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
+}
+
+// Softmax state of 16 query rows: row of lane % 16. O[i][n][c] is dim 64 i + 16 g4 + 4 c + n.
+template <int D>
+struct Kv8State {
+  f32x4 O[D / 64][4];
+  float R, l;
+  __device__ __forceinline__ void reset() {
+#pragma unroll
+    for (int i = 0; i < D / 64; i++)
+#pragma unroll
+      for (int n = 0; n < 4; n++) O[i][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    R = -INFINITY;
+    l = 0.0f;
+  }
+  __device__ __forceinline__ void scale_o(float f) {
+#pragma unroll
+    for (int i = 0; i < D / 64; i++)
+#pragma unroll
+      for (int n = 0; n < 4; n++) O[i][n] *= f;
+  }
+  // E grows by de: s + d falls by it, so R follows and O stays; l is relative to
+  // R alone. (Steps past 2^40, or an l about to leave f32, move O instead.)
+  __device__ __forceinline__ void raise(int de) {
+    const int dc = __ballot(l > 0x1p60f) ? 0 : min(de, kFarExp);
+    R -= (float)dc;
+    l = __builtin_ldexpf(l, dc);
+    if (dc != de) scale_o(__builtin_ldexpf(1.0f, dc - de));
+  }
+};
+
+// The weights of two blocks, from t = s + d (hidden keys -inf): state moved on,
+// operands of the PV product in p (and the second part of f32 rows in p2).
+template <int D, bool F32>
+__device__ __forceinline__ void kv8_weights(const float (&t)[2][4], const int (&d)[2], const int (&far)[2],
+                                            Kv8State<D> &st, f16x8 &p, f16x8 &p2) {
+  float top = fmaxf(fmaxf(fmaxf(t[0][0], t[0][1]), fmaxf(t[0][2], t[0][3])),
+                    fmaxf(fmaxf(t[1][0], t[1][1]), fmaxf(t[1][2], t[1][3])));
+  if (__ballot(top > st.R + kRescaleSlack)) {
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float R = top > st.R + kRescaleSlack ? top : st.R;
+    const float f = st.R == -INFINITY ? 0.0f : fast_exp2(st.R - R);
+    st.l *= f;
+    st.scale_o(f);
+    st.R = R;
+  }
+  const float base = st.R == -INFINITY ? 0.0f : st.R - kBias;
+#pragma unroll
+  for (int kb = 0; kb < 2; kb++) {
+    float w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = fast_exp2(t[kb][i] - base);
+    st.l += __builtin_ldexpf((w[0] + w[1]) + (w[2] + w[3]), -d[kb]);
+    if (far[kb]) {  // (uniform, rare)
+      const float f = __builtin_ldexpf(1.0f, far[kb]);
+#pragma unroll
+      for (int i = 0; i < 4; i++) w[i] *= f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const _Float16 h = (_Float16)w[i];
+      p[4 * kb + i] = h;
+      if constexpr (F32) p2[4 * kb + i] = (_Float16)(w[i] - (float)h);
+    }
+  }
+}
+
+// E of a step with tile exponents ev (two blocks): raised where needed; d >= -kFarExp
+// and what is left of ev - E beyond that.
+template <int D, int RT>
+__device__ __forceinline__ void kv8_exponents(int &E, int ev0, int ev1, Kv8State<D> (&st)[RT], int (&d)[2],
+                                              int (&far)[2]) {
+  const int top = max(ev0, ev1);
+  if (top > E) {
+    if (E != kNoExp)
+#pragma unroll
+      for (int i = 0; i < RT; i++) st[i].raise(top - E);
+    E = top;
+  }
+  d[0] = max(ev0 - E, -kFarExp);
+  d[1] = max(ev1 - E, -kFarExp);
+  far[0] = ev0 - E - d[0];
+  far[1] = ev1 - E - d[1];
+}
+
+// A finished row: the result, or its partial (m, l, O) for a merge.
+template <int D, bool F32>
+__device__ __forceinline__ void kv8_store(const Kv8State<D> &st, int E, int g4, bool final, void *o, int64_t row,
+                                          float *ws_ml, float *ws_o, int64_t prow, int32_t zero_sink) {
+  const float m = st.R == -INFINITY ? -INFINITY : st.R - kBias;
+  float f = E == kNoExp ? 0.0f : __builtin_ldexpf(1.0f, E);
+  if (final) f *= final_scale(m, st.l, zero_sink);
+#pragma unroll
+  for (int i = 0; i < D / 64; i++) {
+    float y[16];
+#pragma unroll
+    for (int c = 0; c < 4; c++)
+#pragma unroll
+      for (int n = 0; n < 4; n++) y[4 * c + n] = st.O[i][n][c] * f;
+    const int64_t at = (final ? row : prow) * D + 64 * i + 16 * g4;
+    if (final && !F32) {
+#pragma unroll
+      for (int z = 0; z < 2; z++)
+        reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(o) + at)[z] =
+            u32x4{pack_bf16x2(y[8 * z], y[8 * z + 1]), pack_bf16x2(y[8 * z + 2], y[8 * z + 3]),
+                  pack_bf16x2(y[8 * z + 4], y[8 * z + 5]), pack_bf16x2(y[8 * z + 6], y[8 * z + 7])};
+    } else {
+      f32x4 *p = reinterpret_cast<f32x4 *>((final ? static_cast<float *>(o) : ws_o) + at);
+#pragma unroll
+      for (int z = 0; z < 4; z++) p[z] = f32x4{y[4 * z], y[4 * z + 1], y[4 * z + 2], y[4 * z + 3]};
+    }
+  }
+  if (!final && g4 == 0) *reinterpret_cast<float2 *>(ws_ml + 2 * prow) = make_float2(m, st.l);
+}
+
+// ===========================================================================
+// Decode.
+//
+// A wave takes a run of steps (32 tokens) of one KV head and up to 16 query
+// heads, tiles straight from memory into the operand layout, kRing steps deep.
+// Two decompositions:
+//   split: the steps of all sequences stand in one row, cut into equal pieces;
+//     every workgroup finds its place itself by a scan over the lengths, so nothing
+//     is planned on the host and a captured call follows the lengths it finds.
+//     A sequence that lies in one piece is stored at once, others leave at most
+//     two partials per piece, which a second launch merges;
+//   seq: one workgroup of 8 waves (4 at head_dim 256) per (sequence, KV head, 16 query
+//     heads), their states merged in LDS; one launch.
+// What bounds it: memory, see the launch rule below.
+// ===========================================================================
+
+constexpr int kSplitSeqs = 4096;   // sequences of one split launch (their scan stands in LDS)
+// Waves of the seq kernel (their states take 512 registers at head_dim 256).
+constexpr int kv8_seq_waves(int D) { return D == 256 ? 4 : 8; }
+constexpr int kKv8Step = 32;       // tokens of a step
+
+struct Kv8Dec {
+  const void *q;
+  void *o;
+  const uint8_t *new_k, *new_v;  // or null
+  float *ws_ml, *ws_o;
+  int32_t max_ctx, nqc;
+  int32_t pieces, min_steps;  // pieces of a split launch, at least min_steps steps each
+  float sl2;
+  int32_t zero_sink;
+};
+
+// What a wave needs of one step, a step per lane.
+struct Kv8Items {
+  int32_t seq, id0, id1, exps, meta;  // exps: ek0 | ek1 | ev0 | ev1, one byte each
+};
+constexpr int kItemValid = 63;      // tokens inside the context, 1..32
+constexpr int kItemBad0 = 1 << 6;   // block 0 (1) has an id outside the pool
+constexpr int kItemBad1 = 1 << 7;
+constexpr int kItemLast = 1 << 8;   // the sequence's last step
+
+// Step j of sequence b, which has ctx tokens and its table at tab0.
+__device__ __forceinline__ Kv8Items kv8_item(const Kv8Args &a, int b, int ctx, int tab0, int j) {
+  Kv8Items it;
+  const int left = ctx - kKv8Step * j;
+  const bool two = left > kPageSize;
+  const int32_t *t = a.ids + (int64_t)tab0 + 2 * j;
+  it.seq = b;
+  it.id0 = t[0];
+  it.id1 = two ? t[1] : it.id0;
+  it.meta = min(left, kKv8Step) | (left <= kKv8Step ? kItemLast : 0);
+  if (it.id0 < 0 || it.id0 >= a.nblocks) {
+    it.meta |= kItemBad0;
+    it.id0 = 0;
+    record_error(a.d_err, MKV_DEVERR_BLOCK);
+  }
+  if (it.id1 < 0 || it.id1 >= a.nblocks) {
+    it.meta |= kItemBad1;
+    it.id1 = 0;
+    record_error(a.d_err, MKV_DEVERR_BLOCK);
+  }
+  it.exps = 0;
+  return it;
+}
+
+template <int D>
+struct Kv8Raw {
+  u32x4 k[2][D / 64], v[2][D / 64];
+};
+
+// The new rows of the n steps whose ids `it` holds, written into their tiles before
+// these are read: a step that is its sequence's last has one. (Put into the loaded
+// registers inside the loop instead, they spilled: 36 registers at head_dim 128.)
+template <int D, bool F32>
+__device__ __forceinline__ void kv8_insert(const Kv8Args &a, const Kv8Dec &dc, int lane, int h, int n,
+                                           const Kv8Items &it) {
+  const int left = it.meta & kItemValid;  // tokens of the last step
+  const bool bad = it.meta & (left > kPageSize ? kItemBad1 : kItemBad0);
+  uint64_t last = __ballot(lane < n && (it.meta & kItemLast) && !bad);
+  if (!last) return;
+  const int64_t stride = (int64_t)a.Hkv * D * Kv8Row<F32>::ES;
+  while (last) {
+    const int k = __builtin_ctzll(last);
+    last &= last - 1;
+    const int nv = __builtin_amdgcn_readlane(it.meta, k) & kItemValid, kb = nv > kPageSize;
+    const int row = nv - 1 - kPageSize * kb;
+    const int id = kb ? __builtin_amdgcn_readlane(it.id1, k) : __builtin_amdgcn_readlane(it.id0, k);
+    const int64_t at = (int64_t)id * a.Hkv + h;
+    const int64_t src = __builtin_amdgcn_readlane(it.seq, k) * stride + (int64_t)h * D * Kv8Row<F32>::ES;
+    kv8_write_k<D, F32>(dc.new_k + src, stride, a.k_tiles + at * 16 * D, a.k_exps + at, lane, row, row + 1);
+    kv8_write_v<D, F32>(dc.new_v + src, stride, a.v_tiles + at * 16 * D, a.v_exps + at, lane, row, row + 1);
+  }
+  // Read again by this wave alone, through the cache that it wrote through.
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+}
+
+// The exponents of a step's tiles (after its new row is written).
+__device__ __forceinline__ void kv8_item_exps(const Kv8Args &a, int h, Kv8Items &it) {
+  const int64_t e0 = (int64_t)it.id0 * a.Hkv + h, e1 = (int64_t)it.id1 * a.Hkv + h;
+  it.exps = (uint8_t)a.k_exps[e0] | (uint8_t)a.k_exps[e1] << 8 | (uint8_t)a.v_exps[e0] << 16 |
+            (uint32_t)(uint8_t)a.v_exps[e1] << 24;
+}
+
+// One step: scores of both blocks, weights, O += P.V.
+template <int D, bool F32>
+__device__ __forceinline__ void kv8_step(float sl2, Kv8Raw<D> &raw, int lane, int exps, int meta,
+                                         const Kv8Q<D, F32> &q, int &E, Kv8State<D> (&st)[1]) {
+  const int g4 = lane >> 4;
+  int ek[2] = {(int8_t)exps, (int8_t)(exps >> 8)}, ev[2] = {(int8_t)(exps >> 16), exps >> 24};
+  const int nv = meta & kItemValid;
+  if (nv <= kPageSize) ev[1] = ev[0];
+  const bool partial = (meta & (kItemBad0 | kItemBad1)) || nv < kKv8Step;
+  if (partial) {
+    // V of tokens past the context (or of a rejected block) counts as zero: bytes
+    // there may be NaN, and 0 * NaN would poison the sum.
+#pragma unroll
+    for (int kb = 0; kb < 2; kb++) {
+      const bool bad = meta & (kb ? kItemBad1 : kItemBad0);
+      const uint32_t m = bad ? 0u : kv8_tok_mask(g4, 0, nv - kPageSize * kb);
+#pragma unroll
+      for (int i = 0; i < D / 64; i++)
+#pragma unroll
+        for (int n = 0; n < 4; n++) raw.v[kb][i][n] &= m;
+    }
+  }
+  int d[2], far[2];
+  kv8_exponents<D, 1>(E, ev[0], ev[1], st, d, far);
+  float t[2][4];
+#pragma unroll
+  for (int kb = 0; kb < 2; kb++) {
+    const float ks = kv8_scale(ek[kb]);
+    f32x4 S = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < D / 64; r++)
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        const bf16x8 k = kv8_k_operand(raw.k[kb][r][2 * half], raw.k[kb][r][2 * half + 1], ks);
+#pragma unroll
+        for (int part = Kv8Q<D, F32>::QP - 1; part >= 0; part--)
+          S = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q.op[part][r][half], S, 0, 0, 0);
+      }
+    // Lane holds S[token 16 kb + 4 g4 + i][query lane % 16].
+#pragma unroll
+    for (int i = 0; i < 4; i++) t[kb][i] = fmaf(S[i], sl2, (float)d[kb]);
+    if (partial) {
+      const bool bad = meta & (kb ? kItemBad1 : kItemBad0);
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (bad || kPageSize * kb + 4 * g4 + i >= nv) t[kb][i] = -INFINITY;
+    }
+  }
+  f16x8 p, p2;
+  kv8_weights<D, F32>(t, d, far, st[0], p, p2);
+#pragma unroll
+  for (int i = 0; i < D / 64; i++)
+#pragma unroll
+    for (int n = 0; n < 4; n++) {
+      const uint2 v0 = kv8_v_half(raw.v[0][i][n]), v1 = kv8_v_half(raw.v[1][i][n]);
+      const f16x8 v = __builtin_bit_cast(f16x8, u32x4{v0.x, v0.y, v1.x, v1.y});
+      if constexpr (F32) st[0].O[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p2, st[0].O[i][n], 0, 0, 0);
+      st[0].O[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p, st[0].O[i][n], 0, 0, 0);
+    }
+}
+
+// The n steps that `it` holds (lane k: step k), carried on from sequence cur_b
+// (-1: none). finish(b) stores a sequence that is done, start(b) loads the next
+// one's q.
+template <int D, bool F32, class Start, class Finish>
+__device__ __forceinline__ void kv8_run(const Kv8Args &a, const Kv8Dec &dc, int lane, int h, int n, Kv8Items it,
+                                        int &cur_b, const Kv8Q<D, F32> &q, int &E,
+                                        Kv8State<D> (&st)[1], Start start, Finish finish) {
+  constexpr int RING = D == 256 ? 2 : 3;
+  if (dc.new_k) kv8_insert<D, F32>(a, dc, lane, h, n, it);
+  if (lane < n) kv8_item_exps(a, h, it);
+  Kv8Raw<D> raw[RING];
+  auto issue = [&](Kv8Raw<D> &w, int k) {
+    const bool live = k < n;
+    const int kk = live ? k : n - 1;
+    // Steps past the end read one line of the last tile again: every stage issues
+    // the same loads, so that the compiler's wait counts cover the one in use.
+    const int off = live ? lane : lane & 7;
+    const int64_t t0 = ((int64_t)__builtin_amdgcn_readlane(it.id0, kk) * a.Hkv + h) * 16 * D;
+    const int64_t t1 = ((int64_t)__builtin_amdgcn_readlane(it.id1, kk) * a.Hkv + h) * 16 * D;
+    const u32x4 *k0 = reinterpret_cast<const u32x4 *>(a.k_tiles + t0) + off;
+    const u32x4 *k1 = reinterpret_cast<const u32x4 *>(a.k_tiles + t1) + off;
+    const u32x4 *v0 = reinterpret_cast<const u32x4 *>(a.v_tiles + t0) + off;
+    const u32x4 *v1 = reinterpret_cast<const u32x4 *>(a.v_tiles + t1) + off;
+#pragma unroll
+    for (int r = 0; r < D / 64; r++) {
+      w.k[0][r] = __builtin_nontemporal_load(k0 + 64 * r);
+      w.k[1][r] = __builtin_nontemporal_load(k1 + 64 * r);
+    }
+#pragma unroll
+    for (int r = 0; r < D / 64; r++) {
+      w.v[0][r] = __builtin_nontemporal_load(v0 + 64 * r);
+      w.v[1][r] = __builtin_nontemporal_load(v1 + 64 * r);
+    }
+  };
+  auto stage = [&](int s, int k) {
+    issue(raw[(s + RING - 1) % RING], k + RING - 1);
+    const int b = __builtin_amdgcn_readlane(it.seq, k);
+    if (b != cur_b) {
+      if (cur_b >= 0) finish(cur_b);
+      st[0].reset();
+      E = kNoExp;
+      cur_b = b;
+      start(b);
+    }
+    kv8_step<D, F32>(dc.sl2, raw[s], lane, __builtin_amdgcn_readlane(it.exps, k),
+                     __builtin_amdgcn_readlane(it.meta, k), q, E, st);
+  };
+#pragma unroll
+  for (int s = 0; s < RING - 1; s++) issue(raw[s], s);
+  int k0 = 0;
+  for (int i = 0; i < n / RING; i++, k0 += RING) {
+#pragma unroll
+    for (int s = 0; s < RING; s++) stage(s, k0 + s);
+  }
+#pragma unroll
+  for (int s = 0; s < RING - 1; s++)
+    if (k0 + s < n) stage(s, k0 + s);
+}
+
+// Steps of sequence b, 0 for one that does not fit or is padding.
+__device__ __forceinline__ int kv8_steps(const Kv8Args &a, int b, int max_ctx, uint32_t &err) {
+  const int ctx = a.ctx[b], tab0 = a.indptr[b];
+  const int64_t tabn = (int64_t)a.indptr[b + 1] - tab0;
+  err = 0;
+  if (ctx == 0) return 0;
+  if (ctx < 0 || ctx > max_ctx) err = MKV_DEVERR_CTX;
+  else if (tab0 < 0 || tabn < ((int64_t)ctx + kPageSize - 1) / kPageSize) err = MKV_DEVERR_TABLE;
+  return err ? 0 : (int)(((int64_t)ctx + kKv8Step - 1) / kKv8Step);
+}
+
+__device__ __forceinline__ int wave_sum_int(int v) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+// Query heads of chunk qc of a group.
+__device__ __forceinline__ int kv8_chunk_heads(int G, int qc) { return min(16, G - 16 * qc); }
+
+template <int D, bool F32>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
+kv8_decode_split_kernel(Kv8Args a, Kv8Dec dc) {
+  extern __shared__ int32_t pre[];  // [B + 1] steps before each sequence
+  __shared__ int32_t wsum[4];
+  const int lane = threadIdx.x & 63, m16 = lane & 15, g4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  {
+    const int per = (a.B + 255) / 256, b0 = min((int)threadIdx.x * per, a.B), b1 = min(b0 + per, a.B);
+    int sum = 0;
+    for (int b = b0; b < b1; b++) {
+      uint32_t err;
+      const int n = kv8_steps(a, b, dc.max_ctx, err);
+      if (err && blockIdx.x == 0) record_error(a.d_err, err);
+      pre[b + 1] = n;  // (own entries only, turned into the scan below)
+      sum += n;
+    }
+    int inc = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int up = __shfl_up(inc, o);
+      if (lane >= o) inc += up;
+    }
+    if (lane == 63) wsum[wave] = inc;
+    __syncthreads();
+    int at = inc - sum;
+    for (int w = 0; w < wave; w++) at += wsum[w];
+    for (int b = b0; b < b1; b++) {
+      at += pre[b + 1];
+      pre[b + 1] = at;
+    }
+    if (threadIdx.x == 0) pre[0] = 0;
+    __syncthreads();
+  }
+  const int total = pre[a.B], heads = a.Hkv * dc.nqc;
+  const int per = max(dc.min_steps, (total + dc.pieces - 1) / dc.pieces);
+  const int wid = (int)blockIdx.x * 4 + wave, p = wid / heads, hc = wid % heads;
+  const int h = hc / dc.nqc, qc = hc % dc.nqc;
+  if (p >= dc.pieces || (int64_t)p * per >= total) return;
+  const int f0 = p * per, f1 = min(total, f0 + per);
+  const int nq = kv8_chunk_heads(a.G, qc), q0 = h * a.G + 16 * qc;
+  Kv8Q<D, F32> q;
+  Kv8State<D> st[1];
+  int E = kNoExp, cur = -1;
+  auto start = [&](int b) { q.load(dc.q, (int64_t)b * a.Hq + q0 + min(m16, nq - 1), g4); };
+  auto finish = [&](int b) {
+    st[0].l += __shfl_xor(st[0].l, 16);
+    st[0].l += __shfl_xor(st[0].l, 32);
+    const int s0 = __builtin_amdgcn_readfirstlane(pre[b]), s1 = __builtin_amdgcn_readfirstlane(pre[b + 1]);
+    if (m16 >= nq) return;
+    // A sequence that starts in this piece and goes on behind it is its second partial.
+    const int64_t slot = 2 * (int64_t)p + (s0 >= f0);
+    kv8_store<D, F32>(st[0], E, g4, s0 >= f0 && s1 <= f1, dc.o, (int64_t)b * a.Hq + q0 + m16, dc.ws_ml, dc.ws_o,
+                      slot * a.Hq + q0 + m16, dc.zero_sink);
+  };
+  for (int c = f0; c < f1; c += 64) {
+    const int n = min(64, f1 - c);
+    Kv8Items it = {0, 0, 0, 0, 0};
+    if (lane < n) {
+      const int f = c + lane;
+      int lo = 0, hi = a.B;  // the last sequence that starts at or before f
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (pre[mid] <= f) lo = mid;
+        else hi = mid;
+      }
+      it = kv8_item(a, lo, a.ctx[lo], a.indptr[lo], f - pre[lo]);
+    }
+    kv8_run<D, F32>(a, dc, lane, h, n, it, cur, q, E, st, start, finish);
+  }
+  finish(cur);
+}
+
+// The merge of a split launch, a workgroup per (query head, sequence); also the
+// zeros of padding sequences.
+template <int D, bool F32>
+__global__ void __launch_bounds__(256) kv8_decode_merge_kernel(Kv8Args a, Kv8Dec dc) {
+  constexpr int NW = 4, DPL = MergeVec<D>::DPL;
+  typedef typename MergeVec<D>::type fvec;
+  __shared__ int32_t sums[2][NW];
+  __shared__ float part[NW][2 + 64 * DPL];
+  const int lane = threadIdx.x & 63, hq = blockIdx.x, b = blockIdx.y;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int before = 0, all = 0;
+  uint32_t err;
+  for (int i = threadIdx.x; i < a.B; i += 256) {
+    const int n = kv8_steps(a, i, dc.max_ctx, err);
+    all += n;
+    before += i < b ? n : 0;
+  }
+  const int mine = kv8_steps(a, b, dc.max_ctx, err);
+  before = wave_sum_int(before);
+  all = wave_sum_int(all);
+  if (lane == 0) sums[0][wave] = before, sums[1][wave] = all;
+  __syncthreads();
+  before = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
+  all = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
+  if (err) return;
+  const int64_t row = (int64_t)b * a.Hq + hq;
+  if (mine == 0) {
+    for (int i = threadIdx.x; i < D; i += 256) {
+      if constexpr (F32) static_cast<float *>(dc.o)[row * D + i] = 0.0f;
+      else static_cast<uint16_t *>(dc.o)[row * D + i] = 0;
+    }
+    return;
+  }
+  const int per = max(dc.min_steps, (all + dc.pieces - 1) / dc.pieces);
+  const int p0 = before / per, p1 = (before + mine - 1) / per;
+  if (p0 == p1) return;  // stored already
+  const int n = p1 - p0 + 1, waves = n <= 16 ? 1 : NW;
+  if (wave >= waves) return;  // (no barrier follows where waves is 1)
+  const int s0 = (int)((int64_t)n * wave / waves), s1 = (int)((int64_t)n * (wave + 1) / waves);
+  // Partial s: piece p0 + s; in the first one the sequence starts.
+  auto at = [&](int s) {
+    const int pc = p0 + s0 + s;
+    return (2 * (int64_t)pc + (before >= pc * per)) * a.Hq + hq;
+  };
+  float M, L;
+  fvec acc;
+  merge_partials_state<D>(
+      lane, s1 - s0, [&](int s) { return dc.ws_ml + 2 * at(s); }, [&](int s) { return dc.ws_o + at(s) * D; }, M, L, acc);
+  if (waves > 1) {
+    if (lane == 0) part[wave][0] = M, part[wave][1] = L;
+#pragma unroll
+    for (int k = 0; k < DPL; k++) part[wave][2 + lane * DPL + k] = acc[k];
+    __syncthreads();
+    if (wave != 0) return;
+    float Mx = -INFINITY, Lx = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; w++) Mx = fmaxf(Mx, part[w][0]);
+    fvec ax = fvec{};
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+      const float f = part[w][0] == -INFINITY ? 0.0f : fast_exp2(part[w][0] - Mx);
+      Lx = fmaf(part[w][1], f, Lx);
+#pragma unroll
+      for (int k = 0; k < DPL; k++) ax[k] = fmaf(part[w][2 + lane * DPL + k], f, ax[k]);
+    }
+    M = Mx, L = Lx, acc = ax;
+  }
+  KArgs ka;
+  ka.o = dc.o;
+  ka.zero_sink = dc.zero_sink;
+  store_merged_row<D, !F32>(ka, lane, M, L, acc, row);
+}
+
+template <int D, bool F32>
+__global__ void __launch_bounds__(64 * kv8_seq_waves(D)) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
+kv8_decode_seq_kernel(Kv8Args a, Kv8Dec dc) {
+  constexpr int NW = kv8_seq_waves(D);
+  __shared__ __attribute__((aligned(16))) float part[NW][16][D];
+  __shared__ float2 ml[NW][16];
+  const int lane = threadIdx.x & 63, m16 = lane & 15, g4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = blockIdx.y, h = blockIdx.x / dc.nqc, qc = blockIdx.x % dc.nqc;
+  const int nq = kv8_chunk_heads(a.G, qc), q0 = h * a.G + 16 * qc;
+  uint32_t err;
+  const int steps = __builtin_amdgcn_readfirstlane(kv8_steps(a, b, dc.max_ctx, err));
+  if (err) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) record_error(a.d_err, err);
+    return;
+  }
+  const int f0 = (int)((int64_t)steps * wave / NW), f1 = (int)((int64_t)steps * (wave + 1) / NW);
+  if (f0 < f1) {
+    const int ctx = a.ctx[b], tab0 = a.indptr[b];
+    Kv8Q<D, F32> q;
+    Kv8State<D> st[1];
+    int E = kNoExp, cur = b;
+    st[0].reset();
+    q.load(dc.q, (int64_t)b * a.Hq + q0 + min(m16, nq - 1), g4);
+    for (int c = f0; c < f1; c += 64) {
+      const int n = min(64, f1 - c);
+      Kv8Items it = {b, 0, 0, 0, 0};
+      if (lane < n) it = kv8_item(a, b, ctx, tab0, c + lane);
+      kv8_run<D, F32>(a, dc, lane, h, n, it, cur, q, E, st, [](int) {}, [](int) {});
+    }
+    st[0].l += __shfl_xor(st[0].l, 16);
+    st[0].l += __shfl_xor(st[0].l, 32);
+    kv8_store<D, true>(st[0], E, g4, false, nullptr, 0, &ml[wave][0].x, &part[wave][0][0], m16, 0);
+  }
+  __syncthreads();
+  const int used = min(NW, steps);
+  for (int i = threadIdx.x; i < nq * (D / 4); i += 64 * NW) {
+    const int r = i / (D / 4), dim = 4 * (i % (D / 4));
+    float M = -INFINITY, L = 0.0f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int w = 0; w < NW; w++)
+      if ((int64_t)steps * w / NW < (int64_t)steps * (w + 1) / NW) M = fmaxf(M, ml[w][r].x);
+    for (int w = 0; w < NW; w++) {
+      if ((int64_t)steps * w / NW == (int64_t)steps * (w + 1) / NW) continue;
+      const float2 s = ml[w][r];
+      const float f = s.x == -INFINITY ? 0.0f : fast_exp2(s.x - M);
+      L = fmaf(s.y, f, L);
+      acc += *reinterpret_cast<const f32x4 *>(&part[w][r][dim]) * f;
+    }
+    // (No keys at all: a padding sequence, a row of zeros.)
+    acc *= used ? final_scale(M, L, dc.zero_sink) : 0.0f;
+    const int64_t at = ((int64_t)b * a.Hq + q0 + r) * D + dim;
+    if constexpr (F32) *reinterpret_cast<f32x4 *>(static_cast<float *>(dc.o) + at) = acc;
+    else
+      *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(dc.o) + at) =
+          make_uint2(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]));
+  }
+}
+
+// ===========================================================================
+// Extend: causal attention of the newest q_len tokens over the whole cache.
+//
+// The rows of one (sequence, KV head) are its (position, query head of the group)
+// pairs in memory order. A workgroup of W waves takes 16 * RT * W of them, RT groups
+// of 16 rows a wave, and streams the keys they see, 32 a step. A tile's bytes are
+// converted once, on the way into LDS (K bf16 with its exponent, V f16), and lie
+// there in operand order: 16 bytes a lane, contiguous, no bank conflicts either way.
+// An operand is read once for RT products: LDS gives 128 bytes a cycle and CU, so at
+// RT = 1 the reads of a step take as long as twice its products, at RT = 2 as long.
+// Loads run kExtRing - 1 steps ahead in registers (16 bytes a lane and 1 KiB of tile);
+// one barrier a step.
+// ===========================================================================
+
+constexpr int kKv8ExtRing = 4;    // steps in registers, the one in use included
+constexpr int kKv8ExtIds = 1024;  // block ids staged in LDS at a time
+
+struct Kv8Ext {
+  const void *q;
+  void *o;
+  float *ws_ml, *ws_o;
+  int32_t max_ctx, tiles, splits;
+  float sl2;
+  int32_t zero_sink;
+};
+
+// Row tile t0 (rows t0 ..) of one sequence and KV head over its share sp of the keys.
+template <int D, bool F32, int RT, int W>
+__device__ __forceinline__ void kv8_extend_tile(const Kv8Args &a, const Kv8Ext &e, const Kv8Seq &s, int h, int t0,
+                                                int sp) {
+  constexpr int NR = D / 64, UNITS = 4 * NR;  // 1 KiB pieces of a step: (K | V, block, r)
+  constexpr int LPL = (UNITS + W - 1) / W;    // of them a wave loads
+  constexpr int HALF = 64 * D;                // bytes of K, or V, of a step in LDS
+  constexpr int R = D == 256 && F32 ? 2 : kKv8ExtRing;  // (four spill there)
+  __shared__ __attribute__((aligned(16))) uint8_t buf[2][2 * HALF];
+  __shared__ int32_t ids_s[kKv8ExtIds];
+  __shared__ int32_t ev_s[2][2];
+  __shared__ int32_t odd_s;
+  const int tid = threadIdx.x, lane = tid & 63, m16 = lane & 15, g4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t rows = (int64_t)s.n * a.G;
+  const int p0 = s.ctx - s.n;
+  const int last = (int)min(rows, (int64_t)t0 + 16 * RT * W) - 1;  // the tile's last row
+  const int qlo_wg = p0 + t0 / a.G, qhi_wg = p0 + last / a.G;
+  const int steps_all = qhi_wg / kKv8Step + 1;
+  const int share = (steps_all + e.splits - 1) / e.splits;
+  const int st0 = min(sp * share, steps_all), st1 = min(st0 + share, steps_all);
+  const int nblk = qhi_wg / kPageSize + 1;
+
+  int qp[RT], qlo[RT], row0[RT];
+  int64_t qrow[RT];
+  Kv8Q<D, F32> q[RT];
+  Kv8State<D> st[RT];
+  int E = kNoExp;
+  int qhi = -1;  // last position of the wave's rows; -1: it has none
+#pragma unroll
+  for (int i = 0; i < RT; i++) {
+    row0[i] = t0 + (wave * RT + i) * 16;
+    const int r = min(row0[i] + m16, (int)rows - 1), pos = r / a.G;
+    qp[i] = p0 + pos;
+    qlo[i] = p0 + min(row0[i], (int)rows - 1) / a.G;
+    qrow[i] = (int64_t)(s.q0 + pos) * a.Hq + h * a.G + (r - pos * a.G);
+    if (row0[i] < rows) qhi = p0 + min(row0[i] + 15, (int)rows - 1) / a.G;
+    q[i].load(e.q, qrow[i], g4);
+    st[i].reset();
+  }
+
+  u32x4 raw[R][LPL];
+  int ex[R][LPL];
+  // Unit u = wave + W * i of a step: kv, block kb, KiB r (wave-uniform).
+  auto issue = [&](u32x4 (&w)[LPL], int (&x)[LPL], int step, int c0, int c1) {
+#pragma unroll
+    for (int i = 0; i < LPL; i++) {
+      const int u = wave + W * i;
+      const int kv = u / (2 * NR), kb = (u / NR) & 1, r = u % NR;
+      // Past the last step, and past the last block of an odd count: the last block once more.
+      const int k = min(min(2 * step + kb, 2 * c1 - 1), nblk - 1);
+      const int32_t id = max(__builtin_amdgcn_readfirstlane(ids_s[k - 2 * c0]), 0);
+      const int64_t at = (int64_t)id * a.Hkv + h;
+      x[i] = 0;
+      w[i] = u32x4{0u, 0u, 0u, 0u};
+      if (UNITS % W == 0 || u < UNITS) {
+        const uint8_t *t = (kv ? a.v_tiles : a.k_tiles) + at * 16 * D + 1024 * r;
+        w[i] = *(reinterpret_cast<const u32x4 *>(t) + (step < c1 ? lane : lane & 7));
+        x[i] = (kv ? a.v_exps : a.k_exps)[at];
+      }
+    }
+  };
+  auto stage = [&](int sl, int step, int c0, int c1, bool bad) {
+    issue(raw[(sl + R - 1) % R], ex[(sl + R - 1) % R], step + R - 1, c0, c1);
+    uint8_t *kt = buf[sl & 1], *vt = kt + HALF;
+    const bool masked = kKv8Step * (step + 1) - 1 > qlo_wg;  // some row of the tile does not see all of it
+#pragma unroll
+    for (int i = 0; i < LPL; i++) {
+      const int u = wave + W * i;
+      if (UNITS % W != 0 && u >= UNITS) break;
+      const int kv = u / (2 * NR), kb = (u / NR) & 1, r = u % NR;
+      u32x4 w = raw[sl][i];
+      const int k = 2 * step + kb;
+      if (!kv) {
+        const float f = kv8_scale(ex[sl][i]);
+        uint8_t *p = kt + ((kb * NR + r) * 2) * 1024 + lane * 16;
+        *reinterpret_cast<bf16x8 *>(p) = kv8_k_operand(w[0], w[1], f);
+        *reinterpret_cast<bf16x8 *>(p + 1024) = kv8_k_operand(w[2], w[3], f);
+        continue;
+      }
+      if (bad && ids_s[min(k, nblk - 1) - 2 * c0] < 0) w = u32x4{0u, 0u, 0u, 0u};
+      if (masked) {
+        // Keys past the context count as zero (their bytes may be NaN, and 0 * NaN is
+        // NaN), and so does a NaN that some row must not see: it is given to the rows
+        // that do when the tile is done.
+        const uint32_t in = kv8_tok_mask(g4, 0, s.ctx - kPageSize * k);
+        const uint32_t later = kv8_tok_mask(g4, qlo_wg + 1 - kPageSize * k, kPageSize);
+        uint32_t odd = 0;
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+          w[n] &= in;
+          const uint32_t one = (((w[n] & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u & later;
+          w[n] &= ~((one << 8) - one);
+          odd |= one;
+        }
+        if (odd) odd_s = 1;
+      }
+#pragma unroll
+      for (int n = 0; n < 4; n++)
+        *reinterpret_cast<uint2 *>(vt + (r * 4 + n) * 1024 + lane * 16 + 8 * kb) = kv8_v_half(w[n]);
+      if (r == 0 && lane == 0) ev_s[sl & 1][kb] = ex[sl][i];
+    }
+    __syncthreads();
+    if (kKv8Step * step > qhi) return;  // nothing that this wave's rows see (or no rows)
+    const int ev0 = __builtin_amdgcn_readfirstlane(ev_s[sl & 1][0]);
+    const int ev1 = __builtin_amdgcn_readfirstlane(ev_s[sl & 1][1]);
+    int d[2], far[2];
+    kv8_exponents<D, RT>(E, ev0, ev1, st, d, far);
+    f32x4 S[RT][2];
+#pragma unroll
+    for (int kb = 0; kb < 2; kb++) {
+#pragma unroll
+      for (int i = 0; i < RT; i++) S[i][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int r = 0; r < NR; r++)
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+          const bf16x8 k = *reinterpret_cast<const bf16x8 *>(kt + ((kb * NR + r) * 2 + half) * 1024 + lane * 16);
+#pragma unroll
+          for (int part = Kv8Q<D, F32>::QP - 1; part >= 0; part--)
+#pragma unroll
+            for (int i = 0; i < RT; i++)
+              S[i][kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[i].op[part][r][half], S[i][kb], 0, 0, 0);
+        }
+    }
+    bool bad0 = false, bad1 = false;
+    if (bad) {
+      bad0 = __builtin_amdgcn_readfirstlane(ids_s[min(2 * step, nblk - 1) - 2 * c0]) < 0;
+      bad1 = __builtin_amdgcn_readfirstlane(ids_s[min(2 * step + 1, nblk - 1) - 2 * c0]) < 0;
+    }
+    f16x8 p[RT], p2[RT];
+#pragma unroll
+    for (int i = 0; i < RT; i++) {
+      float t[2][4];
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) t[kb][c] = fmaf(S[i][kb][c], e.sl2, (float)d[kb]);
+      if (bad || kKv8Step * (step + 1) - 1 > qlo[i]) {
+        const int key = kKv8Step * step + 4 * g4;
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+          for (int c = 0; c < 4; c++)
+            if ((kb ? bad1 : bad0) || key + kPageSize * kb + c > qp[i]) t[kb][c] = -INFINITY;
+      }
+      kv8_weights<D, F32>(t, d, far, st[i], p[i], p2[i]);
+    }
+#pragma unroll
+    for (int r = 0; r < NR; r++)
+#pragma unroll
+      for (int n = 0; n < 4; n++) {
+        const f16x8 v = *reinterpret_cast<const f16x8 *>(vt + (r * 4 + n) * 1024 + lane * 16);
+#pragma unroll
+        for (int i = 0; i < RT; i++) {
+          if constexpr (F32) st[i].O[r][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p2[i], st[i].O[r][n], 0, 0, 0);
+          st[i].O[r][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[i], st[i].O[r][n], 0, 0, 0);
+        }
+      }
+  };
+
+  if (tid == 0) odd_s = 0;
+  for (int c0 = st0; c0 < st1; c0 += kKv8ExtIds / 2) {
+    const int c1 = min(st1, c0 + kKv8ExtIds / 2);
+    __syncthreads();  // the ids and the buffers of the run before are done with
+    int bad = 0;
+    for (int i = tid; i < min(2 * (c1 - c0), nblk - 2 * c0); i += 64 * W) {
+      int32_t id = a.ids[(int64_t)s.tab0 + 2 * c0 + i];
+      if (id < 0 || id >= a.nblocks) {
+        id = -1;
+        bad = 1;
+        record_error(a.d_err, MKV_DEVERR_BLOCK);
+      }
+      ids_s[i] = id;
+    }
+    bad = __builtin_amdgcn_readfirstlane(__syncthreads_or(bad));
+#pragma unroll
+    for (int i = 0; i < R - 1; i++) issue(raw[i], ex[i], c0 + i, c0, c1);
+    int step = c0;
+    for (int it = 0; it < (c1 - c0) / R; it++, step += R) {
+#pragma unroll
+      for (int i = 0; i < R; i++) stage(i, step + i, c0, c1, bad);
+    }
+#pragma unroll
+    for (int i = 0; i < R - 1; i++)
+      if (step + i < c1) stage(i, step + i, c0, c1, bad);
+  }
+  __syncthreads();
+  const bool odd = odd_s;
+#pragma unroll
+  for (int i = 0; i < RT; i++) {
+    st[i].l += __shfl_xor(st[i].l, 16);
+    st[i].l += __shfl_xor(st[i].l, 32);
+    if (row0[i] + m16 < rows)
+      kv8_store<D, F32>(st[i], E, g4, e.splits == 1, e.o, qrow[i], e.ws_ml, e.ws_o, qrow[i] * e.splits + sp,
+                        e.zero_sink);
+  }
+  if (!odd) return;
+  // NaN values of V behind the tile's first position, for the rows that see them.
+  __syncthreads();
+  const int key0 = max(qlo_wg + 1, kKv8Step * st0), key1 = min(s.ctx, kKv8Step * st1);
+  for (int i = tid; i < (last - t0 + 1) * (D / 4); i += 64 * W) {
+    const int r = t0 + i / (D / 4), dim = 4 * (i % (D / 4)), pos = r / a.G;
+    uint32_t nan = 0;
+    for (int key = key0; key < min(key1, p0 + pos + 1); key++) {
+      const int32_t id = a.ids[(int64_t)s.tab0 + key / kPageSize];
+      if (id < 0 || id >= a.nblocks) continue;
+      const int tok = key % kPageSize;
+      const uint8_t *t = a.v_tiles + ((int64_t)id * a.Hkv + h) * 16 * D + dim / 64 * 1024 + tok / 4 * 256 + dim % 64 * 4 + tok % 4;
+#pragma unroll
+      for (int n = 0; n < 4; n++)
+        if ((t[4 * n] & 0x7f) == 0x7f) nan |= 1u << n;
+    }
+    const int64_t qr = (int64_t)(s.q0 + pos) * a.Hq + h * a.G + (r - pos * a.G);
+#pragma unroll
+    for (int n = 0; n < 4; n++) {
+      if (!(nan >> n & 1)) continue;
+      if (e.splits > 1) e.ws_o[(qr * e.splits + sp) * D + dim + n] = __uint_as_float(0x7fc00000u);
+      else if constexpr (F32) static_cast<float *>(e.o)[qr * D + dim + n] = __uint_as_float(0x7fc00000u);
+      else static_cast<uint16_t *>(e.o)[qr * D + dim + n] = 0x7fc0;
+    }
+  }
+}
+
+template <int D, bool F32, int RT, int W>
+__global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2)))
+kv8_extend_kernel(Kv8Args a, Kv8Ext e) {
+  // Tiles with the most keys first, every (KV head, sequence) in turn. Where
+  // their number is a multiple of the 8 XCDs, all tiles of a pair run on one and
+  // share its L2.
+  const int pairs = a.Hkv * a.B;
+  const int64_t L = blockIdx.x;
+  const int pair = (int)(L % pairs), sp = (int)(L / pairs) % e.splits, tr = (int)(L / ((int64_t)pairs * e.splits));
+  const int h = pair % a.Hkv, b = pair / a.Hkv;
+  Kv8Seq s;
+  const uint32_t err = kv8_seq(a, b, e.max_ctx, s);
+  if (err && L < pairs && h == 0 && threadIdx.x == 0) record_error(a.d_err, err);
+  if (err || s.n == 0) return;
+  const int64_t rows = (int64_t)s.n * a.G;
+  const int tile = 16 * RT * W;
+  // (A chunk longer than max_q_len takes further rounds.)
+  const int64_t mine = (rows + tile - 1) / tile;
+  for (int64_t t = mine - 1 - tr; t >= 0; t -= e.tiles) {
+    kv8_extend_tile<D, F32, RT, W>(a, e, s, h, (int)(t * tile), sp);
+    __syncthreads();
+  }
+}
+
+// The merge of split key ranges: a wave per (query head, token of sequence blockIdx.y).
+template <int D, bool F32>
+__global__ void __launch_bounds__(256) kv8_extend_merge_kernel(Kv8Args a, Kv8Ext e) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Kv8Seq s;
+  if (kv8_seq(a, blockIdx.y, e.max_ctx, s) || s.n == 0) return;
+  KArgs ka;
+  ka.o = e.o;
+  ka.zero_sink = e.zero_sink;
+  const int64_t rows = (int64_t)s.n * a.Hq, first = (int64_t)s.q0 * a.Hq;
+  for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < rows; r += (int64_t)gridDim.x * 4) {
+    const int64_t row = first + r;
+    merge_partials<D, !F32>(
+        ka, lane, e.splits, [&](int i) { return e.ws_ml + 2 * (row * e.splits + i); },
+        [&](int i) { return e.ws_o + (row * e.splits + i) * D; }, row);
+  }
+}
+
+// ---- host side ----------------------------------------------------------------------
+
+static uint64_t kv8_ml_bytes(uint64_t rows) { return (rows * 8 + 255) / 256 * 256; }
+
+#define KV8_LAUNCH(KERNEL, GRID, BLOCK, LDS, ...)                                                       \
+  do {                                                                                                  \
+    const bool f32 = g.dtype == MKV_DTYPE_F32;                                                          \
+    switch (g.D) {                                                                                      \
+      case 64: if (f32) hipLaunchKernelGGL((KERNEL<64, true>), GRID, BLOCK, LDS, hs, __VA_ARGS__);       \
+               else hipLaunchKernelGGL((KERNEL<64, false>), GRID, BLOCK, LDS, hs, __VA_ARGS__); break;   \
+      case 128: if (f32) hipLaunchKernelGGL((KERNEL<128, true>), GRID, BLOCK, LDS, hs, __VA_ARGS__);     \
+                else hipLaunchKernelGGL((KERNEL<128, false>), GRID, BLOCK, LDS, hs, __VA_ARGS__); break; \
+      default: if (f32) hipLaunchKernelGGL((KERNEL<256, true>), GRID, BLOCK, LDS, hs, __VA_ARGS__);      \
+               else hipLaunchKernelGGL((KERNEL<256, false>), GRID, BLOCK, LDS, hs, __VA_ARGS__); break;  \
+    }                                                                                                   \
+  } while (0)
+
+static int kv8_check_attn(const Kv8Pool *p, int32_t layer, float scale, uint32_t flags, const void *ws) {
+  int rc = kv8_check_layer(p, layer);
+  if (rc) return rc;
+  if (!(scale > 0.0f) || !std::isfinite(scale))
+    return set_error(MKV_ERR_INVALID_ARGUMENT, "scale must be finite and > 0");
+  if (flags & ~(uint32_t)MKV_ATTN_ZERO_SINK)
+    return set_error(MKV_ERR_INVALID_ARGUMENT, "unknown flags 0x%x", flags);
+  if (!aligned16(ws)) return set_error(MKV_ERR_INVALID_ARGUMENT, "the workspace must be 16-byte aligned");
+  return MKV_OK;
+}
+
+// ---- decode
+
+constexpr int kSplitWavesPerCu = 8;  // waves of a split launch
+constexpr int kSplitMinSteps = 4;    // steps of a piece, at least
+constexpr int kSeqSteps = 6;         // steps a wave of the seq kernel takes, at most
+
+// Up to kSplitSeqs sequences (any number for pieces = 0, the seq kernel).
+static int launch_kv8_decode(const Kv8Pool *p, const Kv8Args &a, Kv8Dec &d, int64_t pieces, hipStream_t hs) {
+  const Geom &g = p->g;
+  const int64_t heads = (int64_t)g.Hkv * d.nqc;
+  if (pieces < 1) {
+    KV8_LAUNCH(kv8_decode_seq_kernel, dim3((unsigned)heads, (unsigned)a.B), dim3(64 * kv8_seq_waves(g.D)), 0, a, d);
+    MKV_CHECK_LAUNCH("kv8_decode_seq_kernel");
+    return MKV_OK;
+  }
+  d.pieces = (int32_t)pieces;
+  KV8_LAUNCH(kv8_decode_split_kernel, dim3((unsigned)((pieces * heads + 3) / 4)), dim3(256), (a.B + 1) * 4, a, d);
+  MKV_CHECK_LAUNCH("kv8_decode_split_kernel");
+  KV8_LAUNCH(kv8_decode_merge_kernel, dim3((unsigned)g.Hq, (unsigned)a.B), dim3(256), 0, a, d);
+  MKV_CHECK_LAUNCH("kv8_decode_merge_kernel");
+  return MKV_OK;
+}
+
+// ---- extend
+
+// Rows and waves of a workgroup: many rows take the wide form (an LDS operand feeds
+// two groups of rows where the registers allow it), few the narrow one.
+struct Kv8ExtForm {
+  const void *fn;
+  int rows, waves;
+};
+static Kv8ExtForm kv8_ext_form(const Geom &g, bool wide) {
+#define KV8_EXT(DD, FF, RR, WW) \
+  Kv8ExtForm { reinterpret_cast<const void *>(&kv8_extend_kernel<DD, FF, RR, WW>), 16 * RR * WW, WW }
+  const bool f32 = g.dtype == MKV_DTYPE_F32;
+  switch (g.D) {
+    case 64:
+      if (f32) return wide ? KV8_EXT(64, true, 2, 4) : KV8_EXT(64, true, 1, 4);
+      return wide ? KV8_EXT(64, false, 2, 4) : KV8_EXT(64, false, 1, 4);
+    case 128:
+      if (f32) return wide ? KV8_EXT(128, true, 1, 8) : KV8_EXT(128, true, 1, 4);
+      return wide ? KV8_EXT(128, false, 2, 8) : KV8_EXT(128, false, 1, 4);
+    default:
+      if (f32) return KV8_EXT(256, true, 1, 8);
+      return wide ? KV8_EXT(256, false, 1, 8) : KV8_EXT(256, false, 1, 4);
+  }
+#undef KV8_EXT
+}
+
+}  // namespace mkv
+
+using namespace mkv;
+
+extern "C" int mkv_kv8_decode_attention(mkv_kv8_pool *pool, int32_t layer, const void *d_k_new, const void *d_v_new,
+                                        const void *d_q, void *d_o, const int32_t *d_block_indptr,
+                                        const int32_t *d_block_ids, const int32_t *d_ctx_lens, int32_t num_seqs,
+                                        int32_t max_ctx_len, float scale, uint32_t flags, void *d_workspace,
+                                        uint64_t workspace_bytes, void *stream) {
+  if (!pool) return set_error(MKV_ERR_INVALID_ARGUMENT, "pool is NULL");
+  Kv8Pool *p = reinterpret_cast<Kv8Pool *>(pool);
+  const Geom &g = p->g;
+  int rc = kv8_check_attn(p, layer, scale, flags, d_workspace);
+  if (rc) return rc;
+  if (num_seqs < 0 || num_seqs > 65535 || max_ctx_len < 0)
+    return set_error(MKV_ERR_INVALID_ARGUMENT, "num_seqs outside [0, 65535], or max_ctx_len < 0");
+  if (!d_k_new != !d_v_new) return set_error(MKV_ERR_INVALID_ARGUMENT, "give both new rows, or neither");
+  if (num_seqs == 0) return MKV_OK;
+  if (!d_q || !d_o || !d_block_indptr || !d_block_ids || !d_ctx_lens)
+    return set_error(MKV_ERR_INVALID_ARGUMENT, "NULL device pointer");
+  if (!aligned16(d_q) || !aligned16(d_o) || !aligned16(d_k_new) || !aligned16(d_v_new))
+    return set_error(MKV_ERR_INVALID_ARGUMENT, "q, o and the new rows must be 16-byte aligned");
+  const uint64_t on = (uint64_t)num_seqs * g.Hq * g.D * g.es, kn = (uint64_t)num_seqs * g.row_bytes;
+  if (overlap(d_o, on, d_q, on) || overlap(d_o, on, d_k_new, kn) || overlap(d_o, on, d_v_new, kn))
+    return set_error(MKV_ERR_INVALID_ARGUMENT, "o overlaps q or the new rows");
+  DeviceGuard guard(p->device);
+  hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
+  const int G = g.Hq / g.Hkv, nqc = (G + 15) / 16;
+  Kv8Args a = kv8_args(p, layer, nullptr, d_block_indptr, d_block_ids, d_ctx_lens, num_seqs, num_seqs);
+  if (nqc > 1 && d_k_new) {
+    // Several waves read a head's tiles: the rows are written before any of them.
+    if ((rc = kv8_append_rows(p, a, d_k_new, d_v_new, max_ctx_len, hs))) return rc;
+    d_k_new = d_v_new = nullptr;
+  }
+  Kv8Dec d{};
+  d.max_ctx = max_ctx_len;
+  d.nqc = nqc;
+  d.min_steps = kSplitMinSteps;
+  d.sl2 = scale * kLog2e;
+  d.zero_sink = (flags & MKV_ATTN_ZERO_SINK) ? 1 : 0;
+  const int64_t most = ((int64_t)max_ctx_len + kKv8Step - 1) / kKv8Step, heads = (int64_t)g.Hkv * nqc;
+  int64_t pieces = 0;
+  Kv8Ws ws;
+  if (most > kv8_seq_waves(g.D) * kSeqSteps) {
+    if ((rc = kv8_ws_begin(p, d_workspace, workspace_bytes, hs, &ws))) return rc;
+    // Two partials a piece; fewer pieces where there are no more steps, or the
+    // workspace holds no more.
+    pieces = std::max<int64_t>(1, (int64_t)p->cus * kSplitWavesPerCu / heads);
+    pieces = std::min(pieces, (most * num_seqs + kSplitMinSteps - 1) / kSplitMinSteps);
+    const uint64_t room = ws.bytes > 256 ? ws.bytes - 256 : 0;
+    pieces = std::min<int64_t>(pieces, (int64_t)(room / ((uint64_t)2 * g.Hq * (8 + 4 * g.D))));
+    d.ws_ml = static_cast<float *>(ws.ptr);
+    d.ws_o = reinterpret_cast<float *>(static_cast<uint8_t *>(ws.ptr) + kv8_ml_bytes((uint64_t)2 * pieces * g.Hq));
+  }
+  const int32_t chunk = pieces < 1 ? num_seqs : kSplitSeqs;
+  for (int32_t b0 = 0; b0 < num_seqs; b0 += chunk) {
+    Kv8Args c = a;
+    c.B = c.tokens = std::min(chunk, num_seqs - b0);
+    c.indptr += b0;
+    c.ctx += b0;
+    const int64_t rows = (int64_t)b0 * g.Hq * g.D * g.es, kv = (int64_t)b0 * g.row_bytes;
+    d.q = static_cast<const uint8_t *>(d_q) + rows;
+    d.o = static_cast<uint8_t *>(d_o) + rows;
+    d.new_k = d_k_new ? static_cast<const uint8_t *>(d_k_new) + kv : nullptr;
+    d.new_v = d_k_new ? static_cast<const uint8_t *>(d_v_new) + kv : nullptr;
+    if ((rc = launch_kv8_decode(p, c, d, pieces, hs))) return rc;
+  }
+  return kv8_ws_end(p, ws, hs);
+}
+
+extern "C" int mkv_kv8_decode_attention_host(mkv_kv8_pool *pool, int32_t layer, const void *d_k_new,
+                                             const void *d_v_new, const void *d_q, void *d_o,
+                                             const int32_t *h_ctx_lens, const uint32_t *h_block_indptr,
+                                             const uint32_t *h_block_ids, int32_t num_seqs, float scale,
+                                             uint32_t flags, void *stream) {
+  if (!pool) return set_error(MKV_ERR_INVALID_ARGUMENT, "pool is NULL");
+  Kv8Pool *p = reinterpret_cast<Kv8Pool *>(pool);
+  int rc = kv8_check_layer(p, layer);
+  if (rc) return rc;
+  if (num_seqs == 0) return MKV_OK;
+  DeviceGuard guard(p->device);
+  hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
+  Kv8Meta m;
+  if ((rc = kv8_stage(p, p->decode_cache, nullptr, h_ctx_lens, h_block_indptr, h_block_ids, nullptr, num_seqs,
+                      d_k_new != nullptr, hs, &m)))
+    return rc;
+  rc = mkv_kv8_decode_attention(pool, layer, d_k_new, d_v_new, d_q, d_o, m.indptr, m.ids, m.ctx, num_seqs, m.max_ctx,
+                                scale, flags, nullptr, 0, stream);
+  const int rr = meta_release(m.slot, hs);
+  return rc ? rc : rr;
+}
+
+extern "C" int mkv_kv8_extend_attention(mkv_kv8_pool *pool, int32_t layer, const void *d_q, void *d_o,
+                                        const int32_t *d_q_indptr, const int32_t *d_block_indptr,
+                                        const int32_t *d_block_ids, const int32_t *d_ctx_lens, int32_t num_seqs,
+                                        int32_t num_tokens, int32_t max_q_len, int32_t max_ctx_len, float scale,
+                                        uint32_t flags, void *d_workspace, uint64_t workspace_bytes, void *stream) {
+  if (!pool) return set_error(MKV_ERR_INVALID_ARGUMENT, "pool is NULL");
+  Kv8Pool *p = reinterpret_cast<Kv8Pool *>(pool);
+  const Geom &g = p->g;
+  int rc = kv8_check_attn(p, layer, scale, flags, d_workspace);
+  if (rc) return rc;
+  if (num_seqs < 0 || num_seqs > 65535 || num_tokens < 0 || max_q_len < 0 || max_ctx_len < 0)
+    return set_error(MKV_ERR_INVALID_ARGUMENT, "num_seqs outside [0, 65535], or negative sizes");
+  if (num_seqs == 0 || num_tokens == 0 || max_q_len == 0) return MKV_OK;
+  if (max_q_len > max_ctx_len)
+    return set_error(MKV_ERR_INVALID_ARGUMENT, "max_q_len %d > max_ctx_len %d", max_q_len, max_ctx_len);
+  if (!d_q || !d_o || !d_q_indptr || !d_block_indptr || !d_block_ids || !d_ctx_lens)
+    return set_error(MKV_ERR_INVALID_ARGUMENT, "NULL device pointer");
+  if (!aligned16(d_q) || !aligned16(d_o)) return set_error(MKV_ERR_INVALID_ARGUMENT, "q and o must be 16-byte aligned");
+  const uint64_t on = (uint64_t)num_tokens * g.Hq * g.D * g.es;
+  if (overlap(d_o, on, d_q, on)) return set_error(MKV_ERR_INVALID_ARGUMENT, "o overlaps q");
+  DeviceGuard guard(p->device);
+  hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
+  Kv8Args a = kv8_args(p, layer, d_q_indptr, d_block_indptr, d_block_ids, d_ctx_lens, num_seqs, num_tokens);
+  Kv8Ext e{};
+  e.q = d_q;
+  e.o = d_o;
+  e.max_ctx = max_ctx_len;
+  e.splits = 1;
+  e.sl2 = scale * kLog2e;
+  e.zero_sink = (flags & MKV_ATTN_ZERO_SINK) ? 1 : 0;
+  const int64_t pairs = (int64_t)g.Hkv * num_seqs, rows = (int64_t)std::min(max_q_len, num_tokens) * a.G;
+  if ((int64_t)num_tokens * a.G > INT32_MAX / 2) return set_error(MKV_ERR_INVALID_ARGUMENT, "too many tokens");
+  Kv8ExtForm form = kv8_ext_form(g, true);
+  if ((rows + form.rows - 1) / form.rows * pairs < p->cus) form = kv8_ext_form(g, false);
+  const int64_t tiles = (rows + form.rows - 1) / form.rows;
+  Kv8Ws ws;
+  // Key ranges are split where the tiles leave CUs without one: into shares of at
+  // least 8 steps, and no more than the workspace holds the partials of.
+  const int64_t steps = ((int64_t)max_ctx_len + kKv8Step - 1) / kKv8Step;
+  const int64_t slots = (int64_t)p->cus * (8 / form.waves);
+  const int64_t want = std::min({slots / std::max<int64_t>(1, tiles * pairs), steps / 8, (int64_t)16});
+  if (want > 1) {
+    if ((rc = kv8_ws_begin(p, d_workspace, workspace_bytes, hs, &ws))) return rc;
+    const uint64_t per = (uint64_t)num_tokens * g.Hq * (8 + 4 * g.D), room = ws.bytes > 256 ? ws.bytes - 256 : 0;
+    e.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(want, (int64_t)(room / per)));
+    e.ws_ml = static_cast<float *>(ws.ptr);
+    e.ws_o = reinterpret_cast<float *>(static_cast<uint8_t *>(ws.ptr) +
+                                       kv8_ml_bytes((uint64_t)num_tokens * g.Hq * e.splits));
+  }
+  const int64_t grid = tiles * pairs * e.splits;
+  if (grid > INT32_MAX || tiles > INT32_MAX) return set_error(MKV_ERR_INVALID_ARGUMENT, "grid too large");
+  e.tiles = (int32_t)tiles;
+  void *args[] = {&a, &e};
+  MKV_CHECK_HIP(hipLaunchKernel(form.fn, dim3((unsigned)grid), dim3(64 * form.waves), args, 0, hs));
+  MKV_CHECK_LAUNCH("kv8_extend_kernel");
+  if (e.splits > 1) {
+    const int64_t wgs = ((int64_t)std::min(max_q_len, num_tokens) * g.Hq + 3) / 4;
+    const dim3 mgrid((unsigned)std::min<int64_t>(wgs, 1 << 20), (unsigned)num_seqs);
+    KV8_LAUNCH(kv8_extend_merge_kernel, mgrid, dim3(256), 0, a, e);
+    MKV_CHECK_LAUNCH("kv8_extend_merge_kernel");
+  }
+  return kv8_ws_end(p, ws, hs);
+}
+
+extern "C" int mkv_kv8_extend_attention_host(mkv_kv8_pool *pool, int32_t layer, const void *d_q, void *d_o,
+                                             const int32_t *h_q_lens, const int32_t *h_ctx_lens,
+                                             const uint32_t *h_block_indptr, const uint32_t *h_block_ids,
+                                             int32_t num_seqs, float scale, uint32_t flags, void *stream) {
+  if (!pool) return set_error(MKV_ERR_INVALID_ARGUMENT, "pool is NULL");
+  Kv8Pool *p = reinterpret_cast<Kv8Pool *>(pool);
+  int rc = kv8_check_layer(p, layer);
+  if (rc) return rc;
+  if (num_seqs == 0) return MKV_OK;
+  if (!h_q_lens) return set_error(MKV_ERR_INVALID_ARGUMENT, "NULL q_lens");
+  DeviceGuard guard(p->device);
+  hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
+  Kv8Meta m;
+  if ((rc = kv8_stage(p, p->extend_cache, h_q_lens, h_ctx_lens, h_block_indptr, h_block_ids, nullptr, num_seqs, false,
+                      hs, &m)))
+    return rc;
+  rc = mkv_kv8_extend_attention(pool, layer, d_q, d_o, m.q_indptr, m.indptr, m.ids, m.ctx, num_seqs, m.tokens, m.max_q,
+                                m.max_ctx, scale, flags, nullptr, 0, stream);
+  const int rr = meta_release(m.slot, hs);
+  return rc ? rc : rr;
+}

@@ -29,6 +29,7 @@ pub const MKV_ATTN_PER_HEAD_LOADS: u32 = 8;
 pub const MKV_ATTN_CACHED_LOADS: u32 = 16;
 pub const MKV_PREP_PLAIN_Q: u32 = 1;
 pub const MKV_PREP_NO_NORM: u32 = 2;
+pub const MKV_PREP_INTERLEAVED: u32 = 4;
 pub const MKV_STATE_NONE: u32 = 0xFFFF_FFFF;
 pub const MKV_LINEAR_HEAD_DECAY: u32 = 1;
 pub const MKV_WIRE_MAGIC: u32 = 0x57564B4D;
@@ -70,6 +71,7 @@ pub struct mkv_wire_header {
 #[repr(C)] pub struct mkv_pool { _p: [u8; 0] }
 #[repr(C)] pub struct mkv_decode_plan { _p: [u8; 0] }
 #[repr(C)] pub struct mkv_state_pool { _p: [u8; 0] }
+#[repr(C)] pub struct mkv_kv8_pool { _p: [u8; 0] }
 pub type hipStream_t = *mut c_void;
 
 extern "C" {
@@ -213,6 +215,58 @@ extern "C" {
                             d_weight: *const f32, eps: f32, num_rows: i32, dim: i32, dtype: i32,
                             d_sum: *mut c_void, d_out: *mut c_void, d_fp8: *mut c_void, d_scales: *mut f32,
                             group: i32, stream: hipStream_t) -> i32;
+
+    pub fn mkv_kv8_required_bytes(desc: *const mkv_pool_desc, out_tile_bytes: *mut u64,
+        out_exponent_bytes: *mut u64) -> i32;
+    pub fn mkv_kv8_pool_create(desc: *const mkv_pool_desc, device: i32, out_pool: *mut *mut mkv_kv8_pool) -> i32;
+    pub fn mkv_kv8_pool_destroy(pool: *mut mkv_kv8_pool) -> i32;
+    pub fn mkv_kv8_pool_get_desc(pool: *const mkv_kv8_pool, out_desc: *mut mkv_pool_desc) -> i32;
+    pub fn mkv_kv8_pool_buffers(pool: *const mkv_kv8_pool, out_tiles: *mut *mut c_void,
+        out_tile_bytes: *mut u64, out_exponents: *mut *mut c_void, out_exponent_bytes: *mut u64) -> i32;
+    pub fn mkv_kv8_pool_check(pool: *mut mkv_kv8_pool, stream: hipStream_t, out_bits: *mut u32) -> i32;
+    pub fn mkv_kv8_append(pool: *mut mkv_kv8_pool, layer: i32, d_k: *const c_void, d_v: *const c_void,
+        d_q_indptr: *const i32, d_block_indptr: *const i32, d_block_ids: *const i32,
+        d_ctx_lens: *const i32, num_seqs: i32, num_tokens: i32, max_q_len: i32, stream: hipStream_t) -> i32;
+    pub fn mkv_kv8_append_host(pool: *mut mkv_kv8_pool, layer: i32, d_k: *const c_void, d_v: *const c_void,
+        h_q_lens: *const i32, h_ctx_lens: *const i32, h_block_indptr: *const u32, h_block_ids: *const u32,
+        num_seqs: i32, stream: hipStream_t) -> i32;
+    pub fn mkv_kv8_qk_norm_rope_append(pool: *mut mkv_kv8_pool, layer: i32, d_q: *const c_void,
+        d_k: *const c_void, d_v: *const c_void, d_q_norm_w: *const f32, d_k_norm_w: *const f32,
+        d_inv_freq: *const f32, rotary_dim: i32, eps: f32, rope_factor: f32, d_positions: *const i32,
+        d_q_indptr: *const i32, d_block_indptr: *const i32, d_block_ids: *const i32,
+        d_ctx_lens: *const i32, num_seqs: i32, num_tokens: i32, max_q_len: i32, d_q_out: *mut c_void,
+        flags: u32, stream: hipStream_t) -> i32;
+    pub fn mkv_kv8_qk_norm_rope_append_host(pool: *mut mkv_kv8_pool, layer: i32, d_q: *const c_void,
+        d_k: *const c_void, d_v: *const c_void, d_q_norm_w: *const f32, d_k_norm_w: *const f32,
+        d_inv_freq: *const f32, rotary_dim: i32, eps: f32, rope_factor: f32, h_positions: *const i32,
+        h_q_lens: *const i32, h_ctx_lens: *const i32, h_block_indptr: *const u32, h_block_ids: *const u32,
+        num_seqs: i32, d_q_out: *mut c_void, flags: u32, stream: hipStream_t) -> i32;
+    pub fn mkv_kv8_gather(pool: *mut mkv_kv8_pool, layer: i32, d_block_indptr: *const i32,
+        d_block_ids: *const i32, d_ctx_lens: *const i32, num_seqs: i32, max_ctx_len: i32,
+        d_out_k: *mut c_void, d_out_v: *mut c_void, out_capacity_tokens: i64, stream: hipStream_t) -> i32;
+    pub fn mkv_kv8_gather_host(pool: *mut mkv_kv8_pool, layer: i32, h_block_indptr: *const u32,
+        h_block_ids: *const u32, h_ctx_lens: *const i32, num_seqs: i32, d_out_k: *mut c_void,
+        d_out_v: *mut c_void, out_capacity_tokens: i64, stream: hipStream_t) -> i32;
+    pub fn mkv_kv8_copy_blocks(pool: *mut mkv_kv8_pool, d_src_blocks: *const i32, d_dst_blocks: *const i32,
+        num_pairs: i32, stream: hipStream_t) -> i32;
+    pub fn mkv_kv8_copy_blocks_host(pool: *mut mkv_kv8_pool, h_src_blocks: *const u32,
+        h_dst_blocks: *const u32, num_pairs: i32, stream: hipStream_t) -> i32;
+    pub fn mkv_kv8_decode_attention(pool: *mut mkv_kv8_pool, layer: i32, d_k_new: *const c_void,
+        d_v_new: *const c_void, d_q: *const c_void, d_o: *mut c_void, d_block_indptr: *const i32,
+        d_block_ids: *const i32, d_ctx_lens: *const i32, num_seqs: i32, max_ctx_len: i32, scale: f32,
+        flags: u32, d_workspace: *mut c_void, workspace_bytes: u64, stream: hipStream_t) -> i32;
+    pub fn mkv_kv8_decode_attention_host(pool: *mut mkv_kv8_pool, layer: i32, d_k_new: *const c_void,
+        d_v_new: *const c_void, d_q: *const c_void, d_o: *mut c_void, h_ctx_lens: *const i32,
+        h_block_indptr: *const u32, h_block_ids: *const u32, num_seqs: i32, scale: f32, flags: u32,
+        stream: hipStream_t) -> i32;
+    pub fn mkv_kv8_workspace_size(pool: *const mkv_kv8_pool, out_bytes: *mut u64) -> i32;
+    pub fn mkv_kv8_extend_attention(pool: *mut mkv_kv8_pool, layer: i32, d_q: *const c_void,
+        d_o: *mut c_void, d_q_indptr: *const i32, d_block_indptr: *const i32, d_block_ids: *const i32,
+        d_ctx_lens: *const i32, num_seqs: i32, num_tokens: i32, max_q_len: i32, max_ctx_len: i32,
+        scale: f32, flags: u32, d_workspace: *mut c_void, workspace_bytes: u64, stream: hipStream_t) -> i32;
+    pub fn mkv_kv8_extend_attention_host(pool: *mut mkv_kv8_pool, layer: i32, d_q: *const c_void,
+        d_o: *mut c_void, h_q_lens: *const i32, h_ctx_lens: *const i32, h_block_indptr: *const u32,
+        h_block_ids: *const u32, num_seqs: i32, scale: f32, flags: u32, stream: hipStream_t) -> i32;
     pub fn mkv_validate_slots(desc: *const mkv_pool_desc, slots: *const i32, n: i32) -> i32;
     pub fn mkv_validate_block_tables(desc: *const mkv_pool_desc, indptr: *const i32, ids: *const i32,
                                      ctx_lens: *const i32, num_seqs: i32, max_ctx_len: i32) -> i32;
