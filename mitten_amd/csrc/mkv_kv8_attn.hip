@@ -19,12 +19,18 @@
 // 32 keys (two blocks) per softmax step: the k-slots of lane group g4 in the PV
 // product are keys 4 g4 .. +3 of the first block, then of the second, where S^T
 // left the scores.
+#include <cfloat>
+
 #include "mkv_kv8.h"
 
 namespace mkv {
 
 constexpr float kBias = 15.0f - kRescaleSlack;
-constexpr int kFarExp = 40;  // a tile 2^-40 below the greatest adds nothing to O that f32 keeps
+constexpr int kMaxRaise = 40;
+// d, at least: what a tile lies below that is taken from its weights after l is
+// summed. (With sums from the matrix unit 2^-d is an f16 number.)
+template <bool SUMS>
+constexpr int kFarExp = SUMS ? 15 : 40;
 constexpr int kNoExp = -1000;
 
 template <int D, bool F32>
@@ -79,17 +85,31 @@ __device__ __forceinline__ uint2 kv8_v_half(uint32_t w) {
 }
 
 // Softmax state of 16 query rows: row of lane % 16. O[i][n][c] is dim 64 i + 16 g4 + 4 c + n.
-template <int D>
+// l: this lane's keys only, or with SUMS all keys, summed by the matrix unit (each of
+// the four is the same sum).
+template <int D, bool SUMS = false>
 struct Kv8State {
+  typedef typename std::conditional<SUMS, f32x4, float>::type sum_t;
   f32x4 O[D / 64][4];
-  float R, l;
+  float R;
+  sum_t l;
+  __device__ __forceinline__ float sum() const {
+    if constexpr (SUMS) return l[0];
+    else return l;
+  }
+  __device__ __forceinline__ void join() {  // l of all keys
+    if constexpr (!SUMS) {
+      l += __shfl_xor(l, 16);
+      l += __shfl_xor(l, 32);
+    }
+  }
   __device__ __forceinline__ void reset() {
 #pragma unroll
     for (int i = 0; i < D / 64; i++)
 #pragma unroll
       for (int n = 0; n < 4; n++) O[i][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-    R = -INFINITY;
-    l = 0.0f;
+    R = -FLT_MAX;  // (finite: no difference of two of them is NaN)
+    l = sum_t{};
   }
   __device__ __forceinline__ void scale_o(float f) {
 #pragma unroll
@@ -100,75 +120,92 @@ struct Kv8State {
   // E grows by de: s + d falls by it, so R follows and O stays; l is relative to
   // R alone. (Steps past 2^40, or an l about to leave f32, move O instead.)
   __device__ __forceinline__ void raise(int de) {
-    const int dc = __ballot(l > 0x1p60f) ? 0 : min(de, kFarExp);
+    const int dc = __ballot(sum() > 0x1p60f) ? 0 : min(de, kMaxRaise);
     R -= (float)dc;
-    l = __builtin_ldexpf(l, dc);
+    l *= __builtin_ldexpf(1.0f, dc);
     if (dc != de) scale_o(__builtin_ldexpf(1.0f, dc - de));
   }
 };
 
-// The weights of two blocks, from t = s + d (hidden keys -inf): state moved on,
-// operands of the PV product in p (and the second part of f32 rows in p2).
-template <int D, bool F32>
-__device__ __forceinline__ void kv8_weights(const float (&t)[2][4], const int (&d)[2], const int (&far)[2],
-                                            Kv8State<D> &st, f16x8 &p, f16x8 &p2) {
-  float top = fmaxf(fmaxf(fmaxf(t[0][0], t[0][1]), fmaxf(t[0][2], t[0][3])),
-                    fmaxf(fmaxf(t[1][0], t[1][1]), fmaxf(t[1][2], t[1][3])));
-  if (__ballot(top > st.R + kRescaleSlack)) {
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    const float R = top > st.R + kRescaleSlack ? top : st.R;
-    const float f = st.R == -INFINITY ? 0.0f : fast_exp2(st.R - R);
-    st.l *= f;
-    st.scale_o(f);
-    st.R = R;
-  }
-  const float base = st.R == -INFINITY ? 0.0f : st.R - kBias;
-#pragma unroll
-  for (int kb = 0; kb < 2; kb++) {
-    float w[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) w[i] = fast_exp2(t[kb][i] - base);
-    st.l += __builtin_ldexpf((w[0] + w[1]) + (w[2] + w[3]), -d[kb]);
-    if (far[kb]) {  // (uniform, rare)
-      const float f = __builtin_ldexpf(1.0f, far[kb]);
-#pragma unroll
-      for (int i = 0; i < 4; i++) w[i] *= f;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const _Float16 h = (_Float16)w[i];
-      p[4 * kb + i] = h;
-      if constexpr (F32) p2[4 * kb + i] = (_Float16)(w[i] - (float)h);
-    }
-  }
-}
-
-// E of a step with tile exponents ev (two blocks): raised where needed; d >= -kFarExp
-// and what is left of ev - E beyond that.
-template <int D, int RT>
-__device__ __forceinline__ void kv8_exponents(int &E, int ev0, int ev1, Kv8State<D> (&st)[RT], int (&d)[2],
-                                              int (&far)[2]) {
-  const int top = max(ev0, ev1);
-  if (top > E) {
-    if (E != kNoExp)
-#pragma unroll
-      for (int i = 0; i < RT; i++) st[i].raise(top - E);
-    E = top;
-  }
-  d[0] = max(ev0 - E, -kFarExp);
-  d[1] = max(ev1 - E, -kFarExp);
+// Exponents of a step's two tiles against E: d >= -kFarExp, and what is left of
+// ev - E beyond that.
+template <bool SUMS>
+__device__ __forceinline__ void kv8_offsets(int E, int ev0, int ev1, int (&d)[2], int (&far)[2]) {
+  d[0] = max(ev0 - E, -kFarExp<SUMS>);
+  d[1] = max(ev1 - E, -kFarExp<SUMS>);
   far[0] = ev0 - E - d[0];
   far[1] = ev1 - E - d[1];
 }
 
+// E for a step with tile exponents ev: raised where needed.
+template <int D, bool SUMS, int RT>
+__device__ __forceinline__ void kv8_raise(int &E, int ev0, int ev1, Kv8State<D, SUMS> (&st)[RT]) {
+  const int top = max(ev0, ev1);
+  if (top <= E) return;
+  if (E != kNoExp)
+#pragma unroll
+    for (int i = 0; i < RT; i++) st[i].raise(top - E);
+  E = top;
+}
+
+// The greatest s + d of this lane's scores S (hidden keys -inf).
+__device__ __forceinline__ float kv8_top(const float (&S)[2][4], float sl2, const int (&d)[2]) {
+  const float a = fmaxf(fmaxf(S[0][0], S[0][1]), fmaxf(S[0][2], S[0][3]));
+  const float b = fmaxf(fmaxf(S[1][0], S[1][1]), fmaxf(S[1][2], S[1][3]));
+  return fmaxf(fmaf(a, sl2, (float)d[0]), fmaf(b, sl2, (float)d[1]));
+}
+
+// R for a step whose greatest s + d in this lane is top.
+template <int D, bool SUMS>
+__device__ __forceinline__ void kv8_rescale(float top, Kv8State<D, SUMS> &st) {
+  top = fmaxf(top, __shfl_xor(top, 16));
+  top = fmaxf(top, __shfl_xor(top, 32));
+  const float R = top > st.R + kRescaleSlack ? top : st.R;
+  const float f = fast_exp2(st.R - R);
+  st.l *= f;
+  st.scale_o(f);
+  st.R = R;
+}
+
+// The weights of two blocks: operands of the PV product in p (and the second part of
+// f32 rows in p2), their sums in l but with SUMS.
+template <int D, bool F32, bool SUMS>
+__device__ __forceinline__ void kv8_weights(const float (&S)[2][4], float sl2, const int (&d)[2],
+                                            Kv8State<D, SUMS> &st, f16x8 &p, f16x8 &p2) {
+#pragma unroll
+  for (int kb = 0; kb < 2; kb++) {
+    const float base = st.R - kBias - (float)d[kb];
+    float w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      w[i] = fast_exp2(fmaf(S[kb][i], sl2, -base));
+      const _Float16 h = (_Float16)w[i];
+      p[4 * kb + i] = h;
+      if constexpr (F32) p2[4 * kb + i] = (_Float16)(w[i] - (float)h);
+    }
+    if constexpr (!SUMS) st.l += __builtin_ldexpf((w[0] + w[1]) + (w[2] + w[3]), -d[kb]);
+  }
+}
+
+// 2^-d of each key, with which the matrix unit sums the weights (SUMS).
+__device__ __forceinline__ f16x8 kv8_ones(const int (&d)[2]) {
+  const _Float16 a = (_Float16)__builtin_ldexpf(1.0f, -d[0]), b = (_Float16)__builtin_ldexpf(1.0f, -d[1]);
+  return f16x8{a, a, a, a, b, b, b, b};
+}
+
+// What a tile lies below E - kFarExp, taken from its weights.
+__device__ __forceinline__ void kv8_far(const int (&far)[2], f16x8 &p) {
+  const _Float16 f0 = (_Float16)__builtin_ldexpf(1.0f, far[0]), f1 = (_Float16)__builtin_ldexpf(1.0f, far[1]);
+  p *= f16x8{f0, f0, f0, f0, f1, f1, f1, f1};
+}
+
 // A finished row: the result, or its partial (m, l, O) for a merge.
-template <int D, bool F32>
-__device__ __forceinline__ void kv8_store(const Kv8State<D> &st, int E, int g4, bool final, void *o, int64_t row,
+template <int D, bool F32, bool SUMS>
+__device__ __forceinline__ void kv8_store(const Kv8State<D, SUMS> &st, int E, int g4, bool final, void *o, int64_t row,
                                           float *ws_ml, float *ws_o, int64_t prow, int32_t zero_sink) {
-  const float m = st.R == -INFINITY ? -INFINITY : st.R - kBias;
+  const float m = st.R - kBias;
   float f = E == kNoExp ? 0.0f : __builtin_ldexpf(1.0f, E);
-  if (final) f *= final_scale(m, st.l, zero_sink);
+  if (final) f *= final_scale(m, st.sum(), zero_sink);
 #pragma unroll
   for (int i = 0; i < D / 64; i++) {
     float y[16];
@@ -189,7 +226,7 @@ __device__ __forceinline__ void kv8_store(const Kv8State<D> &st, int E, int g4, 
       for (int z = 0; z < 4; z++) p[z] = f32x4{y[4 * z], y[4 * z + 1], y[4 * z + 2], y[4 * z + 3]};
     }
   }
-  if (!final && g4 == 0) *reinterpret_cast<float2 *>(ws_ml + 2 * prow) = make_float2(m, st.l);
+  if (!final && g4 == 0) *reinterpret_cast<float2 *>(ws_ml + 2 * prow) = make_float2(m, st.sum());
 }
 
 // ===========================================================================
@@ -318,8 +355,9 @@ __device__ __forceinline__ void kv8_step(float sl2, Kv8Raw<D> &raw, int lane, in
         for (int n = 0; n < 4; n++) raw.v[kb][i][n] &= m;
     }
   }
+  kv8_raise(E, ev[0], ev[1], st);
   int d[2], far[2];
-  kv8_exponents<D, 1>(E, ev[0], ev[1], st, d, far);
+  kv8_offsets<false>(E, ev[0], ev[1], d, far);
   float t[2][4];
 #pragma unroll
   for (int kb = 0; kb < 2; kb++) {
@@ -336,7 +374,7 @@ __device__ __forceinline__ void kv8_step(float sl2, Kv8Raw<D> &raw, int lane, in
       }
     // Lane holds S[token 16 kb + 4 g4 + i][query lane % 16].
 #pragma unroll
-    for (int i = 0; i < 4; i++) t[kb][i] = fmaf(S[i], sl2, (float)d[kb]);
+    for (int i = 0; i < 4; i++) t[kb][i] = S[i];
     if (partial) {
       const bool bad = meta & (kb ? kItemBad1 : kItemBad0);
 #pragma unroll
@@ -344,8 +382,14 @@ __device__ __forceinline__ void kv8_step(float sl2, Kv8Raw<D> &raw, int lane, in
         if (bad || kPageSize * kb + 4 * g4 + i >= nv) t[kb][i] = -INFINITY;
     }
   }
+  const float top = kv8_top(t, sl2, d);
+  if (__ballot(top > st[0].R + kRescaleSlack)) kv8_rescale(top, st[0]);
   f16x8 p, p2;
-  kv8_weights<D, F32>(t, d, far, st[0], p, p2);
+  kv8_weights<D, F32>(t, sl2, d, st[0], p, p2);
+  if (far[0] | far[1]) {  // (uniform, rare)
+    kv8_far(far, p);
+    if constexpr (F32) kv8_far(far, p2);
+  }
 #pragma unroll
   for (int i = 0; i < D / 64; i++)
 #pragma unroll
@@ -482,13 +526,12 @@ kv8_decode_split_kernel(Kv8Args a, Kv8Dec dc) {
   int E = kNoExp, cur = -1;
   auto start = [&](int b) { q.load(dc.q, (int64_t)b * a.Hq + q0 + min(m16, nq - 1), g4); };
   auto finish = [&](int b) {
-    st[0].l += __shfl_xor(st[0].l, 16);
-    st[0].l += __shfl_xor(st[0].l, 32);
+    st[0].join();
     const int s0 = __builtin_amdgcn_readfirstlane(pre[b]), s1 = __builtin_amdgcn_readfirstlane(pre[b + 1]);
     if (m16 >= nq) return;
     // A sequence that starts in this piece and goes on behind it is its second partial.
     const int64_t slot = 2 * (int64_t)p + (s0 >= f0);
-    kv8_store<D, F32>(st[0], E, g4, s0 >= f0 && s1 <= f1, dc.o, (int64_t)b * a.Hq + q0 + m16, dc.ws_ml, dc.ws_o,
+    kv8_store<D, F32, false>(st[0], E, g4, s0 >= f0 && s1 <= f1, dc.o, (int64_t)b * a.Hq + q0 + m16, dc.ws_ml, dc.ws_o,
                       slot * a.Hq + q0 + m16, dc.zero_sink);
   };
   for (int c = f0; c < f1; c += 64) {
@@ -612,9 +655,8 @@ kv8_decode_seq_kernel(Kv8Args a, Kv8Dec dc) {
       if (lane < n) it = kv8_item(a, b, ctx, tab0, c + lane);
       kv8_run<D, F32>(a, dc, lane, h, n, it, cur, q, E, st, [](int) {}, [](int) {});
     }
-    st[0].l += __shfl_xor(st[0].l, 16);
-    st[0].l += __shfl_xor(st[0].l, 32);
-    kv8_store<D, true>(st[0], E, g4, false, nullptr, 0, &ml[wave][0].x, &part[wave][0][0], m16, 0);
+    st[0].join();
+    kv8_store<D, true, false>(st[0], E, g4, false, nullptr, 0, &ml[wave][0].x, &part[wave][0][0], m16, 0);
   }
   __syncthreads();
   const int used = min(NW, steps);
@@ -672,12 +714,12 @@ template <int D, bool F32, int RT, int W>
 __device__ __forceinline__ void kv8_extend_tile(const Kv8Args &a, const Kv8Ext &e, const Kv8Seq &s, int h, int t0,
                                                 int sp) {
   constexpr int NR = D / 64, UNITS = 4 * NR;  // 1 KiB pieces of a step: (K | V, block, r)
-  constexpr int LPL = (UNITS + W - 1) / W;    // of them a wave loads
+  constexpr int LPL = UNITS / W;              // of them a wave loads
+  static_assert(UNITS % W == 0, "every wave loads the same number of pieces");
   constexpr int HALF = 64 * D;                // bytes of K, or V, of a step in LDS
-  constexpr int R = D == 256 && F32 ? 2 : kKv8ExtRing;  // (four spill there)
-  __shared__ __attribute__((aligned(16))) uint8_t buf[2][2 * HALF];
-  __shared__ int32_t ids_s[kKv8ExtIds];
-  __shared__ int32_t ev_s[2][2];
+  constexpr int R = kKv8ExtRing;
+  __shared__ __attribute__((aligned(16))) uint8_t kbuf[2][HALF], vbuf[2][HALF];
+  __shared__ int32_t ids_s[kKv8ExtIds], exps_s[kKv8ExtIds];  // exps: ek, then ev, a byte each
   __shared__ int32_t odd_s;
   const int tid = threadIdx.x, lane = tid & 63, m16 = lane & 15, g4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -693,7 +735,7 @@ __device__ __forceinline__ void kv8_extend_tile(const Kv8Args &a, const Kv8Ext &
   int qp[RT], qlo[RT], row0[RT];
   int64_t qrow[RT];
   Kv8Q<D, F32> q[RT];
-  Kv8State<D> st[RT];
+  Kv8State<D, !F32> st[RT];
   int E = kNoExp;
   int qhi = -1;  // last position of the wave's rows; -1: it has none
 #pragma unroll
@@ -709,131 +751,100 @@ __device__ __forceinline__ void kv8_extend_tile(const Kv8Args &a, const Kv8Ext &
   }
 
   u32x4 raw[R][LPL];
-  int ex[R][LPL];
-  // Unit u = wave + W * i of a step: kv, block kb, KiB r (wave-uniform).
-  auto issue = [&](u32x4 (&w)[LPL], int (&x)[LPL], int step, int c0, int c1) {
-#pragma unroll
-    for (int i = 0; i < LPL; i++) {
-      const int u = wave + W * i;
-      const int kv = u / (2 * NR), kb = (u / NR) & 1, r = u % NR;
-      // Past the last step, and past the last block of an odd count: the last block once more.
-      const int k = min(min(2 * step + kb, 2 * c1 - 1), nblk - 1);
-      const int32_t id = max(__builtin_amdgcn_readfirstlane(ids_s[k - 2 * c0]), 0);
-      const int64_t at = (int64_t)id * a.Hkv + h;
-      x[i] = 0;
-      w[i] = u32x4{0u, 0u, 0u, 0u};
-      if (UNITS % W == 0 || u < UNITS) {
-        const uint8_t *t = (kv ? a.v_tiles : a.k_tiles) + at * 16 * D + 1024 * r;
-        w[i] = *(reinterpret_cast<const u32x4 *>(t) + (step < c1 ? lane : lane & 7));
-        x[i] = (kv ? a.v_exps : a.k_exps)[at];
-      }
-    }
+  // Piece u = wave + W * i of a step: K or V (known at compile time but at head_dim 64),
+  // block kb, KiB r; all of it wave-uniform.
+  auto is_v = [&](int i) { return (2 * NR) % W == 0 ? (W * i) / (2 * NR) : (wave + W * i) / (2 * NR); };
+  auto load = [&](int i, int32_t id, bool live) {
+    const int r = (wave + W * i) % NR;
+    const uint8_t *t = (is_v(i) ? a.v_tiles : a.k_tiles) + ((int64_t)max(id, 0) * a.Hkv + h) * 16 * D + 1024 * r;
+    // (A step past the end reads one line of the last block again.)
+    return *(reinterpret_cast<const u32x4 *>(t) + (live ? lane : lane & 7));
   };
-  auto stage = [&](int sl, int step, int c0, int c1, bool bad) {
-    issue(raw[(sl + R - 1) % R], ex[(sl + R - 1) % R], step + R - 1, c0, c1);
-    uint8_t *kt = buf[sl & 1], *vt = kt + HALF;
-    const bool masked = kKv8Step * (step + 1) - 1 > qlo_wg;  // some row of the tile does not see all of it
+  // A piece, converted, into buffer y: K times 2^ek, V as it is.
+  auto put_k = [&](u32x4 w, int i, int y, int ek) {
+    const int u = wave + W * i, kb = (u / NR) & 1, r = u % NR;
+    const float f = kv8_scale(ek);
+    uint8_t *p = kbuf[y] + ((kb * NR + r) * 2) * 1024 + lane * 16;
+    *reinterpret_cast<bf16x8 *>(p) = kv8_k_operand(w[0], w[1], f);
+    *reinterpret_cast<bf16x8 *>(p + 1024) = kv8_k_operand(w[2], w[3], f);
+  };
+  auto put_v = [&](u32x4 w, int i, int y) {
+    const int u = wave + W * i, kb = (u / NR) & 1, r = u % NR;
 #pragma unroll
-    for (int i = 0; i < LPL; i++) {
-      const int u = wave + W * i;
-      if (UNITS % W != 0 && u >= UNITS) break;
-      const int kv = u / (2 * NR), kb = (u / NR) & 1, r = u % NR;
-      u32x4 w = raw[sl][i];
-      const int k = 2 * step + kb;
-      if (!kv) {
-        const float f = kv8_scale(ex[sl][i]);
-        uint8_t *p = kt + ((kb * NR + r) * 2) * 1024 + lane * 16;
-        *reinterpret_cast<bf16x8 *>(p) = kv8_k_operand(w[0], w[1], f);
-        *reinterpret_cast<bf16x8 *>(p + 1024) = kv8_k_operand(w[2], w[3], f);
-        continue;
-      }
-      if (bad && ids_s[min(k, nblk - 1) - 2 * c0] < 0) w = u32x4{0u, 0u, 0u, 0u};
-      if (masked) {
-        // Keys past the context count as zero (their bytes may be NaN, and 0 * NaN is
-        // NaN), and so does a NaN that some row must not see: it is given to the rows
-        // that do when the tile is done.
-        const uint32_t in = kv8_tok_mask(g4, 0, s.ctx - kPageSize * k);
-        const uint32_t later = kv8_tok_mask(g4, qlo_wg + 1 - kPageSize * k, kPageSize);
-        uint32_t odd = 0;
+    for (int n = 0; n < 4; n++)
+      *reinterpret_cast<uint2 *>(vbuf[y] + (r * 4 + n) * 1024 + lane * 16 + 8 * kb) = kv8_v_half(w[n]);
+  };
+  auto read_k = [&](bf16x8 (&k)[2][2], int y, int r) {
 #pragma unroll
-        for (int n = 0; n < 4; n++) {
-          w[n] &= in;
-          const uint32_t one = (((w[n] & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u & later;
-          w[n] &= ~((one << 8) - one);
-          odd |= one;
-        }
-        if (odd) odd_s = 1;
-      }
-#pragma unroll
-      for (int n = 0; n < 4; n++)
-        *reinterpret_cast<uint2 *>(vt + (r * 4 + n) * 1024 + lane * 16 + 8 * kb) = kv8_v_half(w[n]);
-      if (r == 0 && lane == 0) ev_s[sl & 1][kb] = ex[sl][i];
-    }
-    __syncthreads();
-    if (kKv8Step * step > qhi) return;  // nothing that this wave's rows see (or no rows)
-    const int ev0 = __builtin_amdgcn_readfirstlane(ev_s[sl & 1][0]);
-    const int ev1 = __builtin_amdgcn_readfirstlane(ev_s[sl & 1][1]);
-    int d[2], far[2];
-    kv8_exponents<D, RT>(E, ev0, ev1, st, d, far);
-    f32x4 S[RT][2];
-#pragma unroll
-    for (int kb = 0; kb < 2; kb++) {
-#pragma unroll
-      for (int i = 0; i < RT; i++) S[i][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int r = 0; r < NR; r++)
-#pragma unroll
-        for (int half = 0; half < 2; half++) {
-          const bf16x8 k = *reinterpret_cast<const bf16x8 *>(kt + ((kb * NR + r) * 2 + half) * 1024 + lane * 16);
-#pragma unroll
-          for (int part = Kv8Q<D, F32>::QP - 1; part >= 0; part--)
-#pragma unroll
-            for (int i = 0; i < RT; i++)
-              S[i][kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[i].op[part][r][half], S[i][kb], 0, 0, 0);
-        }
-    }
-    bool bad0 = false, bad1 = false;
-    if (bad) {
-      bad0 = __builtin_amdgcn_readfirstlane(ids_s[min(2 * step, nblk - 1) - 2 * c0]) < 0;
-      bad1 = __builtin_amdgcn_readfirstlane(ids_s[min(2 * step + 1, nblk - 1) - 2 * c0]) < 0;
-    }
-    f16x8 p[RT], p2[RT];
-#pragma unroll
-    for (int i = 0; i < RT; i++) {
-      float t[2][4];
+    for (int half = 0; half < 2; half++)
 #pragma unroll
       for (int kb = 0; kb < 2; kb++)
+        k[half][kb] = *reinterpret_cast<const bf16x8 *>(kbuf[y] + ((kb * NR + r) * 2 + half) * 1024 + lane * 16);
+  };
+  auto dot_k = [&](f32x4 (&S)[RT][2], const bf16x8 (&k)[2][2], int r) {
 #pragma unroll
-        for (int c = 0; c < 4; c++) t[kb][c] = fmaf(S[i][kb][c], e.sl2, (float)d[kb]);
-      if (bad || kKv8Step * (step + 1) - 1 > qlo[i]) {
-        const int key = kKv8Step * step + 4 * g4;
+    for (int half = 0; half < 2; half++)
+#pragma unroll
+      for (int part = Kv8Q<D, F32>::QP - 1; part >= 0; part--)
 #pragma unroll
         for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-          for (int c = 0; c < 4; c++)
-            if ((kb ? bad1 : bad0) || key + kPageSize * kb + c > qp[i]) t[kb][c] = -INFINITY;
-      }
-      kv8_weights<D, F32>(t, d, far, st[i], p[i], p2[i]);
-    }
+          for (int x = 0; x < RT; x++)
+            S[x][kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[half][kb], q[x].op[part][r][half],
+                                                               r == 0 && half == 0 && part == Kv8Q<D, F32>::QP - 1
+                                                                   ? f32x4{0.f, 0.f, 0.f, 0.f} : S[x][kb], 0, 0, 0);
+  };
+  auto read_v = [&](f16x8 (&v)[4], int y, int r) {
 #pragma unroll
-    for (int r = 0; r < NR; r++)
+    for (int n = 0; n < 4; n++) v[n] = *reinterpret_cast<const f16x8 *>(vbuf[y] + (r * 4 + n) * 1024 + lane * 16);
+  };
+  auto add_v = [&](const f16x8 (&v)[4], const f16x8 (&p)[RT], const f16x8 (&p2)[RT], int r) {
 #pragma unroll
-      for (int n = 0; n < 4; n++) {
-        const f16x8 v = *reinterpret_cast<const f16x8 *>(vt + (r * 4 + n) * 1024 + lane * 16);
+    for (int n = 0; n < 4; n++)
 #pragma unroll
-        for (int i = 0; i < RT; i++) {
-          if constexpr (F32) st[i].O[r][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p2[i], st[i].O[r][n], 0, 0, 0);
-          st[i].O[r][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[i], st[i].O[r][n], 0, 0, 0);
-        }
+      for (int x = 0; x < RT; x++) {
+        f32x4 &o = st[x].O[r][n];
+        if constexpr (F32) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[n], p2[x], o, 0, 0, 0);
+        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[n], p[x], o, 0, 0, 0);
       }
   };
+  auto sum_p = [&](const f16x8 (&p)[RT], const int (&d)[2]) {
+    if constexpr (!F32) {
+      const f16x8 ones = kv8_ones(d);
+#pragma unroll
+      for (int x = 0; x < RT; x++) st[x].l = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[x], st[x].l, 0, 0, 0);
+    }
+  };
+  // E and R for the scores S of a step with V exponents ev0, ev1.
+  auto settle = [&](const f32x4 (&S)[RT][2], int ev0, int ev1, float (&t)[RT][2][4], int (&d)[2], int (&far)[2],
+                    auto mask) {
+    kv8_raise(E, ev0, ev1, st);
+    kv8_offsets<!F32>(E, ev0, ev1, d, far);
+    float top[RT];
+    bool move = false;
+#pragma unroll
+    for (int x = 0; x < RT; x++) {
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) t[x][kb][c] = S[x][kb][c];
+      mask(t[x], x);
+      top[x] = kv8_top(t[x], e.sl2, d);
+      move |= top[x] > st[x].R + kRescaleSlack;
+    }
+    if (__ballot(move))
+#pragma unroll
+      for (int x = 0; x < RT; x++) kv8_rescale(top[x], st[x]);
+  };
 
+  f32x4 S[2][RT][2];
   if (tid == 0) odd_s = 0;
   for (int c0 = st0; c0 < st1; c0 += kKv8ExtIds / 2) {
     const int c1 = min(st1, c0 + kKv8ExtIds / 2);
-    __syncthreads();  // the ids and the buffers of the run before are done with
+    const int nid = min(2 * c1, nblk) - 2 * c0;  // ids of this run; behind them the last one counts
+    __syncthreads();
     int bad = 0;
-    for (int i = tid; i < min(2 * (c1 - c0), nblk - 2 * c0); i += 64 * W) {
+    for (int i = tid; i < nid; i += 64 * W) {
       int32_t id = a.ids[(int64_t)s.tab0 + 2 * c0 + i];
       if (id < 0 || id >= a.nblocks) {
         id = -1;
@@ -841,27 +852,190 @@ __device__ __forceinline__ void kv8_extend_tile(const Kv8Args &a, const Kv8Ext &
         record_error(a.d_err, MKV_DEVERR_BLOCK);
       }
       ids_s[i] = id;
+      const int64_t at = (int64_t)max(id, 0) * a.Hkv + h;
+      exps_s[i] = (uint8_t)a.k_exps[at] | a.v_exps[at] * 256;
     }
     bad = __builtin_amdgcn_readfirstlane(__syncthreads_or(bad));
+    auto block = [&](int step, int kb) { return min(2 * (step - c0) + kb, nid - 1); };
+    auto kb_of = [&](int i) { return ((wave + W * i) / NR) & 1; };
+    auto issue = [&](u32x4 (&w)[LPL], int step) {
 #pragma unroll
-    for (int i = 0; i < R - 1; i++) issue(raw[i], ex[i], c0 + i, c0, c1);
+      for (int i = 0; i < LPL; i++)
+        w[i] = load(i, __builtin_amdgcn_readfirstlane(ids_s[block(step, kb_of(i))]), step < c1);
+    };
+    // Pieces of K of step ks and of V of step vs, with what has to be left out.
+    auto put = [&](const u32x4 (&kw)[LPL], int ks, const u32x4 (&vw)[LPL], int vs) {
+#pragma unroll
+      for (int i = 0; i < LPL; i++) {
+        if (!is_v(i)) {
+          if (ks < c1) put_k(kw[i], i, ks - c0 & 1, (int8_t)exps_s[block(ks, kb_of(i))]);
+          continue;
+        }
+        if (vs >= c1) continue;
+        u32x4 w = vw[i];
+        const int k = 2 * vs + kb_of(i);
+        if (bad && ids_s[block(vs, kb_of(i))] < 0) w = u32x4{0u, 0u, 0u, 0u};
+        if (kKv8Step * (vs + 1) - 1 > qlo_wg) {  // some row of the tile does not see all of it
+          // Keys past the context count as zero (their bytes may be NaN, and 0 * NaN is
+          // NaN), and so does a NaN that some row must not see: it is given to the rows
+          // that do when the tile is done.
+          const uint32_t in = kv8_tok_mask(g4, 0, s.ctx - kPageSize * k);
+          const uint32_t later = kv8_tok_mask(g4, qlo_wg + 1 - kPageSize * k, kPageSize);
+          uint32_t odd = 0;
+#pragma unroll
+          for (int n = 0; n < 4; n++) {
+            w[n] &= in;
+            const uint32_t one = (((w[n] & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u & later;
+            w[n] &= ~((one << 8) - one);
+            odd |= one;
+          }
+          if (odd) odd_s = 1;
+        }
+        put_v(w, i, vs - c0 & 1);
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < R - 1; i++) issue(raw[i], c0 + i);
+    put(raw[0], c0, raw[0], c0);
+    put(raw[1], c0 + 1, raw[1], c1);
+    __syncthreads();
+    auto scores = [&](f32x4 (&N)[RT][2], int y) {
+#pragma unroll
+      for (int r = 0; r < NR; r++) {
+        bf16x8 k[2][2];
+        read_k(k, y, r);
+        dot_k(N, k, r);
+      }
+    };
+    if (kKv8Step * c0 <= qhi) scores(S[0], 0);
+    __syncthreads();
+
+    // Steps whose keys, and those of the two after, every row of the workgroup sees,
+    // R at a time. A step's turn: its scores are in S, its V in buffer y. The scores of
+    // the next step go into N beside its weights, so that the matrix and the vector units
+    // both have work, and its products with V beside the conversion of later tiles: K
+    // of the step after the next and V of the next, into the buffers that every wave
+    // left at the last barrier. Ids and exponents of a round stand in lanes.
+    const int full = bad ? c0 : min(c1, (qlo_wg + 1) / kKv8Step) - 2;
     int step = c0;
-    for (int it = 0; it < (c1 - c0) / R; it++, step += R) {
+    int idw = ids_s[min(lane, nid - 1)], exw = exps_s[min(lane, nid - 1)];
+    for (int it = 0, n = max(full - c0, 0) / R; it < n; it++, step += R) {
+      const int at = min(2 * (step + R - c0) + lane, nid - 1);
+      const int idn = ids_s[at], exn = exps_s[at];
 #pragma unroll
-      for (int i = 0; i < R; i++) stage(i, step + i, c0, c1, bad);
+      for (int i = 0; i < R; i++) {
+        constexpr auto lane_of = [](int x, int kb) { return 2 * x + kb; };
+        const int y = i & 1;
+        f32x4(&cur)[RT][2] = S[y];
+        f32x4(&nxt)[RT][2] = S[y ^ 1];
+        u32x4(&in)[LPL] = raw[(i + R - 1) % R];
+#pragma unroll
+        for (int l = 0; l < LPL; l++) {
+          // (Blocks past the last step are the last block again: step < c1 - 2 here.)
+          const int32_t id = __builtin_amdgcn_readlane(idw, lane_of(i + R - 1, 0) + kb_of(l));
+          in[l] = load(l, id, step + i + R - 1 < c1);
+        }
+        if (qhi >= 0) {
+          bf16x8 k[2][2][2];
+          read_k(k[0], y ^ 1, 0);
+          float t[RT][2][4];
+          int d[2], far[2];
+          settle(cur, __builtin_amdgcn_readlane(exw, lane_of(i, 0)) >> 8, __builtin_amdgcn_readlane(exw, lane_of(i, 1)) >> 8,
+                 t, d, far, [](float (&)[2][4], int) {});
+          f16x8 p[RT], p2[RT], v[2][4];
+#pragma unroll
+          for (int r = 0; r < NR; r++) {
+            if (r + 1 < NR) read_k(k[(r + 1) & 1], y ^ 1, r + 1);
+            dot_k(nxt, k[r & 1], r);
+          }
+          read_v(v[0], y, 0);
+#pragma unroll
+          for (int x = 0; x < RT; x++) kv8_weights<D, F32, !F32>(t[x], e.sl2, d, st[x], p[x], p2[x]);
+          // One product, then some of the weights' instructions, in turn.
+#pragma unroll
+          for (int g = 0; g < 4 * NR * RT * Kv8Q<D, F32>::QP; g++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, F32 ? 2 : 4, 0);
+          }
+          if (far[0] | far[1])  // (uniform, rare)
+#pragma unroll
+            for (int x = 0; x < RT; x++) {
+              kv8_far(far, p[x]);
+              if constexpr (F32) kv8_far(far, p2[x]);
+            }
+          sum_p(p, d);
+#pragma unroll
+          for (int r = 0; r < NR; r++) {
+            if (r + 1 < NR) read_v(v[(r + 1) & 1], y, r + 1);
+            add_v(v[r & 1], p, p2, r);
+          }
+        }
+#pragma unroll
+        for (int l = 0; l < LPL; l++) {
+          if (!is_v(l)) {
+            const int ek = (int8_t)__builtin_amdgcn_readlane(exw, lane_of(i + 2, 0) + kb_of(l));
+            put_k(raw[(i + 2) % R][l], l, y, ek);
+          } else {
+            put_v(raw[(i + 1) % R][l], l, y ^ 1);
+          }
+        }
+        __syncthreads();
+      }
+      idw = idn;
+      exw = exn;
     }
+    // The rest a step at a time, masked, the ring moved down, the next scores in the
+    // place of these.
+#pragma unroll 1
+    for (; step < c1; step++) {
+      const int y = step - c0 & 1;
+      if (kKv8Step * step <= qhi) {
+        float t[RT][2][4];
+        int d[2], far[2];
+        settle(S[0], __builtin_amdgcn_readfirstlane(exps_s[block(step, 0)]) >> 8,
+               __builtin_amdgcn_readfirstlane(exps_s[block(step, 1)]) >> 8, t, d, far, [&](float (&u)[2][4], int x) {
+                 if (!bad && kKv8Step * (step + 1) - 1 <= qlo[x]) return;
+                 const int key = kKv8Step * step + 4 * g4;
 #pragma unroll
-    for (int i = 0; i < R - 1; i++)
-      if (step + i < c1) stage(i, step + i, c0, c1, bad);
+                 for (int kb = 0; kb < 2; kb++) {
+                   const bool none = bad && ids_s[block(step, kb)] < 0;
+#pragma unroll
+                   for (int c = 0; c < 4; c++)
+                     if (none || key + kPageSize * kb + c > qp[x]) u[kb][c] = -INFINITY;
+                 }
+               });
+        f16x8 p[RT], p2[RT];
+#pragma unroll
+        for (int x = 0; x < RT; x++) {
+          kv8_weights<D, F32, !F32>(t[x], e.sl2, d, st[x], p[x], p2[x]);
+          if (far[0] | far[1]) {
+            kv8_far(far, p[x]);
+            if constexpr (F32) kv8_far(far, p2[x]);
+          }
+        }
+        scores(S[0], y ^ 1);
+        sum_p(p, d);
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+          f16x8 v[4];
+          read_v(v, y, r);
+          add_v(v, p, p2, r);
+        }
+      }
+      put(raw[2], step + 2, raw[1], step + 1);
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < LPL; i++) raw[1][i] = raw[2][i];
+      issue(raw[2], step + 3);
+    }
   }
   __syncthreads();
   const bool odd = odd_s;
 #pragma unroll
   for (int i = 0; i < RT; i++) {
-    st[i].l += __shfl_xor(st[i].l, 16);
-    st[i].l += __shfl_xor(st[i].l, 32);
+    st[i].join();
     if (row0[i] + m16 < rows)
-      kv8_store<D, F32>(st[i], E, g4, e.splits == 1, e.o, qrow[i], e.ws_ml, e.ws_o, qrow[i] * e.splits + sp,
+      kv8_store<D, F32, !F32>(st[i], E, g4, e.splits == 1, e.o, qrow[i], e.ws_ml, e.ws_o, qrow[i] * e.splits + sp,
                         e.zero_sink);
   }
   if (!odd) return;
@@ -892,7 +1066,7 @@ __device__ __forceinline__ void kv8_extend_tile(const Kv8Args &a, const Kv8Ext &
 }
 
 template <int D, bool F32, int RT, int W>
-__global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2)))
+__global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 256 && F32 ? 1 : 2, D == 256 && F32 ? 1 : 2)))
 kv8_extend_kernel(Kv8Args a, Kv8Ext e) {
   // Tiles with the most keys first, every (KV head, sequence) in turn. Where
   // their number is a multiple of the 8 XCDs, all tiles of a pair run on one and
@@ -1003,9 +1177,9 @@ static Kv8ExtForm kv8_ext_form(const Geom &g, bool wide) {
       return wide ? KV8_EXT(64, false, 2, 4) : KV8_EXT(64, false, 1, 4);
     case 128:
       if (f32) return wide ? KV8_EXT(128, true, 1, 8) : KV8_EXT(128, true, 1, 4);
-      return wide ? KV8_EXT(128, false, 2, 8) : KV8_EXT(128, false, 1, 4);
+      return wide ? KV8_EXT(128, false, 2, 4) : KV8_EXT(128, false, 1, 4);
     default:
-      if (f32) return KV8_EXT(256, true, 1, 8);
+      if (f32) return KV8_EXT(256, true, 1, 4);
       return wide ? KV8_EXT(256, false, 1, 8) : KV8_EXT(256, false, 1, 4);
   }
 #undef KV8_EXT
