@@ -182,8 +182,7 @@ struct Kv8Row<true> {
   static __device__ __forceinline__ void store(uint8_t *p, const float (&x)[N]) {
 #pragma unroll
     for (int i = 0; i < N / 4; i++)
-      __builtin_nontemporal_store(f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]},
-                                  reinterpret_cast<f32x4 *>(p + 16 * i));
+      *reinterpret_cast<f32x4 *>(p + 16 * i) = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
   }
 };
 template <>
@@ -206,15 +205,13 @@ struct Kv8Row<false> {
   template <int N>
   static __device__ __forceinline__ void store(uint8_t *p, const float (&x)[N]) {
     if constexpr (N == 4) {
-      typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-      __builtin_nontemporal_store(u32x2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])},
-                                  reinterpret_cast<u32x2 *>(p));
+      *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
     } else {
 #pragma unroll
       for (int i = 0; i < N / 8; i++)
-        __builtin_nontemporal_store(u32x4{pack_bf16x2(x[8 * i], x[8 * i + 1]), pack_bf16x2(x[8 * i + 2], x[8 * i + 3]),
-                                          pack_bf16x2(x[8 * i + 4], x[8 * i + 5]), pack_bf16x2(x[8 * i + 6], x[8 * i + 7])},
-                                    reinterpret_cast<u32x4 *>(p + 16 * i));
+        *reinterpret_cast<u32x4 *>(p + 16 * i) =
+            u32x4{pack_bf16x2(x[8 * i], x[8 * i + 1]), pack_bf16x2(x[8 * i + 2], x[8 * i + 3]),
+                  pack_bf16x2(x[8 * i + 4], x[8 * i + 5]), pack_bf16x2(x[8 * i + 6], x[8 * i + 7])};
     }
   }
 };

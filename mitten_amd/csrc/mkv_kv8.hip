@@ -98,8 +98,22 @@ struct PrepLane {
   }
 };
 
+#define KV8_EU(D, F32) ((D) * ((F32) ? 2 : 1) <= 64 ? 4 : (D) * ((F32) ? 2 : 1) <= 128 ? 3 : (D) * ((F32) ? 2 : 1) <= 256 ? 2 : 1)
+// VEC values as they are loaded.
+template <bool F32, int VEC>
+struct PrepRaw {
+  typedef uint32_t type __attribute__((ext_vector_type(F32 ? VEC : VEC / 2)));
+  static __device__ __forceinline__ void widen(const type &w, float (&x)[VEC]) {
+#pragma unroll
+    for (int e = 0; e < VEC; e++) {
+      if constexpr (F32) x[e] = __uint_as_float(w[e]);
+      else x[e] = e & 1 ? bf16_hi(w[e >> 1]) : bf16_lo(w[e >> 1]);
+    }
+  }
+};
+
 template <int D, bool F32, int VEC>
-__global__ void __launch_bounds__(256) kv8_prep_kernel(Kv8Args a, Kv8PrepArgs p) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KV8_EU(D, F32)))) kv8_prep_kernel(Kv8Args a, Kv8PrepArgs p) {
   typedef Kv8Row<F32> Row;
   typedef PrepLane<D, VEC> Lane;
   constexpr int ES = Row::ES, NP = Lane::NP;
@@ -114,7 +128,7 @@ __global__ void __launch_bounds__(256) kv8_prep_kernel(Kv8Args a, Kv8PrepArgs p)
   const int blocks = (s.ctx - 1) / kPageSize - (s.ctx - s.n) / kPageSize + 1;
   const int64_t kv_stride = (int64_t)a.Hkv * D * ES;
   const Lane ln(p, lane);
-  const int half = p.rd >> 1, units = a.Hq + 2 * a.Hkv;
+  const int half = p.rd >> 1;
   for (int64_t j = blockIdx.x; j < blocks; j += gridDim.x) {
     int32_t blk;
     int o0, o1;
@@ -133,28 +147,39 @@ __global__ void __launch_bounds__(256) kv8_prep_kernel(Kv8Args a, Kv8PrepArgs p)
       cs[t][1][c] = sn * p.factor;
     }
     __syncthreads();
-    for (int u = blockIdx.z * 4 + wave; u < units; u += gridDim.z * 4) {
-      if (u >= a.Hq + a.Hkv) {
-        const int h = u - a.Hq - a.Hkv;
-        const int64_t at = (int64_t)blk * a.Hkv + h;
-        if (ok)
-          kv8_write_v<D, F32>(p.v + row0 * kv_stride + (int64_t)h * D * ES, kv_stride, a.v_tiles + at * 16 * D,
-                              a.v_exps + at, lane, o0, o1);
-        continue;
+    // Heads of q and k in turn, the next one's rows loaded before this one is used.
+    // Token t of a pass is row o0 + t of the tile; its rows lie at lane offsets of the
+    // first one's (32 bits: 16 rows of a call).
+    const int n = o1 - o0, by = gridDim.z * 4, heads = a.Hq + a.Hkv;
+    typedef typename PrepRaw<F32, VEC>::type raw_t;
+    raw_t cur[NP][2], nxt[NP][2];
+    const uint8_t *q0 = p.q + row0 * a.Hq * p.q_stride * ES, *k0 = p.k + row0 * kv_stride;
+    auto load = [&](int u, raw_t (&r)[NP][2]) {
+      const bool is_k = u >= a.Hq;
+      const uint8_t *src = is_k ? k0 + (u - a.Hq) * D * ES : q0 + u * p.q_stride * ES;
+      const uint32_t stride = (is_k ? a.Hkv * D : a.Hq * p.q_stride) * ES;
+#pragma unroll
+      for (int i = 0; i < NP; i++) {
+        const uint32_t off = (uint32_t)min(ln.tok0 + i * Lane::TPP, n - 1) * stride;
+        r[i][0] = *reinterpret_cast<const raw_t *>(src + (off + ln.a0 * ES));
+        r[i][1] = *reinterpret_cast<const raw_t *>(src + (off + ln.a1 * ES));
       }
-      // Rows o0 .. o1 - 1 of this head, token t of a pass at tile row o0 + t.
+    };
+    int u = blockIdx.z * 4 + wave;
+    if (u < heads) load(u, cur);
+    for (; u < heads; u += by) {
       const bool is_k = u >= a.Hq;
       const int h = is_k ? u - a.Hq : u;
       const float *w = is_k ? p.wk : p.wq;
-      const int n = o1 - o0;
+      if (u + by < heads) load(u + by, nxt);
       float x[NP][2][VEC];
 #pragma unroll
-      for (int i = 0; i < NP; i++) {
-        const int64_t row = row0 + min(ln.tok0 + i * Lane::TPP, n - 1);
-        const uint8_t *src = is_k ? p.k + (row * a.Hkv + h) * D * ES : p.q + (row * a.Hq + h) * p.q_stride * ES;
-        Row::load(src + ln.a0 * ES, x[i][0]);
-        Row::load(src + ln.a1 * ES, x[i][1]);
-      }
+      for (int i = 0; i < NP; i++)
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+          PrepRaw<F32, VEC>::widen(cur[i][r], x[i][r]);
+          cur[i][r] = nxt[i][r];
+        }
       float w0[VEC], w1[VEC];
       if (p.norm) {
         Kv8Row<true>::load(reinterpret_cast<const uint8_t *>(w + ln.a0), w0);
@@ -208,9 +233,10 @@ __global__ void __launch_bounds__(256) kv8_prep_kernel(Kv8Args a, Kv8PrepArgs p)
           for (int e = 0; e < VEC; e++)
             amax = fmaxf(amax, fmaxf(kv8_finite_abs(x[i][0][e]), kv8_finite_abs(x[i][1][e])));
         } else if (ln.tok0 + i * Lane::TPP < n) {
-          uint8_t *dst = p.q_out + ((row0 + t) * a.Hq + h) * D * ES;
-          Row::store(dst + ln.a0 * ES, x[i][0]);
-          Row::store(dst + ln.a1 * ES, x[i][1]);
+          uint8_t *dst = p.q_out + (row0 * a.Hq + h) * D * ES;
+          const uint32_t off = (uint32_t)t * (a.Hq * D * ES);
+          Row::store(dst + (off + ln.a0 * ES), x[i][0]);
+          Row::store(dst + (off + ln.a1 * ES), x[i][1]);
         }
       }
       if (!is_k || !ok) continue;
@@ -242,6 +268,13 @@ __global__ void __launch_bounds__(256) kv8_prep_kernel(Kv8Args a, Kv8PrepArgs p)
       }
       if (lane == 0 && e != e_old) a.k_exps[at] = (int8_t)e;
     }
+    if (ok)
+      for (; u < heads + a.Hkv; u += by) {
+        const int h = u - heads;
+        const int64_t at = (int64_t)blk * a.Hkv + h;
+        kv8_write_v<D, F32>(p.v + row0 * kv_stride + (int64_t)h * D * ES, kv_stride, a.v_tiles + at * 16 * D,
+                            a.v_exps + at, lane, o0, o1);
+      }
     __syncthreads();  // the table is written again for the next block
   }
 }
@@ -281,28 +314,16 @@ __global__ void __launch_bounds__(256) kv8_gather_kernel(Kv8Args a, int32_t max_
       continue;
     }
     const int64_t at = (int64_t)blk * a.Hkv + h;
-    const float scale = kv8_scale((kv ? a.v_exps : a.k_exps)[at]);
     const uint8_t *tile = (kv ? a.v_tiles : a.k_tiles) + at * 16 * D;
     u32x4 w[D / 64];
 #pragma unroll
     for (int r = 0; r < D / 64; r++)
       w[r] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(tile + 1024 * r) + lane);
+    const float scale = kv8_scale((kv ? a.v_exps : a.k_exps)[at]);
     const int nv = min(kPageSize, ctx - j * kPageSize), lo = lane & 15, hi = lane >> 4;
     const int64_t base = (c0 * a.Hkv + (int64_t)h * ctx + (int64_t)j * kPageSize) * D;
-    if (kv) {
-#pragma unroll
-      for (int i = 0; i < D / 64; i++) {
-        float x[4][4];  // [dim][token]
-#pragma unroll
-        for (int n = 0; n < 4; n++) kv8_unpack4(w[i][n], x[n]);
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-          if (4 * hi + t >= nv) continue;
-          const float y[4] = {x[0][t] * scale, x[1][t] * scale, x[2][t] * scale, x[3][t] * scale};
-          Row::store(out_v + (base + (int64_t)(4 * hi + t) * D + 64 * i + 4 * lo) * Row::ES, y);
-        }
-      }
-    } else if (lo < nv) {
+    if (!kv) {
+      if (lo >= nv) continue;
 #pragma unroll
       for (int r = 0; r < D / 64; r++) {
         float y[16];
@@ -314,6 +335,42 @@ __global__ void __launch_bounds__(256) kv8_gather_kernel(Kv8Args a, int32_t max_
           for (int c = 0; c < 4; c++) y[4 * z + c] = x[c] * scale;
         }
         Row::store(out_k + (base + (int64_t)lo * D + 64 * r + 16 * hi) * Row::ES, y);
+      }
+      continue;
+    }
+#pragma unroll
+    for (int i = 0; i < D / 64; i++) {
+      float x[4][4];  // [dim][token]
+#pragma unroll
+      for (int n = 0; n < 4; n++) {
+        kv8_unpack4(w[i][n], x[n]);
+#pragma unroll
+        for (int t = 0; t < 4; t++) x[n][t] *= scale;
+      }
+      if constexpr (F32) {
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+          const float y[4] = {x[0][t], x[1][t], x[2][t], x[3][t]};
+          if (4 * hi + t < nv) Row::store(out_v + (base + (int64_t)(4 * hi + t) * D + 64 * i + 4 * lo) * 4, y);
+        }
+      } else {
+        // Two neighbours trade two tokens each for 16-byte stores: the even lane takes
+        // tokens 0 and 1 of eight dims, the odd one tokens 2 and 3.
+        const bool odd = lane & 1;
+        uint32_t p[4][2];
+#pragma unroll
+        for (int t = 0; t < 4; t++) p[t][0] = pack_bf16x2(x[0][t], x[1][t]), p[t][1] = pack_bf16x2(x[2][t], x[3][t]);
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+          uint32_t got[2];
+#pragma unroll
+          for (int z = 0; z < 2; z++)
+            got[z] = (uint32_t)__builtin_amdgcn_mov_dpp((int)(odd ? p[t][z] : p[t + 2][z]), 0xb1, 0xf, 0xf, false);
+          const int tok = 4 * hi + t + (odd ? 2 : 0);
+          const u32x4 y = odd ? u32x4{got[0], got[1], p[t + 2][0], p[t + 2][1]} : u32x4{p[t][0], p[t][1], got[0], got[1]};
+          if (tok < nv)
+            *reinterpret_cast<u32x4 *>(out_v + (base + (int64_t)tok * D + 64 * i + 4 * (lo & ~1)) * 2) = y;
+        }
       }
     }
   }
@@ -767,7 +824,7 @@ extern "C" int mkv_kv8_qk_norm_rope_append(mkv_kv8_pool *pool, int32_t layer, co
   // Few blocks: the heads of each are dealt to several workgroups, so that a
   // decode step's waves each take one head or two.
   const int64_t units = g.Hq + 2 * g.Hkv, wgs = blocks * num_seqs;
-  const int64_t z = std::max<int64_t>(1, std::min<int64_t>((units + 3) / 4, 4 * p->cus / wgs));
+  const int64_t z = std::max<int64_t>(1, std::min<int64_t>((units + 3) / 4, (8 * p->cus + wgs - 1) / wgs));
   const dim3 grid((unsigned)blocks, (unsigned)num_seqs, (unsigned)z);
 #define KV8_PREP(DD, FF)                                                                                     \
   do {                                                                                                       \
@@ -835,8 +892,8 @@ extern "C" int mkv_kv8_gather(mkv_kv8_pool *pool, int32_t layer, const int32_t *
   DeviceGuard guard(p->device);
   hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
   const Kv8Args a = kv8_args(p, layer, nullptr, d_block_indptr, d_block_ids, d_ctx_lens, num_seqs, 0);
-  const int64_t wgs = (((int64_t)max_ctx_len + kPageSize - 1) / kPageSize * 2 * g.Hkv + 3) / 4;
-  const dim3 grid((unsigned)std::min<int64_t>(wgs, 1 << 20), (unsigned)num_seqs);
+  const int64_t units = ((int64_t)max_ctx_len + kPageSize - 1) / kPageSize * 2 * g.Hkv;
+  const dim3 grid((unsigned)std::min<int64_t>((units + 3) / 4, 1 << 20), (unsigned)num_seqs);
   KV8_DISPATCH(kv8_gather_kernel, grid, hs, a, max_ctx_len, static_cast<uint8_t *>(d_out_k),
                static_cast<uint8_t *>(d_out_v), out_capacity_tokens);
   MKV_CHECK_LAUNCH("kv8_gather_kernel");

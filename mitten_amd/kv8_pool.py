@@ -111,6 +111,8 @@ class DeviceKv8Pool:
                                               ctypes.byref(en)))
         self.tiles_ptr, self.tile_bytes, self.exponents_ptr, self.exponent_bytes = t.value, tn.value, e.value, en.value
         self._dtype = _torch_type(desc.dtype)
+        self._tensor, self._int32 = _torch().Tensor, _torch().int32
+        self._device = _torch().device("cuda", device)
         self._scale = float(np.float32(desc.head_dim ** -0.5))
 
     # -- lifecycle -------------------------------------------------------------------
@@ -174,34 +176,34 @@ class DeviceKv8Pool:
     def _rows(self, t, shape, name, dtype=None):
         """Address of a contiguous tensor of that shape on the pool's device."""
         dtype = dtype or self._dtype
-        torch = _torch()
-        if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != shape or not t.is_cuda or \
-                t.device.index != self.device or not t.is_contiguous():
+        if not isinstance(t, self._tensor) or t.dtype != dtype or t.shape != shape or t.device != self._device or \
+                not t.is_contiguous():
             _check(t, self.device, shape, dtype, name)  # (names what is wrong)
         return t.data_ptr()
 
     def _num_rows(self, t, name, dims):
-        torch = _torch()
-        if not isinstance(t, torch.Tensor) or t.dim() != dims:
+        if not isinstance(t, self._tensor) or t.dim() != dims:
             raise _bad(f"{name} must be a tensor of {dims} dimensions")
         return t.shape[0]
 
     def _i32(self, t, name, n=None):
-        torch = _torch()
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or not t.is_cuda or \
-                t.device.index != self.device or t.dim() != 1 or not t.is_contiguous() or \
-                (n is not None and t.shape[0] != n):
-            _check(t, self.device, None if n is None else (n,), torch.int32, name)
+        if not isinstance(t, self._tensor) or t.dtype != self._int32 or t.device != self._device or t.dim() != 1 or \
+                not t.is_contiguous() or (n is not None and t.shape[0] != n):
+            _check(t, self.device, None if n is None else (n,), self._int32, name)
             raise _bad(f"{name} must have one dimension")
         return t.data_ptr()
 
-    @staticmethod
-    def _form(block_indptr, block_ids, ctx_lens, q_lens=None):
+    def _form(self, block_indptr, block_ids, ctx_lens, q_lens=None):
         """Whether the metadata is the host's; all of it has to be, or none."""
-        host = _is_host(ctx_lens)
-        for x in (block_indptr, block_ids) + (() if q_lens is None else (q_lens,)):
-            if _is_host(x) != host:
+        tensor = self._tensor
+        host = None
+        for x in (ctx_lens, block_indptr, block_ids, q_lens):
+            if x is None and x is q_lens:
+                continue
+            h = not x.is_cuda if isinstance(x, tensor) else _is_host(x)
+            if host is not None and h != host:
                 raise _bad("lengths and tables must all be host arrays or all device tensors")
+            host = h
         return host
 
     def _tables(self, block_indptr, block_ids, ctx_lens):
@@ -238,8 +240,9 @@ class DeviceKv8Pool:
 
     def _out(self, out, shape, stream, name="out"):
         if out is None:
-            out = _empty_on(stream, shape, self._dtype, f"cuda:{self.device}")
-        self._rows(out, shape, name)
+            out = _empty_on(stream, shape, self._dtype, self._device)
+        else:
+            self._rows(out, shape, name)
         return out
 
     def _workspace(self, workspace):
@@ -347,7 +350,7 @@ class DeviceKv8Pool:
         outs = []
         for t, name in ((out_k, "out_k"), (out_v, "out_v")):
             if t is None:
-                t = _empty_on(stream, n, self._dtype, f"cuda:{self.device}")
+                t = _empty_on(stream, n, self._dtype, self._device)
             _check(t, self.device, None, self._dtype, name)
             if t.numel() < n:
                 raise _bad(f"{name} is too small")
