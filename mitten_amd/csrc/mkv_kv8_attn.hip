@@ -483,7 +483,8 @@ __device__ __forceinline__ int kv8_chunk_heads(int G, int qc) { return min(16, G
 template <int D, bool F32>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
 kv8_decode_split_kernel(Kv8Args a, Kv8Dec dc) {
-  extern __shared__ int32_t pre[];  // [B + 1] steps before each sequence
+  extern __shared__ int32_t pre[];  // [B + 1] steps before each sequence, then their lengths and tables
+  int32_t *ctx_s = pre + a.B + 1, *tab_s = ctx_s + a.B;
   __shared__ int32_t wsum[4];
   const int lane = threadIdx.x & 63, m16 = lane & 15, g4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -495,6 +496,8 @@ kv8_decode_split_kernel(Kv8Args a, Kv8Dec dc) {
       const int n = kv8_steps(a, b, dc.max_ctx, err);
       if (err && blockIdx.x == 0) record_error(a.d_err, err);
       pre[b + 1] = n;  // (own entries only, turned into the scan below)
+      ctx_s[b] = a.ctx[b];
+      tab_s[b] = a.indptr[b];
       sum += n;
     }
     int inc = sum;
@@ -545,7 +548,7 @@ kv8_decode_split_kernel(Kv8Args a, Kv8Dec dc) {
         if (pre[mid] <= f) lo = mid;
         else hi = mid;
       }
-      it = kv8_item(a, lo, a.ctx[lo], a.indptr[lo], f - pre[lo]);
+      it = kv8_item(a, lo, ctx_s[lo], tab_s[lo], f - pre[lo]);
     }
     kv8_run<D, F32>(a, dc, lane, h, n, it, cur, q, E, st, start, finish);
   }
@@ -1089,22 +1092,50 @@ kv8_extend_kernel(Kv8Args a, Kv8Ext e) {
   }
 }
 
-// The merge of split key ranges: a wave per (query head, token of sequence blockIdx.y).
+// The merge of split key ranges: a thread per 4 dims of a (token, query head) row of
+// sequence blockIdx.y.
 template <int D, bool F32>
 __global__ void __launch_bounds__(256) kv8_extend_merge_kernel(Kv8Args a, Kv8Ext e) {
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr int TPR = D / 4;  // threads of a row
   Kv8Seq s;
   if (kv8_seq(a, blockIdx.y, e.max_ctx, s) || s.n == 0) return;
-  KArgs ka;
-  ka.o = e.o;
-  ka.zero_sink = e.zero_sink;
   const int64_t rows = (int64_t)s.n * a.Hq, first = (int64_t)s.q0 * a.Hq;
-  for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < rows; r += (int64_t)gridDim.x * 4) {
-    const int64_t row = first + r;
-    merge_partials<D, !F32>(
-        ka, lane, e.splits, [&](int i) { return e.ws_ml + 2 * (row * e.splits + i); },
-        [&](int i) { return e.ws_o + (row * e.splits + i) * D; }, row);
+  const int dim = 4 * (threadIdx.x % TPR);
+  for (int64_t r = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR; r < rows; r += (int64_t)gridDim.x * (256 / TPR)) {
+    const int64_t at = (first + r) * e.splits;
+    float M = -FLT_MAX, L = 0.0f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    constexpr int N = 8;  // partials loaded at a time
+    for (int i0 = 0; i0 < e.splits; i0 += N) {
+      float2 y[N];
+      f32x4 o[N];
+#pragma unroll
+      for (int i = 0; i < N; i++) {  // (past the last partial: the last one, with no weight)
+        const int64_t c = at + min(i0 + i, e.splits - 1);
+        y[i] = *reinterpret_cast<const float2 *>(e.ws_ml + 2 * c);
+        o[i] = *reinterpret_cast<const f32x4 *>(e.ws_o + c * D + dim);
+      }
+      float m = M;
+#pragma unroll
+      for (int i = 0; i < N; i++) m = fmaxf(m, y[i].x);
+      const float f = fast_exp2(M - m);
+      L *= f;
+      acc *= f;
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        if (i0 + i >= e.splits) break;
+        const float w = fast_exp2(y[i].x - m);
+        L = fmaf(y[i].y, w, L);
+        acc += o[i] * w;
+      }
+      M = m;
+    }
+    acc *= final_scale(M, L, e.zero_sink);
+    const int64_t out = (first + r) * D + dim;
+    if constexpr (F32) *reinterpret_cast<f32x4 *>(static_cast<float *>(e.o) + out) = acc;
+    else
+      *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(e.o) + out) =
+          make_uint2(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]));
   }
 }
 
@@ -1152,7 +1183,7 @@ static int launch_kv8_decode(const Kv8Pool *p, const Kv8Args &a, Kv8Dec &d, int6
     return MKV_OK;
   }
   d.pieces = (int32_t)pieces;
-  KV8_LAUNCH(kv8_decode_split_kernel, dim3((unsigned)((pieces * heads + 3) / 4)), dim3(256), (a.B + 1) * 4, a, d);
+  KV8_LAUNCH(kv8_decode_split_kernel, dim3((unsigned)((pieces * heads + 3) / 4)), dim3(256), (3 * a.B + 1) * 4, a, d);
   MKV_CHECK_LAUNCH("kv8_decode_split_kernel");
   KV8_LAUNCH(kv8_decode_merge_kernel, dim3((unsigned)g.Hq, (unsigned)a.B), dim3(256), 0, a, d);
   MKV_CHECK_LAUNCH("kv8_decode_merge_kernel");
@@ -1161,28 +1192,40 @@ static int launch_kv8_decode(const Kv8Pool *p, const Kv8Args &a, Kv8Dec &d, int6
 
 // ---- extend
 
-// Rows and waves of a workgroup: many rows take the wide form (an LDS operand feeds
-// two groups of rows where the registers allow it), few the narrow one.
+// The forms of the extend kernel: rows and waves of a workgroup, and what a step of 32
+// keys takes it in us, alone on a CU and beside a second one (0: none fits). Wide: an
+// LDS operand feeds two groups of rows where the registers allow it. Measured: 16
+// chunks of 5-24 tokens after 4-8k unsplit, and 8 of 512 after 4k.
 struct Kv8ExtForm {
   const void *fn;
   int rows, waves;
+  double alone, beside;
 };
 static Kv8ExtForm kv8_ext_form(const Geom &g, bool wide) {
-#define KV8_EXT(DD, FF, RR, WW) \
-  Kv8ExtForm { reinterpret_cast<const void *>(&kv8_extend_kernel<DD, FF, RR, WW>), 16 * RR * WW, WW }
+#define KV8_EXT(DD, FF, RR, WW, ALONE, BESIDE) \
+  Kv8ExtForm { reinterpret_cast<const void *>(&kv8_extend_kernel<DD, FF, RR, WW>), 16 * RR * WW, WW, ALONE, BESIDE }
   const bool f32 = g.dtype == MKV_DTYPE_F32;
   switch (g.D) {
     case 64:
-      if (f32) return wide ? KV8_EXT(64, true, 2, 4) : KV8_EXT(64, true, 1, 4);
-      return wide ? KV8_EXT(64, false, 2, 4) : KV8_EXT(64, false, 1, 4);
+      if (f32) return wide ? KV8_EXT(64, true, 2, 4, .77, 1.37) : KV8_EXT(64, true, 1, 4, .56, .75);
+      return wide ? KV8_EXT(64, false, 2, 4, .58, .92) : KV8_EXT(64, false, 1, 4, .48, .58);
     case 128:
-      if (f32) return wide ? KV8_EXT(128, true, 1, 8) : KV8_EXT(128, true, 1, 4);
-      return wide ? KV8_EXT(128, false, 2, 4) : KV8_EXT(128, false, 1, 4);
+      if (f32) return wide ? KV8_EXT(128, true, 1, 8, 1.26, 0) : KV8_EXT(128, true, 1, 4, .85, 1.15);
+      return wide ? KV8_EXT(128, false, 2, 4, .76, 1.24) : KV8_EXT(128, false, 1, 4, .60, .78);
     default:
-      if (f32) return KV8_EXT(256, true, 1, 4);
-      return wide ? KV8_EXT(256, false, 1, 8) : KV8_EXT(256, false, 1, 4);
+      if (f32) return KV8_EXT(256, true, 1, 4, 2.0, 0);
+      return wide ? KV8_EXT(256, false, 1, 8, 1.0, 0) : KV8_EXT(256, false, 1, 4, .88, 1.28);
   }
 #undef KV8_EXT
+}
+
+// What a call takes, by that: `tiles` workgroups' worth of rows over `steps` each, in
+// `splits` shares; a merge is a launch and its partials' bytes both ways.
+static double kv8_ext_cost(const Kv8ExtForm &f, double cus, double tiles, double steps, int splits, double values) {
+  const double wgs = tiles * splits / cus;
+  double step = f.alone;
+  if (wgs > 1) step = f.beside > 0 ? std::max(f.beside, f.beside * std::ceil(wgs) / 2) : f.alone * std::ceil(wgs);
+  return std::ceil(steps / splits) * step + 3.0 + (splits > 1 ? 5.0 + values * splits * 8 / 5.0e6 : 0.0);
 }
 
 }  // namespace mkv
@@ -1309,19 +1352,32 @@ extern "C" int mkv_kv8_extend_attention(mkv_kv8_pool *pool, int32_t layer, const
   e.zero_sink = (flags & MKV_ATTN_ZERO_SINK) ? 1 : 0;
   const int64_t pairs = (int64_t)g.Hkv * num_seqs, rows = (int64_t)std::min(max_q_len, num_tokens) * a.G;
   if ((int64_t)num_tokens * a.G > INT32_MAX / 2) return set_error(MKV_ERR_INVALID_ARGUMENT, "too many tokens");
-  Kv8ExtForm form = kv8_ext_form(g, true);
-  if ((rows + form.rows - 1) / form.rows * pairs < p->cus) form = kv8_ext_form(g, false);
+  // The form and the split of the key ranges that cost least, for sequences of the mean
+  // length of a chunk and the longest context. At most 32 shares of at least 4 steps,
+  // and no more than the workspace holds the partials of.
+  const double mean = std::max(1.0, std::min<double>((double)rows, (double)num_tokens * a.G / num_seqs));
+  const int64_t steps = ((int64_t)max_ctx_len + kKv8Step - 1) / kKv8Step;
+  const uint64_t per = (uint64_t)num_tokens * g.Hq * (8 + 4 * g.D);
+  const uint64_t bytes = d_workspace ? workspace_bytes : kKv8Workspace, room = bytes > 256 ? bytes - 256 : 0;
+  const int most = (int)std::max<int64_t>(1, std::min({steps / 4, (int64_t)32, (int64_t)(room / per)}));
+  Kv8ExtForm form{};
+  double best = INFINITY;
+  for (int narrow = 0; narrow < 2; narrow++) {
+    const Kv8ExtForm f = kv8_ext_form(g, !narrow);
+    for (int sp = 1; sp <= most; sp++) {
+      const double c = kv8_ext_cost(f, p->cus, (double)pairs * std::ceil(mean / f.rows), (double)steps, sp,
+                                    (double)num_tokens * g.Hq * g.D);
+      if (c < 0.97 * best) {  // (equal costs: the wide form, fewer shares)
+        best = c;
+        form = f;
+        e.splits = sp;
+      }
+    }
+  }
   const int64_t tiles = (rows + form.rows - 1) / form.rows;
   Kv8Ws ws;
-  // Key ranges are split where the tiles leave CUs without one: into shares of at
-  // least 8 steps, and no more than the workspace holds the partials of.
-  const int64_t steps = ((int64_t)max_ctx_len + kKv8Step - 1) / kKv8Step;
-  const int64_t slots = (int64_t)p->cus * (8 / form.waves);
-  const int64_t want = std::min({slots / std::max<int64_t>(1, tiles * pairs), steps / 8, (int64_t)16});
-  if (want > 1) {
+  if (e.splits > 1) {
     if ((rc = kv8_ws_begin(p, d_workspace, workspace_bytes, hs, &ws))) return rc;
-    const uint64_t per = (uint64_t)num_tokens * g.Hq * (8 + 4 * g.D), room = ws.bytes > 256 ? ws.bytes - 256 : 0;
-    e.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(want, (int64_t)(room / per)));
     e.ws_ml = static_cast<float *>(ws.ptr);
     e.ws_o = reinterpret_cast<float *>(static_cast<uint8_t *>(ws.ptr) +
                                        kv8_ml_bytes((uint64_t)num_tokens * g.Hq * e.splits));
@@ -1333,7 +1389,7 @@ extern "C" int mkv_kv8_extend_attention(mkv_kv8_pool *pool, int32_t layer, const
   MKV_CHECK_HIP(hipLaunchKernel(form.fn, dim3((unsigned)grid), dim3(64 * form.waves), args, 0, hs));
   MKV_CHECK_LAUNCH("kv8_extend_kernel");
   if (e.splits > 1) {
-    const int64_t wgs = ((int64_t)std::min(max_q_len, num_tokens) * g.Hq + 3) / 4;
+    const int64_t per = 1024 / g.D, wgs = ((int64_t)std::min(max_q_len, num_tokens) * g.Hq + per - 1) / per;
     const dim3 mgrid((unsigned)std::min<int64_t>(wgs, 1 << 20), (unsigned)num_seqs);
     KV8_LAUNCH(kv8_extend_merge_kernel, mgrid, dim3(256), 0, a, e);
     MKV_CHECK_LAUNCH("kv8_extend_merge_kernel");
