@@ -721,7 +721,8 @@ MKV_API int mkv_kv8_copy_blocks_host(mkv_kv8_pool *pool, const uint32_t *h_src_b
  * follow one another across streams; a captured one must not be replayed beside
  * another call or graph that uses it (give each a workspace). Scores, sums and
  * partials are f32; weights enter the product with V in 11 bits (bf16 rows) or
- * 22 (f32 rows). Flags: MKV_ATTN_ZERO_SINK. num_seqs at most 65535. */
+ * 22 (f32 rows), and one whose product with its tile's 2^e is below 2^-32 of the
+ * greatest such product as nothing. Flags: MKV_ATTN_ZERO_SINK. num_seqs at most 65535. */
 MKV_API int mkv_kv8_decode_attention(mkv_kv8_pool *pool, int32_t layer, const void *d_k_new, const void *d_v_new,
                                      const void *d_q, void *d_o, const int32_t *d_block_indptr,
                                      const int32_t *d_block_ids, const int32_t *d_ctx_lens, int32_t num_seqs,

@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(256) kv8_gather_kernel(Kv8Args a, int32_t max_
     if (blockIdx.x == 0 && threadIdx.x == 0) record_error(a.d_err, err);
     return;
   }
-  const int64_t units = (int64_t)((ctx + kPageSize - 1) / kPageSize) * 2 * a.Hkv;
+  const int64_t units = ((int64_t)ctx + kPageSize - 1) / kPageSize * 2 * a.Hkv;
   for (int64_t u = (int64_t)blockIdx.x * 4 + wave; u < units; u += (int64_t)gridDim.x * 4) {
     const int h = (int)(u % a.Hkv), kv = (int)(u / a.Hkv) & 1, j = (int)(u / (2 * a.Hkv));
     const int32_t blk = ((const kv8_const_i32 *)a.ids)[(int64_t)tab0 + j];

@@ -27,10 +27,12 @@ namespace mkv {
 
 constexpr float kBias = 15.0f - kRescaleSlack;
 constexpr int kMaxRaise = 40;
-// d, at least: what a tile lies below that is taken from its weights after l is
-// summed. (With sums from the matrix unit 2^-d is an f16 number.)
-template <bool SUMS>
-constexpr int kFarExp = SUMS ? 15 : 40;
+// d, at least: what a tile lies below that is taken from its weights after l is summed.
+constexpr int kFarExp = 40;
+// The matrix unit sums the rounded weights of tiles with d >= -kSumExp: what f16 drops
+// of one is below 2^-32 of the greatest s + d, 2^-28 of l. Behind that a long row of
+// small weights could be missed, and l is summed from the f32 weights.
+constexpr int kSumExp = 4;
 constexpr int kNoExp = -1000;
 
 template <int D, bool F32>
@@ -129,10 +131,9 @@ struct Kv8State {
 
 // Exponents of a step's two tiles against E: d >= -kFarExp, and what is left of
 // ev - E beyond that.
-template <bool SUMS>
 __device__ __forceinline__ void kv8_offsets(int E, int ev0, int ev1, int (&d)[2], int (&far)[2]) {
-  d[0] = max(ev0 - E, -kFarExp<SUMS>);
-  d[1] = max(ev1 - E, -kFarExp<SUMS>);
+  d[0] = max(ev0 - E, -kFarExp);
+  d[1] = max(ev1 - E, -kFarExp);
   far[0] = ev0 - E - d[0];
   far[1] = ev1 - E - d[1];
 }
@@ -187,10 +188,30 @@ __device__ __forceinline__ void kv8_weights(const float (&S)[2][4], float sl2, c
   }
 }
 
-// 2^-d of each key, with which the matrix unit sums the weights (SUMS).
+// 2^-d of each key, with which the matrix unit sums the weights (SUMS); 0 of a tile
+// that kv8_sum_low takes.
 __device__ __forceinline__ f16x8 kv8_ones(const int (&d)[2]) {
-  const _Float16 a = (_Float16)__builtin_ldexpf(1.0f, -d[0]), b = (_Float16)__builtin_ldexpf(1.0f, -d[1]);
-  return f16x8{a, a, a, a, b, b, b, b};
+  _Float16 y[2];
+#pragma unroll
+  for (int kb = 0; kb < 2; kb++) y[kb] = (_Float16)(d[kb] < -kSumExp ? 0.0f : __builtin_ldexpf(1.0f, -d[kb]));
+  return f16x8{y[0], y[0], y[0], y[0], y[1], y[1], y[1], y[1]};
+}
+template <int D>
+__device__ __forceinline__ void kv8_sum_low(const float (&S)[2][4], float sl2, const int (&d)[2],
+                                            Kv8State<D, true> &st) {
+  float l = 0.0f;
+#pragma unroll
+  for (int kb = 0; kb < 2; kb++) {
+    if (d[kb] >= -kSumExp) continue;
+    const float base = st.R - kBias - (float)d[kb];
+    float w = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) w += fast_exp2(fmaf(S[kb][i], sl2, -base));
+    l += __builtin_ldexpf(w, -d[kb]);
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  st.l += l;
 }
 
 // What a tile lies below E - kFarExp, taken from its weights.
@@ -357,7 +378,7 @@ __device__ __forceinline__ void kv8_step(float sl2, Kv8Raw<D> &raw, int lane, in
   }
   kv8_raise(E, ev[0], ev[1], st);
   int d[2], far[2];
-  kv8_offsets<false>(E, ev[0], ev[1], d, far);
+  kv8_offsets(E, ev[0], ev[1], d, far);
   float t[2][4];
 #pragma unroll
   for (int kb = 0; kb < 2; kb++) {
@@ -822,7 +843,7 @@ __device__ __forceinline__ void kv8_extend_tile(const Kv8Args &a, const Kv8Ext &
   auto settle = [&](const f32x4 (&S)[RT][2], int ev0, int ev1, float (&t)[RT][2][4], int (&d)[2], int (&far)[2],
                     auto mask) {
     kv8_raise(E, ev0, ev1, st);
-    kv8_offsets<!F32>(E, ev0, ev1, d, far);
+    kv8_offsets(E, ev0, ev1, d, far);
     float top[RT];
     bool move = false;
 #pragma unroll
@@ -838,6 +859,10 @@ __device__ __forceinline__ void kv8_extend_tile(const Kv8Args &a, const Kv8Ext &
     if (__ballot(move))
 #pragma unroll
       for (int x = 0; x < RT; x++) kv8_rescale(top[x], st[x]);
+    if constexpr (!F32)
+      if (min(d[0], d[1]) < -kSumExp)  // (uniform, rare)
+#pragma unroll
+        for (int x = 0; x < RT; x++) kv8_sum_low(t[x], e.sl2, d, st[x]);
   };
 
   f32x4 S[2][RT][2];
