@@ -263,7 +263,9 @@ __device__ __forceinline__ void kv8_store(const Kv8State<D, SUMS> &st, int E, in
 //     two partials per piece, which a second launch merges;
 //   seq: one workgroup of 8 waves (4 at head_dim 256) per (sequence, KV head, 16 query
 //     heads), their states merged in LDS; one launch.
-// What bounds it: memory, see the launch rule below.
+// What bounds it: memory for many long contexts (64 of 1 to 8k tokens, 280 MB: 54 us
+// for the split kernel, 5.2 TB/s, and 5 for the merge), the chain of dependent loads for
+// few or short ones (lengths, ids, tiles, partials: 8 us at the least, 12.7 split).
 // ===========================================================================
 
 constexpr int kSplitSeqs = 4096;   // sequences of one split launch (their scan stands in LDS)
@@ -322,7 +324,8 @@ struct Kv8Raw {
 
 // The new rows of the n steps whose ids `it` holds, written into their tiles before
 // these are read: a step that is its sequence's last has one. (Put into the loaded
-// registers inside the loop instead, they spilled: 36 registers at head_dim 128.)
+// registers inside the loop instead, they spilled: 36 registers at head_dim 128. This
+// costs 2.4 of 63.4 us for 64 sequences of 1 to 8k tokens.)
 template <int D, bool F32>
 __device__ __forceinline__ void kv8_insert(const Kv8Args &a, const Kv8Dec &dc, int lane, int h, int n,
                                            const Kv8Items &it) {
@@ -433,6 +436,7 @@ __device__ __forceinline__ void kv8_run(const Kv8Args &a, const Kv8Dec &dc, int 
   if (dc.new_k) kv8_insert<D, F32>(a, dc, lane, h, n, it);
   if (lane < n) kv8_item_exps(a, h, it);
   Kv8Raw<D> raw[RING];
+  // (Past the caches: 63.4 us for 64 sequences of 1 to 8k tokens, plain loads 70.6.)
   auto issue = [&](Kv8Raw<D> &w, int k) {
     const bool live = k < n;
     const int kk = live ? k : n - 1;
@@ -717,8 +721,12 @@ kv8_decode_seq_kernel(Kv8Args a, Kv8Dec dc) {
 // there in operand order: 16 bytes a lane, contiguous, no bank conflicts either way.
 // An operand is read once for RT products: LDS gives 128 bytes a cycle and CU, so at
 // RT = 1 the reads of a step take as long as twice its products, at RT = 2 as long.
-// Loads run kExtRing - 1 steps ahead in registers (16 bytes a lane and 1 KiB of tile);
+// Loads run kKv8ExtRing - 1 steps ahead in registers (16 bytes a lane and 1 KiB of tile);
 // one barrier a step.
+// What bounds it: the matrix unit and the instructions around it. 8 chunks of 512 tokens
+// after 4k, 28 query heads on 4 KV heads of 128 dims, bf16: 256 GFLOP in 320 us (800
+// TFLOP/s; 990 where the tiles fill the CUs evenly, here 896 of 128 rows on 512 places).
+// With the next step's scores beside the weights; one after the other 420 us.
 // ===========================================================================
 
 constexpr int kKv8ExtRing = 4;    // steps in registers, the one in use included
@@ -1194,9 +1202,21 @@ static int kv8_check_attn(const Kv8Pool *p, int32_t layer, float scale, uint32_t
 
 // ---- decode
 
-constexpr int kSplitWavesPerCu = 8;  // waves of a split launch
-constexpr int kSplitMinSteps = 4;    // steps of a piece, at least
-constexpr int kSeqSteps = 6;         // steps a wave of the seq kernel takes, at most
+// Waves of a split launch and steps of a piece, at least. Measured, 64 sequences of 1 to
+// 8k tokens (280 MB): 8 waves a CU 63.5 us, 7 the same, 12 (with a ring of 2, which
+// their registers allow) 65.9, 16 73.0; one sequence of 8k: 4 steps 16.3 us, 2 the
+// same, 8 18.6.
+constexpr int kSplitWavesPerCu = 8;
+constexpr int kSplitMinSteps = 4;
+
+// Steps of the longest context that a wave of the seq kernel may have to take; behind that
+// the split kernel. The seq kernel saves the scan and the merge, but its longest sequence
+// is on eight waves alone, and its workgroups are large. Measured at head_dim 128, 4 KV
+// heads, seq / split in us: 8 sequences of 1,024 tokens 12.4 / 15.4, 1,536 15.5 / 15.7,
+// 2,048 17.6 / 16.2; 64 of 1,024 16.8 / 26.8, 64 of 1 to 2,048 21.8 / 28.8, of 1 to
+// 3,200 29.1 / 35.3, all but one of 100 17.3 / 16.7 and 23.0 / 16.6; 256 of 512
+// 41.8 / 45.7, all but one of 100 34.8 / 26.8.
+static int kv8_seq_steps(int64_t wgs, int cus) { return 2 * wgs < cus ? 6 : wgs <= 2 * cus ? 10 : 0; }
 
 // Up to kSplitSeqs sequences (any number for pieces = 0, the seq kernel).
 static int launch_kv8_decode(const Kv8Pool *p, const Kv8Args &a, Kv8Dec &d, int64_t pieces, hipStream_t hs) {
@@ -1296,7 +1316,7 @@ extern "C" int mkv_kv8_decode_attention(mkv_kv8_pool *pool, int32_t layer, const
   const int64_t most = ((int64_t)max_ctx_len + kKv8Step - 1) / kKv8Step, heads = (int64_t)g.Hkv * nqc;
   int64_t pieces = 0;
   Kv8Ws ws;
-  if (most > kv8_seq_waves(g.D) * kSeqSteps) {
+  if (most > kv8_seq_waves(g.D) * kv8_seq_steps(heads * num_seqs, p->cus)) {
     if ((rc = kv8_ws_begin(p, d_workspace, workspace_bytes, hs, &ws))) return rc;
     // Two partials a piece; fewer pieces where there are no more steps, or the
     // workspace holds no more.
