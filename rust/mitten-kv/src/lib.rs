@@ -22,10 +22,12 @@
 //!   crates supply everything else through [`PagedModel`].
 //! * [`DeviceStatePool`]: the states of a hybrid model's linear-attention
 //!   layers, and [`add_rms_norm`], the residual + norm between layers.
+//! * [`DeviceKv8Pool`]: the K/V pool in 8 bits, twice the tokens in the same bytes.
 
 mod backend;
 mod error;
 mod host;
+mod kv8;
 mod pool;
 mod state;
 
@@ -34,5 +36,6 @@ pub use error::check;
 pub use host::{
     schedule_prefill_chunks, Appended, CopyQueue, HostBlockManager, PagedLifecycle, PoolView, PrefillSchedule,
 };
+pub use kv8::{DeviceKv8Pool, Preparation, Requests};
 pub use pool::{DeviceKvPool, KvDtype, PoolGeometry, SharedPrefix, Stream, Tables, PAGE_SIZE};
 pub use state::{add_rms_norm, DeviceStatePool, LinearIo, StateGeometry, STATE_NONE};

@@ -66,7 +66,7 @@ impl PoolGeometry {
         }
     }
 
-    fn desc(&self) -> sys::mkv_pool_desc {
+    pub(crate) fn desc(&self) -> sys::mkv_pool_desc {
         sys::mkv_pool_desc {
             num_layers: self.num_layers as i32,
             num_kv_heads: self.num_kv_heads as i32,
