@@ -737,8 +737,9 @@ MKV_API int mkv_kv8_decode_attention_host(mkv_kv8_pool *pool, int32_t layer, con
 MKV_API int mkv_kv8_workspace_size(const mkv_kv8_pool *pool, uint64_t *out_bytes);
 
 /* Causal attention of each sequence's newest tokens, as mkv_extend_attention, the
- * chunk's rows written before by an append. Few short chunks over long contexts
- * split their key ranges (two launches), with partials in the workspace as above. */
+ * chunk's rows written before by an append. Where few tiles of rows lie before long
+ * contexts (up to 512 sequences), their keys are cut into equal pieces (two launches),
+ * with partials in the workspace as above. */
 MKV_API int mkv_kv8_extend_attention(mkv_kv8_pool *pool, int32_t layer, const void *d_q, void *d_o,
                                      const int32_t *d_q_indptr, const int32_t *d_block_indptr,
                                      const int32_t *d_block_ids, const int32_t *d_ctx_lens, int32_t num_seqs,

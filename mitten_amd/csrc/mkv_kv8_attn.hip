@@ -731,20 +731,42 @@ kv8_decode_seq_kernel(Kv8Args a, Kv8Dec dc) {
 
 constexpr int kKv8ExtRing = 4;    // steps in registers, the one in use included
 constexpr int kKv8ExtIds = 1024;  // block ids staged in LDS at a time
+constexpr int kCutSeqs = 512;     // sequences of a cut launch
 
+// Two decompositions. Whole: a workgroup per (tile, KV head, sequence). Cut: the steps of
+// all tiles stand in one row (a tile's as many as its sequence has), cut into equal
+// pieces, as a decode launch's are; a tile that lies in one piece is stored at once, a
+// row of others has a partial per piece, numbered from the tile's first, and a second
+// launch merges them. Measured at 28 query heads on 4 KV heads of 128 dims, bf16, whole /
+// cut in us: 16 chunks of 8 tokens after 2k 48 / 35, after 8k 170 / 55; of 40 after 8k
+// 222 / 145; one of 200 after 30k 622 / 134. (16 chunks of 5 to 24 tokens after 4 to 8k
+// take 73, in equal shares of every tile 87: their workgroups fill the CUs 1.3 times.)
 struct Kv8Ext {
   const void *q;
   void *o;
   float *ws_ml, *ws_o;
-  int32_t max_ctx, tiles, splits;
+  int32_t max_ctx, rows, tiles;  // rows of a tile; tiles of the longest chunk
+  int32_t pieces, parts;         // of a cut launch; partials of a row, at most (1: whole)
   float sl2;
   int32_t zero_sink;
 };
+constexpr int kCutMinSteps = 4;  // steps of a piece, at least
 
-// Row tile t0 (rows t0 ..) of one sequence and KV head over its share sp of the keys.
+// Tiles of a chunk of n tokens, and steps of each.
+__device__ __forceinline__ int kv8_cut_tiles(const Kv8Args &a, const Kv8Ext &e, int n) {
+  return (int)(((int64_t)n * a.G + e.rows - 1) / e.rows);
+}
+__device__ __forceinline__ int kv8_cut_steps(int ctx) { return (int)(((int64_t)ctx + kKv8Step - 1) / kKv8Step); }
+// Steps of a piece, of `total`; no tile (of `longest` steps, at most) has more pieces than parts.
+__device__ __forceinline__ int kv8_cut_per(const Kv8Ext &e, int total, int longest) {
+  return max(kCutMinSteps, max((total + e.pieces - 1) / e.pieces, (longest + e.parts - 2) / (e.parts - 1)));
+}
+
+// Rows t0 .. of one sequence and KV head over the steps [s0, s1) of its keys: the whole
+// result, or partial `part`.
 template <int D, bool F32, int RT, int W>
 __device__ __forceinline__ void kv8_extend_tile(const Kv8Args &a, const Kv8Ext &e, const Kv8Seq &s, int h, int t0,
-                                                int sp) {
+                                                int s0, int s1, bool whole, int part) {
   constexpr int NR = D / 64, UNITS = 4 * NR;  // 1 KiB pieces of a step: (K | V, block, r)
   constexpr int LPL = UNITS / W;              // of them a wave loads
   static_assert(UNITS % W == 0, "every wave loads the same number of pieces");
@@ -760,8 +782,7 @@ __device__ __forceinline__ void kv8_extend_tile(const Kv8Args &a, const Kv8Ext &
   const int last = (int)min(rows, (int64_t)t0 + 16 * RT * W) - 1;  // the tile's last row
   const int qlo_wg = p0 + t0 / a.G, qhi_wg = p0 + last / a.G;
   const int steps_all = qhi_wg / kKv8Step + 1;
-  const int share = (steps_all + e.splits - 1) / e.splits;
-  const int st0 = min(sp * share, steps_all), st1 = min(st0 + share, steps_all);
+  const int st0 = min(s0, steps_all), st1 = min(s1, steps_all);
   const int nblk = qhi_wg / kPageSize + 1;
 
   int qp[RT], qlo[RT], row0[RT];
@@ -1071,8 +1092,8 @@ __device__ __forceinline__ void kv8_extend_tile(const Kv8Args &a, const Kv8Ext &
   for (int i = 0; i < RT; i++) {
     st[i].join();
     if (row0[i] + m16 < rows)
-      kv8_store<D, F32, !F32>(st[i], E, g4, e.splits == 1, e.o, qrow[i], e.ws_ml, e.ws_o, qrow[i] * e.splits + sp,
-                        e.zero_sink);
+      kv8_store<D, F32, !F32>(st[i], E, g4, whole, e.o, qrow[i], e.ws_ml, e.ws_o, qrow[i] * e.parts + part,
+                              e.zero_sink);
   }
   if (!odd) return;
   // NaN values of V behind the tile's first position, for the rows that see them.
@@ -1094,7 +1115,7 @@ __device__ __forceinline__ void kv8_extend_tile(const Kv8Args &a, const Kv8Ext &
 #pragma unroll
     for (int n = 0; n < 4; n++) {
       if (!(nan >> n & 1)) continue;
-      if (e.splits > 1) e.ws_o[(qr * e.splits + sp) * D + dim + n] = __uint_as_float(0x7fc00000u);
+      if (!whole) e.ws_o[(qr * e.parts + part) * D + dim + n] = __uint_as_float(0x7fc00000u);
       else if constexpr (F32) static_cast<float *>(e.o)[qr * D + dim + n] = __uint_as_float(0x7fc00000u);
       else static_cast<uint16_t *>(e.o)[qr * D + dim + n] = 0x7fc0;
     }
@@ -1104,47 +1125,137 @@ __device__ __forceinline__ void kv8_extend_tile(const Kv8Args &a, const Kv8Ext &
 template <int D, bool F32, int RT, int W>
 __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 256 && F32 ? 1 : 2, D == 256 && F32 ? 1 : 2)))
 kv8_extend_kernel(Kv8Args a, Kv8Ext e) {
-  // Tiles with the most keys first, every (KV head, sequence) in turn. Where
-  // their number is a multiple of the 8 XCDs, all tiles of a pair run on one and
-  // share its L2.
+  __shared__ int32_t pre[kCutSeqs + 1], longest_s;
   const int pairs = a.Hkv * a.B;
-  const int64_t L = blockIdx.x;
-  const int pair = (int)(L % pairs), sp = (int)(L / pairs) % e.splits, tr = (int)(L / ((int64_t)pairs * e.splits));
-  const int h = pair % a.Hkv, b = pair / a.Hkv;
+  const bool cut = e.parts > 1;
+  int b = 0, h = 0, u = 0, u1 = 0, per = 1, first = 0;
+  int64_t t = -1;
   Kv8Seq s;
-  const uint32_t err = kv8_seq(a, b, e.max_ctx, s);
-  if (err && L < pairs && h == 0 && threadIdx.x == 0) record_error(a.d_err, err);
-  if (err || s.n == 0) return;
-  const int64_t rows = (int64_t)s.n * a.G;
-  const int tile = 16 * RT * W;
-  // (A chunk longer than max_q_len takes further rounds.)
-  const int64_t mine = (rows + tile - 1) / tile;
-  for (int64_t t = mine - 1 - tr; t >= 0; t -= e.tiles) {
-    kv8_extend_tile<D, F32, RT, W>(a, e, s, h, (int)(t * tile), sp);
+  if (cut) {
+    for (int i = threadIdx.x; i < a.B; i += 64 * W) {
+      Kv8Seq x;
+      const uint32_t err = kv8_seq(a, i, e.max_ctx, x);
+      if (err && blockIdx.x == 0) record_error(a.d_err, err);
+      const bool none = err || x.n == 0;
+      pre[i + 1] = none ? 0 : a.Hkv * kv8_cut_tiles(a, e, x.n) * kv8_cut_steps(x.ctx);
+    }
+    if (threadIdx.x == 0) pre[0] = 0;
     __syncthreads();
+    if (threadIdx.x < 64) {
+      int at = 0, top = 0;
+      for (int i0 = 0; i0 < a.B; i0 += 64) {
+        const int i = i0 + (int)threadIdx.x;
+        int v = i < a.B ? pre[i + 1] : 0;
+        if (v > 0) top = max(top, kv8_cut_steps(a.ctx[i]));
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const int up = __shfl_up(v, o);
+          if ((int)threadIdx.x >= o) v += up;
+        }
+        if (i < a.B) pre[i + 1] = at + v;
+        at += __shfl(v, 63);
+      }
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) top = max(top, __shfl_xor(top, o));
+      if (threadIdx.x == 0) longest_s = top;
+    }
+    __syncthreads();
+    const int total = __builtin_amdgcn_readfirstlane(pre[a.B]);
+    per = kv8_cut_per(e, total, __builtin_amdgcn_readfirstlane(longest_s));
+    // Neighbours, which read the same keys for other rows, on one XCD.
+    const int x = blockIdx.x;
+    first = e.pieces % 8 ? x : x % 8 * (e.pieces / 8) + x / 8;
+    if ((int64_t)first * per >= total) return;
+    u = first * per;
+    u1 = min(total, u + per);
+  } else {
+    // Tiles with the most keys first, every (KV head, sequence) in turn. Where
+    // their number is a multiple of the 8 XCDs, all tiles of a pair run on one and
+    // share its L2.
+    const int64_t L = blockIdx.x;
+    const int pair = (int)(L % pairs);
+    h = pair % a.Hkv;
+    b = pair / a.Hkv;
+    const uint32_t err = kv8_seq(a, b, e.max_ctx, s);
+    if (err && L < pairs && h == 0 && threadIdx.x == 0) record_error(a.d_err, err);
+    if (err || s.n == 0) return;
+    // (A chunk longer than max_q_len takes further rounds.)
+    t = kv8_cut_tiles(a, e, s.n) - 1 - L / pairs;
+  }
+  while (cut ? u < u1 : t >= 0) {
+    int s0 = 0, s1 = INT32_MAX, part = 0;
+    bool whole = true;
+    if (cut) {
+      int lo = 0, hi = a.B;  // the last sequence that starts at or before u
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (__builtin_amdgcn_readfirstlane(pre[mid]) <= u) lo = mid;
+        else hi = mid;
+      }
+      (void)kv8_seq(a, lo, e.max_ctx, s);
+      const int steps = kv8_cut_steps(s.ctx), tiles = kv8_cut_tiles(a, e, s.n);
+      const int r = u - __builtin_amdgcn_readfirstlane(pre[lo]), ht = r / steps;
+      h = ht / tiles;
+      t = ht % tiles;
+      s0 = r - ht * steps;
+      s1 = min(steps, s0 + u1 - u);
+      whole = s0 == 0 && s1 == steps;
+      part = first - (u - s0) / per;
+      u += s1 - s0;
+    }
+    kv8_extend_tile<D, F32, RT, W>(a, e, s, h, (int)t * e.rows, s0, s1, whole, part);
+    __syncthreads();
+    if (!cut) t -= e.tiles;
   }
 }
 
-// The merge of split key ranges: a thread per 4 dims of a (token, query head) row of
+// The merge of a cut launch: a thread per 4 dims of a (token, query head) row of
 // sequence blockIdx.y.
 template <int D, bool F32>
 __global__ void __launch_bounds__(256) kv8_extend_merge_kernel(Kv8Args a, Kv8Ext e) {
   constexpr int TPR = D / 4;  // threads of a row
+  __shared__ int32_t part[4][3];
   Kv8Seq s;
+  int before = 0, total = 0, longest = 0;
+  for (int i = threadIdx.x; i < a.B; i += 256) {
+    if (kv8_seq(a, i, e.max_ctx, s) || s.n == 0) continue;
+    const int steps = kv8_cut_steps(s.ctx), n = a.Hkv * kv8_cut_tiles(a, e, s.n) * steps;
+    total += n;
+    before += i < (int)blockIdx.y ? n : 0;
+    longest = max(longest, steps);
+  }
+  before = wave_sum_int(before);
+  total = wave_sum_int(total);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) longest = max(longest, __shfl_xor(longest, o));
+  if (threadIdx.x % 64 == 0) {
+    int32_t *p = part[threadIdx.x / 64];
+    p[0] = before, p[1] = total, p[2] = longest;
+  }
+  __syncthreads();
+  before = part[0][0] + part[1][0] + part[2][0] + part[3][0];
+  total = part[0][1] + part[1][1] + part[2][1] + part[3][1];
+  longest = max(max(part[0][2], part[1][2]), max(part[2][2], part[3][2]));
   if (kv8_seq(a, blockIdx.y, e.max_ctx, s) || s.n == 0) return;
-  const int64_t rows = (int64_t)s.n * a.Hq, first = (int64_t)s.q0 * a.Hq;
+  const int per = kv8_cut_per(e, total, longest), steps = kv8_cut_steps(s.ctx), tiles = kv8_cut_tiles(a, e, s.n);
+  const int64_t rows = (int64_t)s.n * a.Hq;
   const int dim = 4 * (threadIdx.x % TPR);
   for (int64_t r = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR; r < rows; r += (int64_t)gridDim.x * (256 / TPR)) {
-    const int64_t at = (first + r) * e.splits;
+    const int pos = (int)(r / a.Hq), hq = (int)(r - (int64_t)pos * a.Hq), h = hq / a.G;
+    const int tile = (int)(((int64_t)pos * a.G + (hq - h * a.G)) / e.rows);
+    const int from = before + (h * tiles + tile) * steps;
+    const int parts = (from + steps - 1) / per - from / per + 1;
+    if (parts == 1) continue;  // stored already
+    const int64_t at = ((int64_t)s.q0 * a.Hq + r) * e.parts;
     float M = -FLT_MAX, L = 0.0f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     constexpr int N = 8;  // partials loaded at a time
-    for (int i0 = 0; i0 < e.splits; i0 += N) {
+    for (int i0 = 0; i0 < parts; i0 += N) {
       float2 y[N];
       f32x4 o[N];
 #pragma unroll
       for (int i = 0; i < N; i++) {  // (past the last partial: the last one, with no weight)
-        const int64_t c = at + min(i0 + i, e.splits - 1);
+        const int64_t c = at + min(i0 + i, parts - 1);
         y[i] = *reinterpret_cast<const float2 *>(e.ws_ml + 2 * c);
         o[i] = *reinterpret_cast<const f32x4 *>(e.ws_o + c * D + dim);
       }
@@ -1156,7 +1267,7 @@ __global__ void __launch_bounds__(256) kv8_extend_merge_kernel(Kv8Args a, Kv8Ext
       acc *= f;
 #pragma unroll
       for (int i = 0; i < N; i++) {
-        if (i0 + i >= e.splits) break;
+        if (i0 + i >= parts) break;
         const float w = fast_exp2(y[i].x - m);
         L = fmaf(y[i].y, w, L);
         acc += o[i] * w;
@@ -1164,7 +1275,7 @@ __global__ void __launch_bounds__(256) kv8_extend_merge_kernel(Kv8Args a, Kv8Ext
       M = m;
     }
     acc *= final_scale(M, L, e.zero_sink);
-    const int64_t out = (first + r) * D + dim;
+    const int64_t out = ((int64_t)s.q0 * a.Hq + r) * D + dim;
     if constexpr (F32) *reinterpret_cast<f32x4 *>(static_cast<float *>(e.o) + out) = acc;
     else
       *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(e.o) + out) =
@@ -1264,13 +1375,20 @@ static Kv8ExtForm kv8_ext_form(const Geom &g, bool wide) {
 #undef KV8_EXT
 }
 
-// What a call takes, by that: `tiles` workgroups' worth of rows over `steps` each, in
-// `splits` shares; a merge is a launch and its partials' bytes both ways.
-static double kv8_ext_cost(const Kv8ExtForm &f, double cus, double tiles, double steps, int splits, double values) {
-  const double wgs = tiles * splits / cus;
+// What a call takes, by that: `tiles` tiles of `steps` each. Whole: in rounds of what the
+// CUs hold. Cut: in equal pieces, started twice each, and the merge: a launch, and the
+// partials' bytes both ways.
+static double kv8_ext_whole(const Kv8ExtForm &f, double cus, double tiles, double steps) {
+  const double wgs = tiles / cus;
   double step = f.alone;
   if (wgs > 1) step = f.beside > 0 ? std::max(f.beside, f.beside * std::ceil(wgs) / 2) : f.alone * std::ceil(wgs);
-  return std::ceil(steps / splits) * step + 3.0 + (splits > 1 ? 5.0 + values * splits * 8 / 5.0e6 : 0.0);
+  return steps * step + 3.0;
+}
+static int kv8_ext_slots(const Kv8ExtForm &f, int cus) { return f.beside > 0 ? 2 * cus : cus; }
+static double kv8_ext_cut(const Kv8ExtForm &f, int cus, double tiles, double steps, int parts, double values) {
+  const double per = std::max({(double)kCutMinSteps, tiles * steps / kv8_ext_slots(f, cus), steps / (parts - 1)});
+  const double step = f.beside > 0 && tiles * steps / per > cus ? f.beside : f.alone;
+  return per * step + 6.0 + 6.0 + values * (steps / per + 1) * 8 / 5.0e6;
 }
 
 }  // namespace mkv
@@ -1392,48 +1510,53 @@ extern "C" int mkv_kv8_extend_attention(mkv_kv8_pool *pool, int32_t layer, const
   e.q = d_q;
   e.o = d_o;
   e.max_ctx = max_ctx_len;
-  e.splits = 1;
   e.sl2 = scale * kLog2e;
   e.zero_sink = (flags & MKV_ATTN_ZERO_SINK) ? 1 : 0;
   const int64_t pairs = (int64_t)g.Hkv * num_seqs, rows = (int64_t)std::min(max_q_len, num_tokens) * a.G;
   if ((int64_t)num_tokens * a.G > INT32_MAX / 2) return set_error(MKV_ERR_INVALID_ARGUMENT, "too many tokens");
-  // The form and the split of the key ranges that cost least, for sequences of the mean
-  // length of a chunk and the longest context. At most 32 shares of at least 4 steps,
-  // and no more than the workspace holds the partials of.
+  // The form and the decomposition that cost least, for chunks of the mean length (of
+  // many lengths: half a tile more) and the longest context. A row has at most 32
+  // partials, and no more than the workspace holds of all rows.
   const double mean = std::max(1.0, std::min<double>((double)rows, (double)num_tokens * a.G / num_seqs));
+  auto tiles_of = [&](int n) {
+    const double most = std::ceil((double)rows / n);
+    return mean >= (double)rows ? most : std::max(1.0, std::min(most, mean / n + 0.5));
+  };
   const int64_t steps = ((int64_t)max_ctx_len + kKv8Step - 1) / kKv8Step;
-  const uint64_t per = (uint64_t)num_tokens * g.Hq * (8 + 4 * g.D);
+  const uint64_t row = (uint64_t)num_tokens * g.Hq * (8 + 4 * g.D);
   const uint64_t bytes = d_workspace ? workspace_bytes : kKv8Workspace, room = bytes > 256 ? bytes - 256 : 0;
-  const int most = (int)std::max<int64_t>(1, std::min({steps / 4, (int64_t)32, (int64_t)(room / per)}));
+  const int parts = (int)std::min<uint64_t>(room / row, 32);
   Kv8ExtForm form{};
   double best = INFINITY;
+  e.parts = 1;
   for (int narrow = 0; narrow < 2; narrow++) {
     const Kv8ExtForm f = kv8_ext_form(g, !narrow);
-    for (int sp = 1; sp <= most; sp++) {
-      const double c = kv8_ext_cost(f, p->cus, (double)pairs * std::ceil(mean / f.rows), (double)steps, sp,
-                                    (double)num_tokens * g.Hq * g.D);
-      if (c < 0.97 * best) {  // (equal costs: the wide form, fewer shares)
-        best = c;
-        form = f;
-        e.splits = sp;
-      }
-    }
+    const double tiles = (double)pairs * tiles_of(f.rows);
+    // (Units are 32-bit, also where the chunks' rows overlap.)
+    const double most = (double)pairs * std::ceil((double)num_tokens * a.G / f.rows) * (double)steps;
+    double c = kv8_ext_whole(f, p->cus, tiles, (double)steps);
+    if (c < best) best = c, form = f, e.parts = 1;
+    if (parts < 2 || num_seqs > kCutSeqs || most > INT32_MAX / 2) continue;
+    c = kv8_ext_cut(f, p->cus, tiles, (double)steps, parts, (double)num_tokens * g.Hq * g.D);
+    if (c < best) best = c, form = f, e.parts = parts;
   }
+  e.rows = form.rows;
   const int64_t tiles = (rows + form.rows - 1) / form.rows;
+  int64_t grid = tiles * pairs;
   Kv8Ws ws;
-  if (e.splits > 1) {
+  if (e.parts > 1) {
     if ((rc = kv8_ws_begin(p, d_workspace, workspace_bytes, hs, &ws))) return rc;
     e.ws_ml = static_cast<float *>(ws.ptr);
-    e.ws_o = reinterpret_cast<float *>(static_cast<uint8_t *>(ws.ptr) +
-                                       kv8_ml_bytes((uint64_t)num_tokens * g.Hq * e.splits));
+    e.ws_o = reinterpret_cast<float *>(static_cast<uint8_t *>(ws.ptr) + kv8_ml_bytes((uint64_t)num_tokens * g.Hq * e.parts));
+    e.pieces = kv8_ext_slots(form, p->cus);
+    grid = e.pieces;
   }
-  const int64_t grid = tiles * pairs * e.splits;
-  if (grid > INT32_MAX || tiles > INT32_MAX) return set_error(MKV_ERR_INVALID_ARGUMENT, "grid too large");
+  if (grid > INT32_MAX) return set_error(MKV_ERR_INVALID_ARGUMENT, "grid too large");
   e.tiles = (int32_t)tiles;
   void *args[] = {&a, &e};
   MKV_CHECK_HIP(hipLaunchKernel(form.fn, dim3((unsigned)grid), dim3(64 * form.waves), args, 0, hs));
   MKV_CHECK_LAUNCH("kv8_extend_kernel");
-  if (e.splits > 1) {
+  if (e.parts > 1) {
     const int64_t per = 1024 / g.D, wgs = ((int64_t)std::min(max_q_len, num_tokens) * g.Hq + per - 1) / per;
     const dim3 mgrid((unsigned)std::min<int64_t>(wgs, 1 << 20), (unsigned)num_seqs);
     KV8_LAUNCH(kv8_extend_merge_kernel, mgrid, dim3(256), 0, a, e);
