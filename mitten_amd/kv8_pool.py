@@ -196,6 +196,8 @@ class DeviceKv8Pool:
     def _form(self, block_indptr, block_ids, ctx_lens, q_lens=None):
         """Whether the metadata is the host's; all of it has to be, or none."""
         tensor = self._tensor
+        if isinstance(ctx_lens, tensor) and ctx_lens.is_cuda:
+            return False  # (the others are checked one by one)
         host = None
         for x in (ctx_lens, block_indptr, block_ids, q_lens):
             if x is None and x is q_lens:
@@ -351,9 +353,10 @@ class DeviceKv8Pool:
         for t, name in ((out_k, "out_k"), (out_v, "out_v")):
             if t is None:
                 t = _empty_on(stream, n, self._dtype, self._device)
-            _check(t, self.device, None, self._dtype, name)
-            if t.numel() < n:
-                raise _bad(f"{name} is too small")
+            else:
+                _check(t, self.device, None, self._dtype, name)
+                if t.numel() < n:
+                    raise _bad(f"{name} is too small")
             outs.append(t)
         if n == 0:
             return tuple(outs)
