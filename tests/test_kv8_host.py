@@ -78,3 +78,91 @@ def test_stretched_frequencies():
         kw.update(bad)
         with pytest.raises(ValueError):
             rope_scaled_inv_freq(**kw)
+
+
+def small_pool():
+    r = np.random.default_rng(5)
+    o = kv8.Kv8(9, 2, 64)
+    tables = [[3, 0, 7], [8, 1], [5]]
+    ctx, n = [40, 17, 3], [40, 17, 3]
+    k, v = (r.standard_normal((60, 2, 64)) * 2.0 ** r.integers(-3, 4, (60, 1, 1)) for _ in range(2))
+    o.append(k, v, n, ctx, tables)
+    return o, tables, ctx, k, v
+
+
+def test_oracle_appends_to_half_a_step():
+    o, tables, ctx, k, v = small_pool()
+    at = 0
+    for t, c in zip(tables, ctx):
+        for kv, x in enumerate((k, v)):
+            y = x[at: at + c].transpose(1, 0, 2)
+            e = o.exp[kv][t].repeat(16, 0)[:c].T[..., None]
+            assert np.all(np.abs(o.rows(kv, t, c) - y) <= np.maximum(np.abs(y) * 2.0 ** -4, 2.0 ** (e - 10.0)))
+        at += c
+    # A larger row raises its tile's exponent; the others move by less than half a step of it.
+    before, e0 = o.rows(0, tables[1], 17), int(o.exp[0, 1, 0])
+    big = np.full((1, 2, 64), 3000.0)
+    o.append(big, big, [1], [18], [tables[1]])
+    e = int(o.exp[0, 1, 0])
+    assert e > e0 and 224 * 2.0 ** e < 3000 <= 448 * 2.0 ** e
+    after = o.rows(0, tables[1], 18)
+    assert np.all(np.abs(after[0, 16] - before[0, 16]) <= np.maximum(np.abs(before[0, 16]) * 2.0 ** -4, 2.0 ** (e - 10)))
+    assert np.array_equal(after[:, :16], before[:, :16]) and np.all(after[:, 17] == kv8.to_e4m3(3000 * 2.0 ** -e) * 2.0 ** e)
+
+
+@pytest.mark.parametrize("sink", [False, True])
+def test_oracle_attention(sink):
+    import torch
+
+    o, tables, ctx, _, _ = small_pool()
+    new = [5, 17, 0]
+    q = np.random.default_rng(6).standard_normal((22, 6, 64))
+    got = o.attend(q, new, ctx, tables, 0.125, sink)[0]
+    at = 0
+    for n, c, t in zip(new, ctx, tables):
+        if n == 0:
+            continue
+        k, v = (torch.from_numpy(o.rows(kv, t, c)).repeat_interleave(3, 0) for kv in range(2))
+        mask = torch.ones(n, c, dtype=torch.bool).tril(c - n)
+        if sink:  # a key of zeros with values of zeros that every row sees
+            k, v = (torch.nn.functional.pad(x, (0, 0, 1, 0)) for x in (k, v))
+            mask = torch.nn.functional.pad(mask, (1, 0), value=True)
+        want = torch.nn.functional.scaled_dot_product_attention(
+            torch.from_numpy(q[at: at + n]).transpose(0, 1), k, v, attn_mask=mask, scale=0.125)
+        assert np.allclose(got[at: at + n], want.transpose(0, 1).numpy(), rtol=1e-12, atol=1e-13)
+        at += n
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_oracle_rotation(interleaved):
+    r = np.random.default_rng(7)
+    x, w, pos = r.standard_normal((4, 3, 64)), r.standard_normal(64), np.array([0, 1, 77, 2_000_000])
+    f = rope_inv_freq(32, 1e4)
+    y = kv8.norm_rope(x, w, 1e-6, f, pos, 1.5, interleaved)
+    z = x / np.sqrt((x * x).mean(-1, keepdims=True) + 1e-6) * (1 + w)
+    c = z[..., :32].reshape(4, 3, 16, 2) if interleaved else np.stack([z[..., :16], z[..., 16:32]], -1)
+    turned = (c[..., 0] + 1j * c[..., 1]) * 1.5 * np.exp(1j * pos[:, None, None] * f.astype(np.float64))
+    assert np.allclose(y[..., 32:], z[..., 32:], rtol=1e-14)
+    a, b = (y[..., 0:32:2], y[..., 1:32:2]) if interleaved else (y[..., :16], y[..., 16:32])
+    assert np.allclose(a, turned.real, atol=1e-9) and np.allclose(b, turned.imag, atol=1e-9)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_tolerances_see_mistakes(dtype):
+    """The rounded exact result passes; a lost token, another head's keys, an exponent off by
+    one, or a dropped scale do not."""
+    from kv8_helpers import assert_attention, values
+
+    o, tables, ctx, _, _ = small_pool()
+    new, q = [1, 1, 1], np.random.default_rng(8).standard_normal((3, 6, 64))
+    want = o.attend(q, new, ctx, tables, 0.125)
+    assert_attention(values(want[0], dtype), want, dtype)
+    heads = kv8.Kv8(9, 2, 64)
+    heads.val, heads.exp = o.val[:, :, ::-1], o.exp[:, :, ::-1]
+    off = kv8.Kv8(9, 2, 64)
+    off.val, off.exp = o.val, o.exp.copy()
+    off.exp[1, 0] += 1
+    for bad in (o.attend(q, new, [39, 17, 3], tables, 0.125)[0], heads.attend(q, new, ctx, tables, 0.125)[0],
+                off.attend(q, new, ctx, tables, 0.125)[0], o.attend(q, new, ctx, tables, 0.13)[0]):
+        with pytest.raises(AssertionError):
+            assert_attention(values(bad, dtype), want, dtype)
