@@ -1,4 +1,4 @@
-"""The 8-bit K/V pool's operators in 64 bits, in numpy: the checker of the mkv_kv8_* calls.
+"""The 8-bit K/V pool's operators in 64 bits, in numpy: the oracle of the mkv_kv8_* calls.
 
 TEST INFRASTRUCTURE ONLY, as oracle.py. Rows are float64 arrays holding the values of
 the f32 / bf16 inputs; tiles are e4m3 values (float64) and exponents.

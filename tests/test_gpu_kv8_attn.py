@@ -328,6 +328,92 @@ def test_extend_runs_of_ids():
         assert_attention(host(pool.extend_attention(0, dev(q, "bf16"), new, *b.host())), ref, "bf16")
 
 
+@pytest.mark.parametrize("count", [65, 130, 512, 513])
+def test_extend_short_chunks_of_many_sequences(count):
+    """Keys cut into pieces over more sequences than a wave scans at once, up to the most (and
+    one more, uncut); some without new tokens, some bad."""
+    import torch
+
+    r = np.random.default_rng(count)
+    ctx = r.integers(1, 2500, count)
+    new = np.minimum(r.integers(0, 4, count), ctx)
+    b = Batch(new.tolist(), ctx.tolist())
+    with make_pool(b, 1, 2, 64, "bf16") as pool:
+        want = fill(pool, 3)
+        q = randn(4, (b.tokens, 2, 64), "bf16")
+        lens = ctx.copy()
+        bad = [i for i in (3, 64, count - 1) if new[i]]
+        lens[bad] = 3000  # (more than the tables hold)
+        at = np.concatenate([[0], np.cumsum(new)])
+        ref = want.attend(q, b.new, b.ctx, b.tables, 0.125)
+        for own in (None, torch.empty(0, dtype=torch.uint8, device="cuda")):
+            out = torch.full((b.tokens, 2, 64), 7.0, device="cuda", dtype=torch.bfloat16)
+            pool.extend_attention(0, dev(q, "bf16"), b.q_indptr(), dev(b.indptr), dev(b.ids), dev(lens), max_q_len=3,
+                                  max_ctx_len=3000, out=out, workspace=own)
+            if bad:  # (none of the three has new tokens where there are 65)
+                with pytest.raises(DeviceIndexError) as ei:
+                    pool.check()
+                assert ei.value.bits == TABLE
+            pool.check()
+            y = host(out)
+            for i in bad:
+                assert np.all(y[at[i]: at[i + 1]] == 7.0)
+                y[at[i]: at[i + 1]] = ref[0][at[i]: at[i + 1]]
+            assert_attention(y, ref, "bf16")
+
+
+def test_bounds_far_above_the_lengths():
+    """The largest max_ctx_len and max_q_len: sizes of launches, not of what they do."""
+    top = 2 ** 31 - 1
+    ctx = [40, 700, 3]
+    b = Batch([9, 20, 3], ctx)
+    with make_pool(b, 2, 4, 64, "f32") as pool:
+        want = fill(pool, 1)
+        k, v = randn(1, (32, 2, 64), "f32"), randn(2, (32, 2, 64), "f32")
+        q = randn(3, (32, 8, 64), "f32")
+        pool.append(0, dev(k, "f32"), dev(v, "f32"), b.q_indptr(), *b.device(), max_q_len=top)
+        want.append(k, v, b.new, ctx, b.tables)
+        assert_same(pool, want)
+        for most in (100_000, top):
+            o = pool.extend_attention(0, dev(q, "f32"), b.q_indptr(), *b.device(), max_q_len=most, max_ctx_len=most)
+            assert_attention(host(o), want.attend(q, b.new, ctx, b.tables, 0.125), "f32")
+            o = pool.decode_attention(0, dev(q[:3], "f32"), *b.device(), max_ctx_len=most)
+            assert_attention(host(o), want.attend(q[:3], [1] * 3, ctx, b.tables, 0.125), "f32")
+        out = pool.gather(0, *b.device(), max_ctx_len=top, total_tokens=sum(ctx))
+        assert np.array_equal(host(out[0]), np.concatenate([want.rows(0, t, c).ravel() for t, c in zip(b.tables, ctx)]))
+        pool.check()
+
+
+def test_nothing_to_do():
+    """No sequences, no tokens, padding alone."""
+    import torch
+
+    b = Batch([0, 0], [0, 0], spare=1)
+    with make_pool(b, 2, 4, 64, "bf16") as pool:
+        want = fill(pool, 1)
+        none = dev(np.zeros((0, 2, 64)), "bf16")
+        qn = dev(np.zeros((0, 8, 64)), "bf16")
+        i0, i1 = dev([]), dev([0])
+        pool.append(0, none, none, [], [0], [], [])
+        pool.append(0, none, none, i1, i1, i0, i0, max_q_len=0)
+        pool.append(0, none, none, [0, 0], *b.host())
+        pool.append(0, none, none, b.q_indptr(), *b.device(), max_q_len=5)
+        pool.qk_norm_rope_append(0, qn, none, none, [0, 0], *b.host(), gated=False)
+        assert pool.decode_step(0, none, none, qn, [0], [], []).shape == (0, 8, 64)
+        assert pool.extend_attention(0, qn, [], [0], [], []).shape == (0, 8, 64)
+        assert pool.extend_attention(0, qn, b.q_indptr(), *b.device(), max_q_len=3, max_ctx_len=900).shape == (0, 8, 64)
+        assert pool.gather(0, [0], [], [])[0].numel() == 0
+        assert pool.gather(0, *b.device(), max_ctx_len=50, total_tokens=0)[1].numel() == 0
+        q, k = dev(randn(1, (2, 8, 64), "bf16"), "bf16"), dev(randn(1, (2, 2, 64), "bf16"), "bf16")
+        for most in (0, 40, 5000):
+            out = torch.full((2, 8, 64), 7.0, device="cuda", dtype=torch.bfloat16)
+            pool.decode_step(0, k, k, q, *b.device(), max_ctx_len=most, out=out)
+            assert bool((out == 0).all())
+        assert bool((pool.decode_step(0, k, k, q, *b.host()) == 0).all())
+        pool.check()
+        assert_same(pool, want)
+
+
 # -- refusals ---------------------------------------------------------------------------
 
 
@@ -478,6 +564,44 @@ def test_two_streams_share_the_pool():
         for i in range(2):
             for o in outs[i]:
                 assert torch.equal(o, want[i])
+
+
+def test_two_graphs_with_a_workspace_each():
+    """Replayed at the same time on two streams."""
+    import torch
+
+    ctx = [3000, 2500]
+    b, e = Batch([1, 1], ctx), Batch([4, 3], ctx)
+    hkv, g, d = 4, 7, 128
+    with make_pool(b, hkv, g, d, "bf16") as pool:
+        fill(pool, 1)
+        t, qi = b.device(), e.q_indptr()
+        qs = [dev(randn(i, (2, hkv * g, d), "bf16"), "bf16") for i in range(2)]
+        qe = [dev(randn(i, (7, hkv * g, d), "bf16"), "bf16") for i in range(2)]
+        want = [(pool.decode_attention(0, qs[i], *t, max_ctx_len=3000),
+                 pool.extend_attention(0, qe[i], qi, *t, max_q_len=4, max_ctx_len=3000)) for i in range(2)]
+        outs = [(torch.zeros_like(qs[i]), torch.zeros_like(qe[i])) for i in range(2)]
+        graphs = []
+        torch.cuda.synchronize()
+        for i in range(2):
+            ws = torch.empty(pool.workspace_size(), dtype=torch.uint8, device="cuda")
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                pool.decode_attention(0, qs[i], *t, max_ctx_len=3000, out=outs[i][0], workspace=ws)
+                pool.extend_attention(0, qe[i], qi, *t, max_q_len=4, max_ctx_len=3000, out=outs[i][1], workspace=ws)
+            graphs.append((graph, torch.cuda.Stream(), ws))
+        for _ in range(4):
+            for x in outs:
+                for y in x:
+                    y.fill_(9.0)
+            torch.cuda.synchronize()
+            for _ in range(5):
+                for graph, stream, _ws in graphs:
+                    with torch.cuda.stream(stream):
+                        graph.replay()
+            torch.cuda.synchronize()
+            for got, ref in zip(outs, want):
+                assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
 
 
 def test_results_given_to_a_stream():
