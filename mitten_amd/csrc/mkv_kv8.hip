@@ -74,8 +74,8 @@ struct Kv8PrepArgs {
 // token that rotate against each other (half layout: dims i.. and i + rd/2..;
 // interleaved, and dims that do not rotate: 2 VEC neighbours), so that the
 // partner is always in the lane. A K head goes from there into its tile. Bound by
-// memory: 32 chunks of 512 tokens, 285 MB in 73 us (3.9 TB/s), of which the angles'
-// f64 and the norms hide some loads (86 us with no head loaded ahead).
+// memory: 32 chunks of 512 tokens, 285 MB in 72 us (4.0 TB/s; 86 us with no head
+// loaded ahead). Without the angles it took 71.
 // VEC: 8, or 4 where rd/2 (interleaved: rd/2) is not a multiple of 8.
 template <int D, int VEC>
 struct PrepLane {
