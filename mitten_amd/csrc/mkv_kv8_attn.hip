@@ -34,6 +34,8 @@ constexpr int kFarExp = 40;
 // small weights could be missed, and l is summed from the f32 weights.
 constexpr int kSumExp = 4;
 constexpr int kNoExp = -1000;
+// A row has at most 2^kPartBits partials (a CU has 8 pieces of a decode launch, at most).
+constexpr int kPartBits = 12;
 
 template <int D, bool F32>
 struct Kv8Q {
@@ -220,20 +222,25 @@ __device__ __forceinline__ void kv8_far(const int (&far)[2], f16x8 &p) {
   p *= f16x8{f0, f0, f0, f0, f1, f1, f1, f1};
 }
 
-// A finished row: the result, or its partial (m, l, O) for a merge.
+// A finished row: the result 2^E O / l, or its partial (m, l, o) for a merge, the row's
+// weights 2^m l and o / l their mean. A partial is kept where no merge leaves f32: l's
+// power of two is moved to m, so that l < 2^-kPartBits and o is below 2^-kPartBits of the
+// greatest V, and up to 2^kPartBits partials add up to less than that V. (2^E O alone passes
+// f32 from V of 2^121 on for one key, 2^108 for thousands.) All by exact powers of two.
 template <int D, bool F32, bool SUMS>
 __device__ __forceinline__ void kv8_store(const Kv8State<D, SUMS> &st, int E, int g4, bool final, void *o, int64_t row,
                                           float *ws_ml, float *ws_o, int64_t prow, int32_t zero_sink) {
   const float m = st.R - kBias;
-  float f = E == kNoExp ? 0.0f : __builtin_ldexpf(1.0f, E);
-  if (final) f *= final_scale(m, st.sum(), zero_sink);
+  const int up = __builtin_amdgcn_frexp_expf(st.sum()) + kPartBits;  // (0, infinity and NaN: kPartBits)
+  const int x = final ? E : E - up;
+  const float f = final ? final_scale(m, st.sum(), zero_sink) : 1.0f;
 #pragma unroll
   for (int i = 0; i < D / 64; i++) {
     float y[16];
 #pragma unroll
     for (int c = 0; c < 4; c++)
 #pragma unroll
-      for (int n = 0; n < 4; n++) y[4 * c + n] = st.O[i][n][c] * f;
+      for (int n = 0; n < 4; n++) y[4 * c + n] = __builtin_ldexpf(st.O[i][n][c] * f, x);
     const int64_t at = (final ? row : prow) * D + 64 * i + 16 * g4;
     if (final && !F32) {
 #pragma unroll
@@ -247,7 +254,8 @@ __device__ __forceinline__ void kv8_store(const Kv8State<D, SUMS> &st, int E, in
       for (int z = 0; z < 4; z++) p[z] = f32x4{y[4 * z], y[4 * z + 1], y[4 * z + 2], y[4 * z + 3]};
     }
   }
-  if (!final && g4 == 0) *reinterpret_cast<float2 *>(ws_ml + 2 * prow) = make_float2(m, st.sum());
+  if (!final && g4 == 0)
+    *reinterpret_cast<float2 *>(ws_ml + 2 * prow) = make_float2(m + (float)up, __builtin_ldexpf(st.sum(), -up));
 }
 
 // ===========================================================================
