@@ -9,8 +9,10 @@
 // (8 + 8 + 8 bits), so the products are exact and the sums f32.
 // O^T = V^T.P^T runs on v_mfma_f32_16x16x32_f16: a byte is exact in f16, and the
 // weight carries the tile's exponent: with E the greatest ev so far and d = ev - E,
-//   p_j = 2^(s_j + d - R),  O = sum_j p_j v'_j,  l = sum_j 2^-d p_j,  o = 2^E O / l,
+//   p_j = 2^(s_j + d - R),  O = sum_j p_j v'_j,  l = sum_j 2^(s_j - R - c),  o = 2^(E - c) O / l,
 // R a running maximum of s_j + d (moved when one passes it by more than kRescaleSlack).
+// c is 0 and l = sum_j 2^-d p_j, but where scales lie so far apart (a tile of zeros, by
+// whose score no other is seen in l) that l relative to R would leave f32.
 // p is f16 with 11 bits where it matters: it is held times 2^kBias, so at most
 // 2^15, and a weight 2^-21 below the greatest is still a normal number. (In bf16 its
 // 8 bits would add as much error as the rounding of a bf16 result, 1.41 of it
@@ -27,15 +29,13 @@ namespace mkv {
 
 constexpr float kBias = 15.0f - kRescaleSlack;
 constexpr int kMaxRaise = 40;
-// d, at least: what a tile lies below that is taken from its weights after l is summed.
+// A tile with d below that of -kFarExp is summed into l from its scores: 2^-d p_j could leave f32.
 constexpr int kFarExp = 40;
 // The matrix unit sums the rounded weights of tiles with d >= -kSumExp: what f16 drops
 // of one is below 2^-32 of the greatest s + d, 2^-28 of l. Behind that a long row of
 // small weights could be missed, and l is summed from the f32 weights.
 constexpr int kSumExp = 4;
 constexpr int kNoExp = -1000;
-// A row has at most 2^kPartBits partials (a CU has 8 pieces of a decode launch, at most).
-constexpr int kPartBits = 12;
 
 template <int D, bool F32>
 struct Kv8Q {
@@ -95,7 +95,7 @@ template <int D, bool SUMS = false>
 struct Kv8State {
   typedef typename std::conditional<SUMS, f32x4, float>::type sum_t;
   f32x4 O[D / 64][4];
-  float R;
+  float R, c;  // (the four lanes of a row hold the same)
   sum_t l;
   __device__ __forceinline__ float sum() const {
     if constexpr (SUMS) return l[0];
@@ -113,6 +113,7 @@ struct Kv8State {
 #pragma unroll
       for (int n = 0; n < 4; n++) O[i][n] = f32x4{0.f, 0.f, 0.f, 0.f};
     R = -FLT_MAX;  // (finite: no difference of two of them is NaN)
+    c = 0.0f;
     l = sum_t{};
   }
   __device__ __forceinline__ void scale_o(float f) {
@@ -121,34 +122,43 @@ struct Kv8State {
 #pragma unroll
       for (int n = 0; n < 4; n++) O[i][n] *= f;
   }
-  // E grows by de: s + d falls by it, so R follows and O stays; l is relative to
-  // R alone. (Steps past 2^40, or an l about to leave f32, move O instead.)
-  __device__ __forceinline__ void raise(int de) {
-    const int dc = __ballot(sum() > 0x1p60f) ? 0 : min(de, kMaxRaise);
-    R -= (float)dc;
-    l *= __builtin_ldexpf(1.0f, dc);
-    if (dc != de) scale_o(__builtin_ldexpf(1.0f, dc - de));
+  // E grows by de: s + d and R fall by it, O stays. l goes with R as far as f32 allows
+  // (2^40 at a time, and not from 2^60 on); the rest stands in c. Whether it does.
+  __device__ __forceinline__ bool raise(int de) {
+    const int dl = __ballot(sum() > 0x1p60f) ? 0 : min(de, kMaxRaise);
+    R -= (float)de;
+    c += (float)(de - dl);
+    l *= __builtin_ldexpf(1.0f, dl);
+    return dl != de;
   }
 };
 
-// Exponents of a step's two tiles against E: d >= -kFarExp, and what is left of
-// ev - E beyond that.
-__device__ __forceinline__ void kv8_offsets(int E, int ev0, int ev1, int (&d)[2], int (&far)[2]) {
-  d[0] = max(ev0 - E, -kFarExp);
-  d[1] = max(ev1 - E, -kFarExp);
-  far[0] = ev0 - E - d[0];
-  far[1] = ev1 - E - d[1];
+// The scale of a wave's state: E, and whether some row's l is apart from its R (c is not 0).
+struct Kv8Scale {
+  int E;
+  bool apart;
+  __device__ __forceinline__ void reset() {
+    E = kNoExp;
+    apart = false;
+  }
+};
+
+// d of a step's two tiles. (Only a reference, E, stands between a row and tiles that it
+// does not see: R follows s + d of the keys that it does.)
+__device__ __forceinline__ void kv8_offsets(int E, int ev0, int ev1, int (&d)[2]) {
+  d[0] = ev0 - E;
+  d[1] = ev1 - E;
 }
 
 // E for a step with tile exponents ev: raised where needed.
 template <int D, bool SUMS, int RT>
-__device__ __forceinline__ void kv8_raise(int &E, int ev0, int ev1, Kv8State<D, SUMS> (&st)[RT]) {
+__device__ __forceinline__ void kv8_raise(Kv8Scale &sc, int ev0, int ev1, Kv8State<D, SUMS> (&st)[RT]) {
   const int top = max(ev0, ev1);
-  if (top <= E) return;
-  if (E != kNoExp)
+  if (top <= sc.E) return;
+  if (sc.E != kNoExp)
 #pragma unroll
-    for (int i = 0; i < RT; i++) st[i].raise(top - E);
-  E = top;
+    for (int i = 0; i < RT; i++) sc.apart |= st[i].raise(top - sc.E);
+  sc.E = top;
 }
 
 // The greatest s + d of this lane's scores S (hidden keys -inf).
@@ -158,22 +168,39 @@ __device__ __forceinline__ float kv8_top(const float (&S)[2][4], float sl2, cons
   return fmaxf(fmaf(a, sl2, (float)d[0]), fmaf(b, sl2, (float)d[1]));
 }
 
-// R for a step whose greatest s + d in this lane is top.
+// R for a step whose greatest s + d in this lane is top. R + c moves only where R passes it.
 template <int D, bool SUMS>
 __device__ __forceinline__ void kv8_rescale(float top, Kv8State<D, SUMS> &st) {
   top = fmaxf(top, __shfl_xor(top, 16));
   top = fmaxf(top, __shfl_xor(top, 32));
   const float R = top > st.R + kRescaleSlack ? top : st.R;
-  const float f = fast_exp2(st.R - R);
-  st.l *= f;
-  st.scale_o(f);
+  const float up = R - st.R;
+  st.l *= fast_exp2(fminf(st.c - up, 0.0f));
+  st.c = fmaxf(st.c - up, 0.0f);
+  st.scale_o(fast_exp2(-up));
   st.R = R;
+}
+template <int D, bool SUMS, int RT>
+__device__ __forceinline__ void kv8_rescale_all(const float (&top)[RT], Kv8Scale &sc, Kv8State<D, SUMS> (&st)[RT]) {
+  bool apart = false;
+#pragma unroll
+  for (int i = 0; i < RT; i++) {
+    kv8_rescale(top[i], st[i]);
+    apart |= st[i].c != 0.0f;
+  }
+  sc.apart = __ballot(apart) != 0;
+}
+
+// Whether l takes a tile's weights by kv8_sum_low.
+template <bool SUMS>
+__device__ __forceinline__ bool kv8_low(int d, bool apart) {
+  return d < -(SUMS ? kSumExp : kFarExp) || apart;
 }
 
 // The weights of two blocks: operands of the PV product in p (and the second part of
-// f32 rows in p2), their sums in l but with SUMS.
+// f32 rows in p2), their sums in l but with SUMS and of low tiles.
 template <int D, bool F32, bool SUMS>
-__device__ __forceinline__ void kv8_weights(const float (&S)[2][4], float sl2, const int (&d)[2],
+__device__ __forceinline__ void kv8_weights(const float (&S)[2][4], float sl2, const int (&d)[2], bool apart,
                                             Kv8State<D, SUMS> &st, f16x8 &p, f16x8 &p2) {
 #pragma unroll
   for (int kb = 0; kb < 2; kb++) {
@@ -186,54 +213,101 @@ __device__ __forceinline__ void kv8_weights(const float (&S)[2][4], float sl2, c
       p[4 * kb + i] = h;
       if constexpr (F32) p2[4 * kb + i] = (_Float16)(w[i] - (float)h);
     }
-    if constexpr (!SUMS) st.l += __builtin_ldexpf((w[0] + w[1]) + (w[2] + w[3]), -d[kb]);
+    if constexpr (!SUMS)
+      st.l = fmaf((w[0] + w[1]) + (w[2] + w[3]), kv8_low<SUMS>(d[kb], apart) ? 0.0f : kv8_scale(-d[kb]), st.l);
   }
 }
 
 // 2^-d of each key, with which the matrix unit sums the weights (SUMS); 0 of a tile
 // that kv8_sum_low takes.
-__device__ __forceinline__ f16x8 kv8_ones(const int (&d)[2]) {
+__device__ __forceinline__ f16x8 kv8_ones(const int (&d)[2], bool apart) {
   _Float16 y[2];
 #pragma unroll
-  for (int kb = 0; kb < 2; kb++) y[kb] = (_Float16)(d[kb] < -kSumExp ? 0.0f : __builtin_ldexpf(1.0f, -d[kb]));
+  for (int kb = 0; kb < 2; kb++)
+    y[kb] = (_Float16)(kv8_low<true>(d[kb], apart) ? 0.0f : __builtin_ldexpf(1.0f, -d[kb]));
   return f16x8{y[0], y[0], y[0], y[0], y[1], y[1], y[1], y[1]};
 }
-template <int D>
-__device__ __forceinline__ void kv8_sum_low(const float (&S)[2][4], float sl2, const int (&d)[2],
-                                            Kv8State<D, true> &st) {
-  float l = 0.0f;
+// The low tiles' weights into l, from their scores: 2^(s_j - R - c). First a score far above
+// R + c, whose tile lies so low that R does not follow it, moves c; from then on every tile
+// is low, until R has caught up.
+template <int D, bool SUMS, int RT>
+__device__ __forceinline__ void kv8_sum_low(const float (&S)[RT][2][4], float sl2, const int (&d)[2], Kv8Scale &sc,
+                                            Kv8State<D, SUMS> (&st)[RT]) {
+  bool apart = false;
 #pragma unroll
-  for (int kb = 0; kb < 2; kb++) {
-    if (d[kb] >= -kSumExp) continue;
-    const float base = st.R - kBias - (float)d[kb];
-    float w = 0.0f;
+  for (int x = 0; x < RT; x++) {
+    float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 4; i++) w += fast_exp2(fmaf(S[kb][i], sl2, -base));
-    l += __builtin_ldexpf(w, -d[kb]);
+    for (int kb = 0; kb < 2; kb++)
+      if (kv8_low<SUMS>(d[kb], sc.apart))
+#pragma unroll
+        for (int i = 0; i < 4; i++) top = fmaxf(top, S[x][kb][i] * sl2);
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float M = st[x].R + st[x].c;
+    if (top > M + (kRescaleSlack + kFarExp)) {  // (below, 2^31 such keys add up to less than 2^87)
+      st[x].l *= fast_exp2(M - top);
+      st[x].c = top - st[x].R;
+      apart = true;
+    }
   }
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
-  st.l += l;
+  sc.apart |= __ballot(apart) != 0;
+#pragma unroll
+  for (int x = 0; x < RT; x++) {
+    const float base = st[x].R + st[x].c - kBias;
+    float l = 0.0f;
+#pragma unroll
+    for (int kb = 0; kb < 2; kb++)
+      if (kv8_low<SUMS>(d[kb], sc.apart))
+#pragma unroll
+        for (int i = 0; i < 4; i++) l += fast_exp2(fmaf(S[x][kb][i], sl2, -base));
+    if constexpr (SUMS) {
+      l += __shfl_xor(l, 16);
+      l += __shfl_xor(l, 32);
+    }
+    st[x].l += l;
+  }
 }
 
-// What a tile lies below E - kFarExp, taken from its weights.
-__device__ __forceinline__ void kv8_far(const int (&far)[2], f16x8 &p) {
-  const _Float16 f0 = (_Float16)__builtin_ldexpf(1.0f, far[0]), f1 = (_Float16)__builtin_ldexpf(1.0f, far[1]);
-  p *= f16x8{f0, f0, f0, f0, f1, f1, f1, f1};
+// Partials. A row's weights are l 2^a, l in [0.5, 1), and the sum of its products o 2^b, a and
+// b whole numbers: two powers, for the keys that make the one need not make the other (a
+// tile of zeros), and 2^E stays out of o, so neither leaves f32 where the result does not. Held
+// as (a, l 2^(b - a)) and o, a frexp apart; no merge takes an exponential.
+__device__ __forceinline__ float kv8_pow2(float n) {  // of a whole number n <= 0
+  return __builtin_ldexpf(1.0f, (int)fmaxf(n, -2000.0f));
+}
+__device__ __forceinline__ void kv8_part(float2 ml, float &a, float &b, float &l) {
+  a = ml.x;
+  l = __builtin_amdgcn_frexp_mantf(ml.y);
+  b = a + (float)__builtin_amdgcn_frexp_expf(ml.y);
+}
+// The result of a row is f * 2^x times o. zero_sink: one more key, of weight 1 and value 0.
+__device__ __forceinline__ void kv8_finish(float a, float b, float l, int32_t zero_sink, float &f, int &x) {
+  const float top = zero_sink ? fmaxf(a, 0.0f) : a;
+  f = 1.0f / (zero_sink ? l * kv8_pow2(a - top) + kv8_pow2(-top) : l);
+  x = (int)fminf(fmaxf(b - top, -2000.0f), 2000.0f);
 }
 
-// A finished row: the result 2^E O / l, or its partial (m, l, o) for a merge, the row's
-// weights 2^m l and o / l their mean. A partial is kept where no merge leaves f32: l's
-// power of two is moved to m, so that l < 2^-kPartBits and o is below 2^-kPartBits of the
-// greatest V, and up to 2^kPartBits partials add up to less than that V. (2^E O alone passes
-// f32 from V of 2^121 on for one key, 2^108 for thousands.) All by exact powers of two.
+// A finished row: the result, or its partial for a merge.
 template <int D, bool F32, bool SUMS>
 __device__ __forceinline__ void kv8_store(const Kv8State<D, SUMS> &st, int E, int g4, bool final, void *o, int64_t row,
                                           float *ws_ml, float *ws_o, int64_t prow, int32_t zero_sink) {
-  const float m = st.R - kBias;
-  const int up = __builtin_amdgcn_frexp_expf(st.sum()) + kPartBits;  // (0, infinity and NaN: kPartBits)
-  const int x = final ? E : E - up;
-  const float f = final ? final_scale(m, st.sum(), zero_sink) : 1.0f;
+  // (As the weights and their sums were formed: the same where c is 0.)
+  const float m = st.R + st.c - kBias, r = st.R - kBias;
+  const float ls = st.sum() * fast_exp2(m - floorf(m));
+  const float a = floorf(m) + (float)__builtin_amdgcn_frexp_expf(ls), b = floorf(r) + (float)E;
+  const float l = __builtin_amdgcn_frexp_mantf(ls);
+  float f = fast_exp2(r - floorf(r));
+  int x;
+  float k = 0.0f;
+  if (final) {
+    float g;
+    kv8_finish(a, b, l, zero_sink, g, x);
+    f *= g;
+  } else {  // (b - a past what an exponent holds: the rest to o, whose sum is nothing beside l then, or small)
+    k = fminf(fmaxf(b - a, -120.0f), 120.0f);
+    x = (int)fminf(fmaxf(b - a - k, -2000.0f), 2000.0f);
+  }
 #pragma unroll
   for (int i = 0; i < D / 64; i++) {
     float y[16];
@@ -254,8 +328,7 @@ __device__ __forceinline__ void kv8_store(const Kv8State<D, SUMS> &st, int E, in
       for (int z = 0; z < 4; z++) p[z] = f32x4{y[4 * z], y[4 * z + 1], y[4 * z + 2], y[4 * z + 3]};
     }
   }
-  if (!final && g4 == 0)
-    *reinterpret_cast<float2 *>(ws_ml + 2 * prow) = make_float2(m + (float)up, __builtin_ldexpf(st.sum(), -up));
+  if (!final && g4 == 0) *reinterpret_cast<float2 *>(ws_ml + 2 * prow) = make_float2(a, __builtin_ldexpf(l, (int)k));
 }
 
 // ===========================================================================
@@ -368,7 +441,7 @@ __device__ __forceinline__ void kv8_item_exps(const Kv8Args &a, int h, Kv8Items 
 // One step: scores of both blocks, weights, O += P.V.
 template <int D, bool F32>
 __device__ __forceinline__ void kv8_step(float sl2, Kv8Raw<D> &raw, int lane, int exps, int meta,
-                                         const Kv8Q<D, F32> &q, int &E, Kv8State<D> (&st)[1]) {
+                                         const Kv8Q<D, F32> &q, Kv8Scale &sc, Kv8State<D> (&st)[1]) {
   const int g4 = lane >> 4;
   int ek[2] = {(int8_t)exps, (int8_t)(exps >> 8)}, ev[2] = {(int8_t)(exps >> 16), exps >> 24};
   const int nv = meta & kItemValid;
@@ -387,10 +460,10 @@ __device__ __forceinline__ void kv8_step(float sl2, Kv8Raw<D> &raw, int lane, in
         for (int n = 0; n < 4; n++) raw.v[kb][i][n] &= m;
     }
   }
-  kv8_raise(E, ev[0], ev[1], st);
-  int d[2], far[2];
-  kv8_offsets(E, ev[0], ev[1], d, far);
-  float t[2][4];
+  kv8_raise(sc, ev[0], ev[1], st);
+  int d[2];
+  kv8_offsets(sc.E, ev[0], ev[1], d);
+  float t[1][2][4];
 #pragma unroll
   for (int kb = 0; kb < 2; kb++) {
     const float ks = kv8_scale(ek[kb]);
@@ -406,22 +479,19 @@ __device__ __forceinline__ void kv8_step(float sl2, Kv8Raw<D> &raw, int lane, in
       }
     // Lane holds S[token 16 kb + 4 g4 + i][query lane % 16].
 #pragma unroll
-    for (int i = 0; i < 4; i++) t[kb][i] = S[i];
+    for (int i = 0; i < 4; i++) t[0][kb][i] = S[i];
     if (partial) {
       const bool bad = meta & (kb ? kItemBad1 : kItemBad0);
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        if (bad || kPageSize * kb + 4 * g4 + i >= nv) t[kb][i] = -INFINITY;
+        if (bad || kPageSize * kb + 4 * g4 + i >= nv) t[0][kb][i] = -INFINITY;
     }
   }
-  const float top = kv8_top(t, sl2, d);
-  if (__ballot(top > st[0].R + kRescaleSlack)) kv8_rescale(top, st[0]);
+  const float top[1] = {kv8_top(t[0], sl2, d)};
+  if (__ballot(top[0] > st[0].R + kRescaleSlack)) kv8_rescale_all(top, sc, st);
+  if (kv8_low<false>(min(d[0], d[1]), sc.apart)) kv8_sum_low(t, sl2, d, sc, st);  // (uniform, rare)
   f16x8 p, p2;
-  kv8_weights<D, F32>(t, sl2, d, st[0], p, p2);
-  if (far[0] | far[1]) {  // (uniform, rare)
-    kv8_far(far, p);
-    if constexpr (F32) kv8_far(far, p2);
-  }
+  kv8_weights<D, F32>(t[0], sl2, d, sc.apart, st[0], p, p2);
 #pragma unroll
   for (int i = 0; i < D / 64; i++)
 #pragma unroll
@@ -438,7 +508,7 @@ __device__ __forceinline__ void kv8_step(float sl2, Kv8Raw<D> &raw, int lane, in
 // one's q.
 template <int D, bool F32, class Start, class Finish>
 __device__ __forceinline__ void kv8_run(const Kv8Args &a, const Kv8Dec &dc, int lane, int h, int n, Kv8Items it,
-                                        int &cur_b, const Kv8Q<D, F32> &q, int &E,
+                                        int &cur_b, const Kv8Q<D, F32> &q, Kv8Scale &sc,
                                         Kv8State<D> (&st)[1], Start start, Finish finish) {
   constexpr int RING = D == 256 ? 2 : 3;
   if (dc.new_k) kv8_insert<D, F32>(a, dc, lane, h, n, it);
@@ -474,12 +544,12 @@ __device__ __forceinline__ void kv8_run(const Kv8Args &a, const Kv8Dec &dc, int 
     if (b != cur_b) {
       if (cur_b >= 0) finish(cur_b);
       st[0].reset();
-      E = kNoExp;
+      sc.reset();
       cur_b = b;
       start(b);
     }
     kv8_step<D, F32>(dc.sl2, raw[s], lane, __builtin_amdgcn_readlane(it.exps, k),
-                     __builtin_amdgcn_readlane(it.meta, k), q, E, st);
+                     __builtin_amdgcn_readlane(it.meta, k), q, sc, st);
   };
 #pragma unroll
   for (int s = 0; s < RING - 1; s++) issue(raw[s], s);
@@ -559,7 +629,9 @@ kv8_decode_split_kernel(Kv8Args a, Kv8Dec dc) {
   const int nq = kv8_chunk_heads(a.G, qc), q0 = h * a.G + 16 * qc;
   Kv8Q<D, F32> q;
   Kv8State<D> st[1];
-  int E = kNoExp, cur = -1;
+  Kv8Scale sc;
+  sc.reset();
+  int cur = -1;
   auto start = [&](int b) { q.load(dc.q, (int64_t)b * a.Hq + q0 + min(m16, nq - 1), g4); };
   auto finish = [&](int b) {
     st[0].join();
@@ -567,7 +639,7 @@ kv8_decode_split_kernel(Kv8Args a, Kv8Dec dc) {
     if (m16 >= nq) return;
     // A sequence that starts in this piece and goes on behind it is its second partial.
     const int64_t slot = 2 * (int64_t)p + (s0 >= f0);
-    kv8_store<D, F32, false>(st[0], E, g4, s0 >= f0 && s1 <= f1, dc.o, (int64_t)b * a.Hq + q0 + m16, dc.ws_ml, dc.ws_o,
+    kv8_store<D, F32, false>(st[0], sc.E, g4, s0 >= f0 && s1 <= f1, dc.o, (int64_t)b * a.Hq + q0 + m16, dc.ws_ml, dc.ws_o,
                       slot * a.Hq + q0 + m16, dc.zero_sink);
   };
   for (int c = f0; c < f1; c += 64) {
@@ -583,9 +655,46 @@ kv8_decode_split_kernel(Kv8Args a, Kv8Dec dc) {
       }
       it = kv8_item(a, lo, ctx_s[lo], tab_s[lo], f - pre[lo]);
     }
-    kv8_run<D, F32>(a, dc, lane, h, n, it, cur, q, E, st, start, finish);
+    kv8_run<D, F32>(a, dc, lane, h, n, it, cur, q, sc, st, start, finish);
   }
   finish(cur);
+}
+
+// Merge of n partials by a wave: (a, l 2^(b - a)) of partial s at ml_at(s), o at o_at(s). Lane s
+// holds the numbers of partial s of a round of 16, lane d dims d * DPL .. +DPL of every one.
+template <int D, class MlAt, class OAt>
+__device__ __forceinline__ void kv8_merge(int lane, int n, MlAt ml_at, OAt o_at, float &A, float &B, float &L,
+                                          typename MergeVec<D>::type &acc) {
+  constexpr int DPL = MergeVec<D>::DPL, SB = 16;
+  typedef typename MergeVec<D>::type fvec;
+  acc = fvec{};
+  A = B = -FLT_MAX;
+  L = 0.0f;
+  auto first = [](float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+  };
+  for (int s0 = 0; s0 < n; s0 += SB) {
+    const int cnt = min(SB, n - s0);
+    float2 ml = make_float2(-FLT_MAX, 0.0f);
+    if (lane < cnt) ml = *reinterpret_cast<const float2 *>(ml_at(s0 + lane));
+    fvec ov[SB];
+#pragma unroll
+    for (int i = 0; i < SB; i++) {
+      ov[i] = fvec{};
+      if (i < cnt) ov[i] = *reinterpret_cast<const fvec *>(o_at(s0 + i) + lane * DPL);
+    }
+    float a, b, l;
+    kv8_part(ml, a, b, l);
+    const float An = fmaxf(A, first(row16_max(a))), Bn = fmaxf(B, first(row16_max(b)));
+    L = L * kv8_pow2(A - An) + first(row_sum<16>(l * kv8_pow2(a - An)));
+    acc *= kv8_pow2(B - Bn);
+    const float w = kv8_pow2(b - Bn);
+#pragma unroll
+    for (int i = 0; i < SB; i++)
+      acc += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), i)) * ov[i];
+    A = An;
+    B = Bn;
+  }
 }
 
 // The merge of a split launch, a workgroup per (query head, sequence); also the
@@ -595,7 +704,7 @@ __global__ void __launch_bounds__(256) kv8_decode_merge_kernel(Kv8Args a, Kv8Dec
   constexpr int NW = 4, DPL = MergeVec<D>::DPL;
   typedef typename MergeVec<D>::type fvec;
   __shared__ int32_t sums[2][NW];
-  __shared__ float part[NW][2 + 64 * DPL];
+  __shared__ float part[NW][3 + 64 * DPL];
   const int lane = threadIdx.x & 63, hq = blockIdx.x, b = blockIdx.y;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int before = 0, all = 0;
@@ -632,33 +741,42 @@ __global__ void __launch_bounds__(256) kv8_decode_merge_kernel(Kv8Args a, Kv8Dec
     const int pc = p0 + s0 + s;
     return (2 * (int64_t)pc + (before >= pc * per)) * a.Hq + hq;
   };
-  float M, L;
+  float A, B, L;
   fvec acc;
-  merge_partials_state<D>(
-      lane, s1 - s0, [&](int s) { return dc.ws_ml + 2 * at(s); }, [&](int s) { return dc.ws_o + at(s) * D; }, M, L, acc);
+  kv8_merge<D>(
+      lane, s1 - s0, [&](int s) { return dc.ws_ml + 2 * at(s); }, [&](int s) { return dc.ws_o + at(s) * D; }, A, B, L,
+      acc);
   if (waves > 1) {
-    if (lane == 0) part[wave][0] = M, part[wave][1] = L;
+    if (lane == 0) part[wave][0] = A, part[wave][1] = B, part[wave][2] = L;
 #pragma unroll
-    for (int k = 0; k < DPL; k++) part[wave][2 + lane * DPL + k] = acc[k];
+    for (int k = 0; k < DPL; k++) part[wave][3 + lane * DPL + k] = acc[k];
     __syncthreads();
     if (wave != 0) return;
-    float Mx = -INFINITY, Lx = 0.0f;
+    L = 0.0f;
+    acc = fvec{};
 #pragma unroll
-    for (int w = 0; w < NW; w++) Mx = fmaxf(Mx, part[w][0]);
-    fvec ax = fvec{};
+    for (int w = 1; w < NW; w++) A = fmaxf(A, part[w][0]), B = fmaxf(B, part[w][1]);
 #pragma unroll
     for (int w = 0; w < NW; w++) {
-      const float f = part[w][0] == -INFINITY ? 0.0f : fast_exp2(part[w][0] - Mx);
-      Lx = fmaf(part[w][1], f, Lx);
+      L = fmaf(part[w][2], kv8_pow2(part[w][0] - A), L);
+      const float f = kv8_pow2(part[w][1] - B);
 #pragma unroll
-      for (int k = 0; k < DPL; k++) ax[k] = fmaf(part[w][2 + lane * DPL + k], f, ax[k]);
+      for (int k = 0; k < DPL; k++) acc[k] = fmaf(part[w][3 + lane * DPL + k], f, acc[k]);
     }
-    M = Mx, L = Lx, acc = ax;
   }
-  KArgs ka;
-  ka.o = dc.o;
-  ka.zero_sink = dc.zero_sink;
-  store_merged_row<D, !F32>(ka, lane, M, L, acc, row);
+  float f;
+  int x;
+  kv8_finish(A, B, L, dc.zero_sink, f, x);
+  const int64_t to = row * D + lane * DPL;
+#pragma unroll
+  for (int k = 0; k < DPL; k++) acc[k] = __builtin_ldexpf(acc[k] * f, x);
+  if constexpr (F32) *reinterpret_cast<fvec *>(static_cast<float *>(dc.o) + to) = acc;
+  else {
+    uint16_t *op = static_cast<uint16_t *>(dc.o) + to;
+    if constexpr (DPL == 1) *op = (uint16_t)f32_to_bf16_bits(acc[0]);
+    else if constexpr (DPL == 2) *reinterpret_cast<uint32_t *>(op) = pack_bf16x2(acc[0], acc[1]);
+    else *reinterpret_cast<uint2 *>(op) = make_uint2(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]));
+  }
 }
 
 template <int D, bool F32>
@@ -682,35 +800,45 @@ kv8_decode_seq_kernel(Kv8Args a, Kv8Dec dc) {
     const int ctx = a.ctx[b], tab0 = a.indptr[b];
     Kv8Q<D, F32> q;
     Kv8State<D> st[1];
-    int E = kNoExp, cur = b;
+    Kv8Scale sc;
+    int cur = b;
+    sc.reset();
     st[0].reset();
     q.load(dc.q, (int64_t)b * a.Hq + q0 + min(m16, nq - 1), g4);
     for (int c = f0; c < f1; c += 64) {
       const int n = min(64, f1 - c);
       Kv8Items it = {b, 0, 0, 0, 0};
       if (lane < n) it = kv8_item(a, b, ctx, tab0, c + lane);
-      kv8_run<D, F32>(a, dc, lane, h, n, it, cur, q, E, st, [](int) {}, [](int) {});
+      kv8_run<D, F32>(a, dc, lane, h, n, it, cur, q, sc, st, [](int) {}, [](int) {});
     }
     st[0].join();
-    kv8_store<D, true, false>(st[0], E, g4, false, nullptr, 0, &ml[wave][0].x, &part[wave][0][0], m16, 0);
+    kv8_store<D, true, false>(st[0], sc.E, g4, false, nullptr, 0, &ml[wave][0].x, &part[wave][0][0], m16, 0);
   }
   __syncthreads();
   const int used = min(NW, steps);
   for (int i = threadIdx.x; i < nq * (D / 4); i += 64 * NW) {
     const int r = i / (D / 4), dim = 4 * (i % (D / 4));
-    float M = -INFINITY, L = 0.0f;
+    float A = -FLT_MAX, B = -FLT_MAX, L = 0.0f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int w = 0; w < NW; w++)
-      if ((int64_t)steps * w / NW < (int64_t)steps * (w + 1) / NW) M = fmaxf(M, ml[w][r].x);
+    auto live = [&](int w) { return (int64_t)steps * w / NW < (int64_t)steps * (w + 1) / NW; };
     for (int w = 0; w < NW; w++) {
-      if ((int64_t)steps * w / NW == (int64_t)steps * (w + 1) / NW) continue;
-      const float2 s = ml[w][r];
-      const float f = s.x == -INFINITY ? 0.0f : fast_exp2(s.x - M);
-      L = fmaf(s.y, f, L);
-      acc += *reinterpret_cast<const f32x4 *>(&part[w][r][dim]) * f;
+      if (!live(w)) continue;
+      float pa, pb, pl;
+      kv8_part(ml[w][r], pa, pb, pl);
+      A = fmaxf(A, pa), B = fmaxf(B, pb);
     }
-    // (No keys at all: a padding sequence, a row of zeros.)
-    acc *= used ? final_scale(M, L, dc.zero_sink) : 0.0f;
+    for (int w = 0; w < NW; w++) {
+      if (!live(w)) continue;
+      float pa, pb, pl;
+      kv8_part(ml[w][r], pa, pb, pl);
+      L = fmaf(pl, kv8_pow2(pa - A), L);
+      acc += *reinterpret_cast<const f32x4 *>(&part[w][r][dim]) * kv8_pow2(pb - B);
+    }
+    float f = 0.0f;  // (No keys at all: a padding sequence, a row of zeros.)
+    int x = 0;
+    if (used) kv8_finish(A, B, L, dc.zero_sink, f, x);
+#pragma unroll
+    for (int k = 0; k < 4; k++) acc[k] = __builtin_ldexpf(acc[k] * f, x);
     const int64_t at = ((int64_t)b * a.Hq + q0 + r) * D + dim;
     if constexpr (F32) *reinterpret_cast<f32x4 *>(static_cast<float *>(dc.o) + at) = acc;
     else
@@ -797,7 +925,8 @@ __device__ __forceinline__ void kv8_extend_tile(const Kv8Args &a, const Kv8Ext &
   int64_t qrow[RT];
   Kv8Q<D, F32> q[RT];
   Kv8State<D, !F32> st[RT];
-  int E = kNoExp;
+  Kv8Scale sc;
+  sc.reset();
   int qhi = -1;  // last position of the wave's rows; -1: it has none
 #pragma unroll
   for (int i = 0; i < RT; i++) {
@@ -871,16 +1000,15 @@ __device__ __forceinline__ void kv8_extend_tile(const Kv8Args &a, const Kv8Ext &
   };
   auto sum_p = [&](const f16x8 (&p)[RT], const int (&d)[2]) {
     if constexpr (!F32) {
-      const f16x8 ones = kv8_ones(d);
+      const f16x8 ones = kv8_ones(d, sc.apart);
 #pragma unroll
       for (int x = 0; x < RT; x++) st[x].l = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[x], st[x].l, 0, 0, 0);
     }
   };
-  // E and R for the scores S of a step with V exponents ev0, ev1.
-  auto settle = [&](const f32x4 (&S)[RT][2], int ev0, int ev1, float (&t)[RT][2][4], int (&d)[2], int (&far)[2],
-                    auto mask) {
-    kv8_raise(E, ev0, ev1, st);
-    kv8_offsets(E, ev0, ev1, d, far);
+  // E, R and what kv8_sum_low adds for the scores S of a step with V exponents ev0, ev1.
+  auto settle = [&](const f32x4 (&S)[RT][2], int ev0, int ev1, float (&t)[RT][2][4], int (&d)[2], auto mask) {
+    kv8_raise(sc, ev0, ev1, st);
+    kv8_offsets(sc.E, ev0, ev1, d);
     float top[RT];
     bool move = false;
 #pragma unroll
@@ -893,13 +1021,8 @@ __device__ __forceinline__ void kv8_extend_tile(const Kv8Args &a, const Kv8Ext &
       top[x] = kv8_top(t[x], e.sl2, d);
       move |= top[x] > st[x].R + kRescaleSlack;
     }
-    if (__ballot(move))
-#pragma unroll
-      for (int x = 0; x < RT; x++) kv8_rescale(top[x], st[x]);
-    if constexpr (!F32)
-      if (min(d[0], d[1]) < -kSumExp)  // (uniform, rare)
-#pragma unroll
-        for (int x = 0; x < RT; x++) kv8_sum_low(t[x], e.sl2, d, st[x]);
+    if (__ballot(move)) kv8_rescale_all(top, sc, st);
+    if (kv8_low<!F32>(min(d[0], d[1]), sc.apart)) kv8_sum_low(t, e.sl2, d, sc, st);  // (uniform, rare)
   };
 
   f32x4 S[2][RT][2];
@@ -1004,9 +1127,9 @@ __device__ __forceinline__ void kv8_extend_tile(const Kv8Args &a, const Kv8Ext &
           bf16x8 k[2][2][2];
           read_k(k[0], y ^ 1, 0);
           float t[RT][2][4];
-          int d[2], far[2];
+          int d[2];
           settle(cur, __builtin_amdgcn_readlane(exw, lane_of(i, 0)) >> 8, __builtin_amdgcn_readlane(exw, lane_of(i, 1)) >> 8,
-                 t, d, far, [](float (&)[2][4], int) {});
+                 t, d, [](float (&)[2][4], int) {});
           f16x8 p[RT], p2[RT], v[2][4];
 #pragma unroll
           for (int r = 0; r < NR; r++) {
@@ -1015,19 +1138,14 @@ __device__ __forceinline__ void kv8_extend_tile(const Kv8Args &a, const Kv8Ext &
           }
           read_v(v[0], y, 0);
 #pragma unroll
-          for (int x = 0; x < RT; x++) kv8_weights<D, F32, !F32>(t[x], e.sl2, d, st[x], p[x], p2[x]);
+          for (int x = 0; x < RT; x++) kv8_weights<D, F32, !F32>(t[x], e.sl2, d, sc.apart, st[x], p[x], p2[x]);
           // One product, then some of the weights' instructions, in turn.
 #pragma unroll
           for (int g = 0; g < 4 * NR * RT * Kv8Q<D, F32>::QP; g++) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x002, F32 ? 2 : 4, 0);
           }
-          if (far[0] | far[1])  // (uniform, rare)
-#pragma unroll
-            for (int x = 0; x < RT; x++) {
-              kv8_far(far, p[x]);
-              if constexpr (F32) kv8_far(far, p2[x]);
-            }
+          __builtin_amdgcn_sched_barrier(0);  // (362 us where the products with V may mix in, 323 here: 8 x 512 after 4k)
           sum_p(p, d);
 #pragma unroll
           for (int r = 0; r < NR; r++) {
@@ -1056,9 +1174,9 @@ __device__ __forceinline__ void kv8_extend_tile(const Kv8Args &a, const Kv8Ext &
       const int y = step - c0 & 1;
       if (kKv8Step * step <= qhi) {
         float t[RT][2][4];
-        int d[2], far[2];
+        int d[2];
         settle(S[0], __builtin_amdgcn_readfirstlane(exps_s[block(step, 0)]) >> 8,
-               __builtin_amdgcn_readfirstlane(exps_s[block(step, 1)]) >> 8, t, d, far, [&](float (&u)[2][4], int x) {
+               __builtin_amdgcn_readfirstlane(exps_s[block(step, 1)]) >> 8, t, d, [&](float (&u)[2][4], int x) {
                  if (!bad && kKv8Step * (step + 1) - 1 <= qlo[x]) return;
                  const int key = kKv8Step * step + 4 * g4;
 #pragma unroll
@@ -1071,13 +1189,7 @@ __device__ __forceinline__ void kv8_extend_tile(const Kv8Args &a, const Kv8Ext &
                });
         f16x8 p[RT], p2[RT];
 #pragma unroll
-        for (int x = 0; x < RT; x++) {
-          kv8_weights<D, F32, !F32>(t[x], e.sl2, d, st[x], p[x], p2[x]);
-          if (far[0] | far[1]) {
-            kv8_far(far, p[x]);
-            if constexpr (F32) kv8_far(far, p2[x]);
-          }
-        }
+        for (int x = 0; x < RT; x++) kv8_weights<D, F32, !F32>(t[x], e.sl2, d, sc.apart, st[x], p[x], p2[x]);
         scores(S[0], y ^ 1);
         sum_p(p, d);
 #pragma unroll
@@ -1100,7 +1212,7 @@ __device__ __forceinline__ void kv8_extend_tile(const Kv8Args &a, const Kv8Ext &
   for (int i = 0; i < RT; i++) {
     st[i].join();
     if (row0[i] + m16 < rows)
-      kv8_store<D, F32, !F32>(st[i], E, g4, whole, e.o, qrow[i], e.ws_ml, e.ws_o, qrow[i] * e.parts + part,
+      kv8_store<D, F32, !F32>(st[i], sc.E, g4, whole, e.o, qrow[i], e.ws_ml, e.ws_o, qrow[i] * e.parts + part,
                               e.zero_sink);
   }
   if (!odd) return;
@@ -1255,7 +1367,7 @@ __global__ void __launch_bounds__(256) kv8_extend_merge_kernel(Kv8Args a, Kv8Ext
     const int parts = (from + steps - 1) / per - from / per + 1;
     if (parts == 1) continue;  // stored already
     const int64_t at = ((int64_t)s.q0 * a.Hq + r) * e.parts;
-    float M = -FLT_MAX, L = 0.0f;
+    float A = -FLT_MAX, B = -FLT_MAX, L = 0.0f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     constexpr int N = 8;  // partials loaded at a time
     for (int i0 = 0; i0 < parts; i0 += N) {
@@ -1267,22 +1379,29 @@ __global__ void __launch_bounds__(256) kv8_extend_merge_kernel(Kv8Args a, Kv8Ext
         y[i] = *reinterpret_cast<const float2 *>(e.ws_ml + 2 * c);
         o[i] = *reinterpret_cast<const f32x4 *>(e.ws_o + c * D + dim);
       }
-      float m = M;
+      float pa[N], pb[N], pl[N], An = A, Bn = B;
 #pragma unroll
-      for (int i = 0; i < N; i++) m = fmaxf(m, y[i].x);
-      const float f = fast_exp2(M - m);
-      L *= f;
-      acc *= f;
+      for (int i = 0; i < N; i++) {
+        kv8_part(y[i], pa[i], pb[i], pl[i]);
+        An = fmaxf(An, pa[i]);
+        Bn = fmaxf(Bn, pb[i]);
+      }
+      L *= kv8_pow2(A - An);
+      acc *= kv8_pow2(B - Bn);
 #pragma unroll
       for (int i = 0; i < N; i++) {
         if (i0 + i >= parts) break;
-        const float w = fast_exp2(y[i].x - m);
-        L = fmaf(y[i].y, w, L);
-        acc += o[i] * w;
+        L = fmaf(pl[i], kv8_pow2(pa[i] - An), L);
+        acc += o[i] * kv8_pow2(pb[i] - Bn);
       }
-      M = m;
+      A = An;
+      B = Bn;
     }
-    acc *= final_scale(M, L, e.zero_sink);
+    float f;
+    int x;
+    kv8_finish(A, B, L, e.zero_sink, f, x);
+#pragma unroll
+    for (int k = 0; k < 4; k++) acc[k] = __builtin_ldexpf(acc[k] * f, x);
     const int64_t out = ((int64_t)s.q0 * a.Hq + r) * D + dim;
     if constexpr (F32) *reinterpret_cast<f32x4 *>(static_cast<float *>(e.o) + out) = acc;
     else
