@@ -641,7 +641,7 @@ typedef struct mkv_kv8_pool mkv_kv8_pool;
 
 /* Bytes of the tiles and of the exponents. */
 MKV_API int mkv_kv8_required_bytes(const mkv_pool_desc *desc, uint64_t *out_tile_bytes, uint64_t *out_exponent_bytes);
-/* Allocate the pool and its workspace (64 MiB) on `device` (hipMalloc; contents
+/* Allocate the pool and its workspace (mkv_kv8_workspace_size) on `device` (hipMalloc; contents
  * uninitialised). MKV_ERR_OUT_OF_MEMORY if HBM cannot hold them. */
 MKV_API int mkv_kv8_pool_create(const mkv_pool_desc *desc, int device, mkv_kv8_pool **out_pool);
 MKV_API int mkv_kv8_pool_destroy(mkv_kv8_pool *pool);
@@ -716,7 +716,7 @@ MKV_API int mkv_kv8_copy_blocks_host(mkv_kv8_pool *pool, const uint32_t *h_src_b
  * MKV_DEVERR_CTX, and skipped) and sizes the launch; lengths and tables are read
  * when the kernels run. Long contexts are cut into equal pieces over all
  * sequences, whose partials (f32) stand in d_workspace
- * (mkv_kv8_workspace_size bytes, 16-byte aligned; with less there are fewer
+ * (mkv_kv8_workspace_size bytes, 16-byte aligned; with fewer there are fewer
  * pieces) or, when it is NULL, in the pool's own. Calls that use the pool's own
  * follow one another across streams; a captured one must not be replayed beside
  * another call or graph that uses it (give each a workspace). Scores, sums and
@@ -733,7 +733,11 @@ MKV_API int mkv_kv8_decode_attention_host(mkv_kv8_pool *pool, int32_t layer, con
                                           const int32_t *h_ctx_lens, const uint32_t *h_block_indptr,
                                           const uint32_t *h_block_ids, int32_t num_seqs, float scale, uint32_t flags,
                                           void *stream);
-/* Bytes with which no decode or extend call of this pool is held back. */
+/* Bytes of the pool's own workspace: with them no decode call is held back, which takes
+ * 256 + 2 * num_q_heads * (8 + 4 * head_dim) for each of up to 8 * CUs / (KV heads * ceil(group
+ * / 16)) pieces, and 64 MiB at the least. An extend call of n tokens is cut into at most
+ * min(32, (bytes - 256) / (n * num_q_heads * (8 + 4 * head_dim))) partials a row, and not at
+ * all where that is less than 2: a larger workspace given to it allows more. */
 MKV_API int mkv_kv8_workspace_size(const mkv_kv8_pool *pool, uint64_t *out_bytes);
 
 /* Causal attention of each sequence's newest tokens, as mkv_extend_attention, the

@@ -23,7 +23,9 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
 
 constexpr int kKv8MinExp = -100;
-constexpr uint64_t kKv8Workspace = 64ull << 20;
+constexpr uint64_t kKv8Workspace = 64ull << 20;  // bytes of a pool's own workspace, at least
+// Waves of a split decode launch.
+constexpr int kSplitWavesPerCu = 8;
 
 struct Kv8Pool : MetaRing {
   mkv_pool_desc desc;
@@ -34,7 +36,8 @@ struct Kv8Pool : MetaRing {
   int8_t *exps = nullptr;
   uint64_t tile_bytes = 0, exp_bytes = 0;
   uint32_t *d_err = nullptr;
-  void *ws = nullptr;  // kKv8Workspace bytes, allocated with the pool
+  void *ws = nullptr;  // ws_bytes, allocated with the pool
+  uint64_t ws_bytes = 0;
   hipEvent_t ws_done = nullptr;
   bool ws_used = false;
   // The last host arrays of each kind of call.
@@ -43,6 +46,12 @@ struct Kv8Pool : MetaRing {
 };
 
 inline int64_t kv8_exp_plane(const Geom &g) { return g.nblocks * g.Hkv; }
+
+// Pieces of a split decode launch, at most, and the workspace of n pieces: two partials each.
+inline int64_t kv8_most_pieces(const Geom &g, int cus) {
+  return std::max<int64_t>(1, (int64_t)cus * kSplitWavesPerCu / ((int64_t)g.Hkv * ((g.Hq / g.Hkv + 15) / 16)));
+}
+inline uint64_t kv8_piece_bytes(const Geom &g, int64_t n) { return 256 + (uint64_t)n * 2 * g.Hq * (8 + 4 * g.D); }
 
 int kv8_check_layer(const Kv8Pool *p, int32_t layer);
 

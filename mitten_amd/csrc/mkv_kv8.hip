@@ -448,7 +448,7 @@ int kv8_ws_begin(Kv8Pool *p, void *d_ws, uint64_t bytes, hipStream_t hs, Kv8Ws *
     return MKV_OK;
   }
   out->ptr = p->ws;
-  out->bytes = kKv8Workspace;
+  out->bytes = p->ws_bytes;
   MKV_CHECK_HIP(hipStreamIsCapturing(hs, &st));
   out->own = st == hipStreamCaptureStatusNone;
   if (out->own && p->ws_used) MKV_CHECK_HIP(hipStreamWaitEvent(hs, p->ws_done, 0));
@@ -667,11 +667,12 @@ extern "C" int mkv_kv8_pool_create(const mkv_pool_desc *desc, int device, mkv_kv
   p->exp_bytes = (uint64_t)2 * g.L * (uint64_t)kv8_exp_plane(g);
   hipError_t e = hipMalloc(reinterpret_cast<void **>(&p->tiles), p->tile_bytes);
   if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&p->exps), p->exp_bytes);
-  if (e == hipSuccess) e = hipMalloc(&p->ws, kKv8Workspace);
+  if (e == hipSuccess) e = hipDeviceGetAttribute(&p->cus, hipDeviceAttributeMultiprocessorCount, device);
+  p->ws_bytes = std::max(kKv8Workspace, kv8_piece_bytes(g, kv8_most_pieces(g, p->cus)));
+  if (e == hipSuccess) e = hipMalloc(&p->ws, p->ws_bytes);
   if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&p->d_err), 256);
   if (e == hipSuccess) e = hipMemset(p->d_err, 0, 256);
   if (e == hipSuccess) e = hipEventCreateWithFlags(&p->ws_done, hipEventDisableTiming);
-  if (e == hipSuccess) e = hipDeviceGetAttribute(&p->cus, hipDeviceAttributeMultiprocessorCount, device);
   if (e != hipSuccess) {
     mkv_kv8_pool_destroy(reinterpret_cast<mkv_kv8_pool *>(p));
     return hip_fail(e, "8-bit pool allocation");
@@ -727,7 +728,7 @@ extern "C" int mkv_kv8_pool_check(mkv_kv8_pool *pool, void *stream, uint32_t *ou
 
 extern "C" int mkv_kv8_workspace_size(const mkv_kv8_pool *pool, uint64_t *out_bytes) {
   if (!pool || !out_bytes) return set_error(MKV_ERR_INVALID_ARGUMENT, "NULL argument");
-  *out_bytes = kKv8Workspace;
+  *out_bytes = reinterpret_cast<const Kv8Pool *>(pool)->ws_bytes;
   return MKV_OK;
 }
 

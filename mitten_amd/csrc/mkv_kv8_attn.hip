@@ -1440,11 +1440,10 @@ static int kv8_check_attn(const Kv8Pool *p, int32_t layer, float scale, uint32_t
 
 // ---- decode
 
-// Waves of a split launch and steps of a piece, at least. Measured, 64 sequences of 1 to
+// kSplitWavesPerCu, and the steps of a piece, at least. Measured, 64 sequences of 1 to
 // 8k tokens (280 MB): 8 waves a CU 63.5 us, 7 the same, 12 (with a ring of 2, which
 // their registers allow) 65.9, 16 73.0; one sequence of 8k: 4 steps 16.3 us, 2 the
 // same, 8 18.6.
-constexpr int kSplitWavesPerCu = 8;
 constexpr int kSplitMinSteps = 4;
 
 // Steps of the longest context that a wave of the seq kernel may have to take; behind that
@@ -1565,10 +1564,10 @@ extern "C" int mkv_kv8_decode_attention(mkv_kv8_pool *pool, int32_t layer, const
     if ((rc = kv8_ws_begin(p, d_workspace, workspace_bytes, hs, &ws))) return rc;
     // Two partials a piece; fewer pieces where there are no more steps, or the
     // workspace holds no more.
-    pieces = std::max<int64_t>(1, (int64_t)p->cus * kSplitWavesPerCu / heads);
+    pieces = kv8_most_pieces(g, p->cus);
     pieces = std::min(pieces, (most * num_seqs + kSplitMinSteps - 1) / kSplitMinSteps);
-    const uint64_t room = ws.bytes > 256 ? ws.bytes - 256 : 0;
-    pieces = std::min<int64_t>(pieces, (int64_t)(room / ((uint64_t)2 * g.Hq * (8 + 4 * g.D))));
+    if (kv8_piece_bytes(g, pieces) > ws.bytes)
+      pieces = ws.bytes > 256 ? (int64_t)((ws.bytes - 256) / ((uint64_t)2 * g.Hq * (8 + 4 * g.D))) : 0;
     d.ws_ml = static_cast<float *>(ws.ptr);
     d.ws_o = reinterpret_cast<float *>(static_cast<uint8_t *>(ws.ptr) + kv8_ml_bytes((uint64_t)2 * pieces * g.Hq));
   }
@@ -1651,7 +1650,7 @@ extern "C" int mkv_kv8_extend_attention(mkv_kv8_pool *pool, int32_t layer, const
   };
   const int64_t steps = ((int64_t)max_ctx_len + kKv8Step - 1) / kKv8Step;
   const uint64_t row = (uint64_t)num_tokens * g.Hq * (8 + 4 * g.D);
-  const uint64_t bytes = d_workspace ? workspace_bytes : kKv8Workspace, room = bytes > 256 ? bytes - 256 : 0;
+  const uint64_t bytes = d_workspace ? workspace_bytes : p->ws_bytes, room = bytes > 256 ? bytes - 256 : 0;
   const int parts = (int)std::min<uint64_t>(room / row, 32);
   Kv8ExtForm form{};
   double best = INFINITY;

@@ -146,7 +146,9 @@ class DeviceKv8Pool:
         _raise(st)
 
     def workspace_size(self) -> int:
-        """Bytes of a workspace with which no call is held back."""
+        """Bytes of the pool's own workspace, with which no decode call is held back. An
+        extend call of n tokens takes min(32, (bytes - 256) // (n * Hq * (8 + 4 * D)))
+        partials a row, and is not cut with fewer than 2: a larger one allows more."""
         out = ctypes.c_uint64()
         _raise(self._lib.mkv_kv8_workspace_size(self._h, ctypes.byref(out)))
         return out.value
