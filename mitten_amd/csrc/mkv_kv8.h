@@ -42,7 +42,10 @@ struct Kv8Pool : MetaRing {
   bool ws_used = false;
   // The last host arrays of each kind of call.
   StagedCache app_cache, gather_cache, decode_cache, extend_cache;
-  std::vector<int32_t> stage_tmp, owner;
+  std::vector<int32_t> stage_tmp;
+  // Per block, the last call of those that checked one that writes it, and the sequence.
+  std::vector<uint64_t> owner;
+  uint32_t calls = 0;
 };
 
 inline int64_t kv8_exp_plane(const Geom &g) { return g.nblocks * g.Hkv; }

@@ -522,28 +522,37 @@ static int stage_checked(Kv8Pool *p, StagedCache &c, const int32_t *h_q_lens, co
                            b, h_ids[i], i - h_indptr[b], (long long)g.nblocks);
     }
     if (write) {
-      // owner[block]: 1 + the sequence that writes it.
-      p->owner.assign((size_t)g.nblocks, 0);
+      // owner[block]: this call's number, then the sequence that writes the block. Entries of
+      // other calls count as none, so that a call costs what it names and not the pool.
+      if (p->owner.empty() || ++p->calls == 0) {
+        p->owner.assign((size_t)g.nblocks, 0);
+        p->calls = 1;
+      }
+      const uint64_t tag = (uint64_t)p->calls << 32;
+      auto writer = [&](uint32_t id) {  // the sequence, or -1
+        const uint64_t o = p->owner[id];
+        return o >> 32 == p->calls ? (int32_t)(uint32_t)o : -1;
+      };
       for (int32_t b = 0; b < B; b++) {
         const int32_t nq = qi[b + 1] - qi[b];
         if (nq == 0 || h_ctx[b] == 0) continue;
         for (int32_t j = (h_ctx[b] - nq) / kPageSize; j <= (h_ctx[b] - 1) / kPageSize; j++) {
-          int32_t &o = p->owner[h_ids[h_indptr[b] + j]];
-          if (o)
-            return set_error(MKV_ERR_INVALID_ARGUMENT, "block %u would be written twice (sequences %d and %d)",
-                             h_ids[h_indptr[b] + j], o - 1, b);
-          o = b + 1;
+          const uint32_t id = h_ids[h_indptr[b] + j];
+          if (writer(id) >= 0)
+            return set_error(MKV_ERR_INVALID_ARGUMENT, "block %u would be written twice (sequences %d and %d)", id,
+                             writer(id), b);
+          p->owner[id] = tag | (uint32_t)b;
         }
       }
       for (int32_t b = 0; b < B; b++) {
         const uint32_t need = (uint32_t)(((int64_t)h_ctx[b] + kPageSize - 1) / kPageSize);
         const int32_t nq = qi[b + 1] - qi[b];
         for (uint32_t j = 0; j < need; j++) {
-          const int32_t o = p->owner[h_ids[h_indptr[b] + j]];
-          const bool own = nq && o == b + 1 && (int32_t)j >= (h_ctx[b] - nq) / kPageSize;
-          if (o && !own)
+          const int32_t o = writer(h_ids[h_indptr[b] + j]);
+          const bool own = nq && o == b && (int32_t)j >= (h_ctx[b] - nq) / kPageSize;
+          if (o >= 0 && !own)
             return set_error(MKV_ERR_INVALID_ARGUMENT, "block %u is written by sequence %d and in another part (of sequence %d)",
-                             h_ids[h_indptr[b] + j], o - 1, b);
+                             h_ids[h_indptr[b] + j], o, b);
         }
       }
     }
