@@ -154,23 +154,27 @@ class DeviceKv8Pool:
         return out.value
 
     def _view(self, ptr, shape, typestr):
+        if not self._h:
+            raise _bad("the pool is closed")
+
         class _View:
             pass
 
         view = _View()
-        view.pool = self  # the tensor holds the view: the pool is not freed under it
+        view.pool = self  # the tensor holds the view: the pool lives as long, but for a close()
         view.__cuda_array_interface__ = {"shape": shape, "typestr": typestr, "data": (ptr, False), "version": 3,
                                          "strides": None}
         return _torch().as_tensor(view, device=f"cuda:{self.device}")
 
     def tensor(self):
         """Zero-copy uint8 view of the tiles, [L, 2, num_blocks, Hkv, 16 * D] (bytes in
-        tile order; `.view(torch.float8_e4m3fn)` for their values)."""
+        tile order; `.view(torch.float8_e4m3fn)` for their values). It keeps the pool
+        alive; after close() it must not be read."""
         d = self.desc
         return self._view(self.tiles_ptr, (d.num_layers, 2, int(d.num_blocks), d.num_kv_heads, 16 * d.head_dim), "|u1")
 
     def exponents(self):
-        """Zero-copy int8 view of the exponents, [L, 2, num_blocks, Hkv]."""
+        """Zero-copy int8 view of the exponents, [L, 2, num_blocks, Hkv], as tensor()."""
         d = self.desc
         return self._view(self.exponents_ptr, (d.num_layers, 2, int(d.num_blocks), d.num_kv_heads), "|i1")
 
