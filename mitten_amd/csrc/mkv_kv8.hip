@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KV8_EU
 // ---- read-back -------------------------------------------------------------------
 
 // grid (waves of (block, K | V, head) / 4, sequence); lane as in the tile order. Bound by
-// memory: 64 sequences of 1 to 8k tokens, 971 MB in 196 us, 4.95 TB/s (a copy reaches
+// memory: 64 sequences of 1 to 8k tokens, 973 MB in 196 us, 4.95 TB/s (a copy reaches
 // 5.13). Loads past the caches, plain stores: 235 us with stores past them too.
 template <int D, bool F32>
 __global__ void __launch_bounds__(256) kv8_gather_kernel(Kv8Args a, int32_t max_ctx, uint8_t *__restrict__ out_k,

@@ -344,9 +344,10 @@ __device__ __forceinline__ void kv8_store(const Kv8State<D, SUMS> &st, int E, in
 //     two partials per piece, which a second launch merges;
 //   seq: one workgroup of 8 waves (4 at head_dim 256) per (sequence, KV head, 16 query
 //     heads), their states merged in LDS; one launch.
-// What bounds it: memory for many long contexts (64 of 1 to 8k tokens, 280 MB: 54 us
+// What bounds it: memory for many long contexts (64 of 1 to 8k tokens, 286 MB: 55 us
 // for the split kernel, 5.2 TB/s, and 5 for the merge), the chain of dependent loads for
-// few or short ones (lengths, ids, tiles, partials: 8 us at the least, 12.7 split).
+// few or short ones (lengths, ids, tiles, partials: 9 us at the least, one of 8k tokens split
+// 11 and a merge of 4).
 // ===========================================================================
 
 constexpr int kSplitSeqs = 4096;   // sequences of one split launch (their scan stands in LDS)
@@ -854,14 +855,17 @@ kv8_decode_seq_kernel(Kv8Args a, Kv8Dec dc) {
 // pairs in memory order. A workgroup of W waves takes 16 * RT * W of them, RT groups
 // of 16 rows a wave, and streams the keys they see, 32 a step. A tile's bytes are
 // converted once, on the way into LDS (K bf16 with its exponent, V f16), and lie
-// there in operand order: 16 bytes a lane, contiguous, no bank conflicts either way.
+// there in operand order: 16 bytes a lane, contiguous, for all reads and for K's stores. V's
+// stores are 8 bytes a lane at a stride of 16, one block's half of an operand: half the banks
+// at a time (the SQ_LDS_BANK_CONFLICT of these kernels, 4% of the busy cycles in long chunks).
 // An operand is read once for RT products: LDS gives 128 bytes a cycle and CU, so at
 // RT = 1 the reads of a step take as long as twice its products, at RT = 2 as long.
 // Loads run kKv8ExtRing - 1 steps ahead in registers (16 bytes a lane and 1 KiB of tile);
 // one barrier a step.
 // What bounds it: the matrix unit and the instructions around it. 8 chunks of 512 tokens
-// after 4k, 28 query heads on 4 KV heads of 128 dims, bf16: 256 GFLOP in 320 us (800
-// TFLOP/s; 990 where the tiles fill the CUs evenly, here 896 of 128 rows on 512 places).
+// after 4k, 28 query heads on 4 KV heads of 128 dims, bf16: 256 GFLOP in 323 us (790
+// TFLOP/s). Tiles of 128 rows on 512 places, 4k tokens before them, of equal lengths: 896 take
+// 302 us (847 TFLOP/s), 1,024 308 (957), 1,536 464 (983), 544 233 (613).
 // With the next step's scores beside the weights; one after the other 420 us.
 // ===========================================================================
 
@@ -1441,7 +1445,7 @@ static int kv8_check_attn(const Kv8Pool *p, int32_t layer, float scale, uint32_t
 // ---- decode
 
 // kSplitWavesPerCu, and the steps of a piece, at least. Measured, 64 sequences of 1 to
-// 8k tokens (280 MB): 8 waves a CU 63.5 us, 7 the same, 12 (with a ring of 2, which
+// 8k tokens (286 MB): 8 waves a CU 63.5 us, 7 the same, 12 (with a ring of 2, which
 // their registers allow) 65.9, 16 73.0; one sequence of 8k: 4 steps 16.3 us, 2 the
 // same, 8 18.6.
 constexpr int kSplitMinSteps = 4;
@@ -1452,7 +1456,12 @@ constexpr int kSplitMinSteps = 4;
 // heads, seq / split in us: 8 sequences of 1,024 tokens 12.4 / 15.4, 1,536 15.5 / 15.7,
 // 2,048 17.6 / 16.2; 64 of 1,024 16.8 / 26.8, 64 of 1 to 2,048 21.8 / 28.8, of 1 to
 // 3,200 29.1 / 35.3, all but one of 100 17.3 / 16.7 and 23.0 / 16.6; 256 of 512
-// 41.8 / 45.7, all but one of 100 34.8 / 26.8.
+// 41.8 / 45.7, all but one of 100 34.8 / 26.8. Those are bf16, three batches in turn; other
+// types and head dims follow the same steps. Of one batch, which stays in the caches: f32, 128
+// dims, 8 of 1,024 12.6 / 18.4, of 2,048 17.2 / 19.0; f32, 256 dims, 8 of 1,024 21.7 / 24.9, of
+// 1,536 28.4 / 25.1, 64 of 1,024 31.9 / 56.4; bf16, 64 dims, 8 of 1,536 9.7 / 15.3, of 2,048
+// 10.6 / 15.5, 256 of 512 26.3 / 33.7. (So 64 dims are split early.) The bound on the lengths
+// counts, not what a captured call finds.
 static int kv8_seq_steps(int64_t wgs, int cus) { return 2 * wgs < cus ? 6 : wgs <= 2 * cus ? 10 : 0; }
 
 // Up to kSplitSeqs sequences (any number for pieces = 0, the seq kernel).
@@ -1477,7 +1486,8 @@ static int launch_kv8_decode(const Kv8Pool *p, const Kv8Args &a, Kv8Dec &d, int6
 // The forms of the extend kernel: rows and waves of a workgroup, and what a step of 32
 // keys takes it in us, alone on a CU and beside a second one (0: none fits). Wide: an
 // LDS operand feeds two groups of rows where the registers allow it. Measured: 16
-// chunks of 5-24 tokens after 4-8k unsplit, and 8 of 512 after 4k.
+// chunks of 5-24 tokens after 4-8k unsplit, and 8 of 512 after 4k. (Every tile is priced by
+// the longest context; a cheaper form or cut by a few percent of this is not to be relied on.)
 struct Kv8ExtForm {
   const void *fn;
   int rows, waves;
