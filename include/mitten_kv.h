@@ -636,7 +636,8 @@ MKV_API int mkv_add_rms_norm(int device, const void *d_x, const void *d_residual
  * the device forms a sequence whose numbers do not fit is skipped and reported as
  * by mkv_extend_attention (its rows of o stay as they are); ctx 0 is a padding
  * sequence: nothing is written for it but zeros in its row of o. Rows behind the last
- * sequence stay as they are. */
+ * sequence stay as they are. d_block_ids NULL is an empty array: a sequence with tokens has
+ * a table too short then. */
 typedef struct mkv_kv8_pool mkv_kv8_pool;
 
 /* Bytes of the tiles and of the exponents. */

@@ -87,7 +87,7 @@ int kv8_stage(Kv8Pool *p, StagedCache &c, const int32_t *h_q_lens, const int32_t
 struct Kv8Args {
   uint8_t *k_tiles, *v_tiles;
   int8_t *k_exps, *v_exps;  // [blocks][Hkv]
-  const int32_t *q_indptr, *indptr, *ids, *ctx;
+  const int32_t *q_indptr, *indptr, *ids, *ctx;  // ids null: no table holds a block
   uint32_t *d_err;
   int64_t nblocks;
   int32_t B, Hq, Hkv, G, tokens;
@@ -113,7 +113,7 @@ __device__ __forceinline__ uint32_t kv8_seq(const Kv8Args &a, int b, int32_t max
   s.q0 = qi ? qi[b] : b;
   const int q1 = qi ? qi[b + 1] : b + (s.ctx > 0);  // (no indptr: one row each, none for padding)
   s.tab0 = ip[b];
-  const int64_t tabn = (int64_t)ip[b + 1] - s.tab0;
+  const int64_t tabn = a.ids ? (int64_t)ip[b + 1] - s.tab0 : 0;
   const int64_t n = (int64_t)q1 - s.q0;
   s.n = 0;
   if (n < 0 || s.q0 < 0 || q1 > a.tokens || s.ctx < 0 || n > s.ctx || s.ctx > max_ctx) return MKV_DEVERR_CTX;

@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(256) kv8_gather_kernel(Kv8Args a, int32_t max_
   const int ctx = ((const kv8_const_i32 *)a.ctx)[b];
   const kv8_const_i32 *ip = (const kv8_const_i32 *)a.indptr;
   const int tab0 = ip[b];
-  const int64_t tabn = (int64_t)ip[b + 1] - tab0;
+  const int64_t tabn = a.ids ? (int64_t)ip[b + 1] - tab0 : 0;
   // The token that the sequence starts at: the sum of the lengths before it (as
   // they are: a length that does not fit spoils its own sequence only).
   int64_t c0 = 0;
@@ -753,7 +753,7 @@ extern "C" int mkv_kv8_append(mkv_kv8_pool *pool, int32_t layer, const void *d_k
   int rc = kv8_check_layer(p, layer);
   if (rc || (rc = kv8_check_batch(num_seqs, num_tokens, max_q_len))) return rc;
   if (num_seqs == 0 || num_tokens == 0 || max_q_len == 0) return MKV_OK;
-  if (!d_k || !d_v || !d_q_indptr || !d_block_indptr || !d_block_ids || !d_ctx_lens)
+  if (!d_k || !d_v || !d_q_indptr || !d_block_indptr || !d_ctx_lens)
     return set_error(MKV_ERR_INVALID_ARGUMENT, "NULL device pointer");
   if (!aligned16(d_k) || !aligned16(d_v))
     return set_error(MKV_ERR_INVALID_ARGUMENT, "K/V rows must be 16-byte aligned");
@@ -809,7 +809,7 @@ extern "C" int mkv_kv8_qk_norm_rope_append(mkv_kv8_pool *pool, int32_t layer, co
     return set_error(MKV_ERR_INVALID_ARGUMENT, "eps must be finite and >= 0");
   if (!std::isfinite(rope_factor)) return set_error(MKV_ERR_INVALID_ARGUMENT, "rope_factor must be finite");
   if (num_seqs == 0 || num_tokens == 0 || max_q_len == 0) return MKV_OK;
-  if (!d_q || !d_k || !d_v || !d_q_out || !d_q_indptr || !d_block_indptr || !d_block_ids || !d_ctx_lens ||
+  if (!d_q || !d_k || !d_v || !d_q_out || !d_q_indptr || !d_block_indptr || !d_ctx_lens ||
       (norm && (!d_q_norm_w || !d_k_norm_w)) || (rotary_dim > 0 && !d_inv_freq))
     return set_error(MKV_ERR_INVALID_ARGUMENT, "NULL device pointer");
   if (!aligned16(d_q) || !aligned16(d_k) || !aligned16(d_v) || !aligned16(d_q_out) ||
@@ -900,7 +900,7 @@ extern "C" int mkv_kv8_gather(mkv_kv8_pool *pool, int32_t layer, const int32_t *
   if (num_seqs < 0 || num_seqs > 65535 || max_ctx_len < 0 || out_capacity_tokens < 0)
     return set_error(MKV_ERR_INVALID_ARGUMENT, "num_seqs outside [0, 65535], or negative sizes");
   if (num_seqs == 0 || max_ctx_len == 0) return MKV_OK;
-  if (!d_block_indptr || !d_block_ids || !d_ctx_lens || !d_out_k || !d_out_v)
+  if (!d_block_indptr || !d_ctx_lens || !d_out_k || !d_out_v)
     return set_error(MKV_ERR_INVALID_ARGUMENT, "NULL device pointer");
   if (!aligned16(d_out_k) || !aligned16(d_out_v))
     return set_error(MKV_ERR_INVALID_ARGUMENT, "gather outputs must be 16-byte aligned");

@@ -567,7 +567,7 @@ __device__ __forceinline__ void kv8_run(const Kv8Args &a, const Kv8Dec &dc, int 
 // Steps of sequence b, 0 for one that does not fit or is padding.
 __device__ __forceinline__ int kv8_steps(const Kv8Args &a, int b, int max_ctx, uint32_t &err) {
   const int ctx = a.ctx[b], tab0 = a.indptr[b];
-  const int64_t tabn = (int64_t)a.indptr[b + 1] - tab0;
+  const int64_t tabn = a.ids ? (int64_t)a.indptr[b + 1] - tab0 : 0;
   err = 0;
   if (ctx == 0) return 0;
   if (ctx < 0 || ctx > max_ctx) err = MKV_DEVERR_CTX;
@@ -1545,7 +1545,7 @@ extern "C" int mkv_kv8_decode_attention(mkv_kv8_pool *pool, int32_t layer, const
     return set_error(MKV_ERR_INVALID_ARGUMENT, "num_seqs outside [0, 65535], or max_ctx_len < 0");
   if (!d_k_new != !d_v_new) return set_error(MKV_ERR_INVALID_ARGUMENT, "give both new rows, or neither");
   if (num_seqs == 0) return MKV_OK;
-  if (!d_q || !d_o || !d_block_indptr || !d_block_ids || !d_ctx_lens)
+  if (!d_q || !d_o || !d_block_indptr || !d_ctx_lens)
     return set_error(MKV_ERR_INVALID_ARGUMENT, "NULL device pointer");
   if (!aligned16(d_q) || !aligned16(d_o) || !aligned16(d_k_new) || !aligned16(d_v_new))
     return set_error(MKV_ERR_INVALID_ARGUMENT, "q, o and the new rows must be 16-byte aligned");
@@ -1634,7 +1634,7 @@ extern "C" int mkv_kv8_extend_attention(mkv_kv8_pool *pool, int32_t layer, const
   if (num_seqs == 0 || num_tokens == 0 || max_q_len == 0) return MKV_OK;
   if (max_q_len > max_ctx_len)
     return set_error(MKV_ERR_INVALID_ARGUMENT, "max_q_len %d > max_ctx_len %d", max_q_len, max_ctx_len);
-  if (!d_q || !d_o || !d_q_indptr || !d_block_indptr || !d_block_ids || !d_ctx_lens)
+  if (!d_q || !d_o || !d_q_indptr || !d_block_indptr || !d_ctx_lens)
     return set_error(MKV_ERR_INVALID_ARGUMENT, "NULL device pointer");
   if (!aligned16(d_q) || !aligned16(d_o)) return set_error(MKV_ERR_INVALID_ARGUMENT, "q and o must be 16-byte aligned");
   const uint64_t on = (uint64_t)num_tokens * g.Hq * g.D * g.es;
